@@ -128,6 +128,53 @@ class RelayAttentionArgs(ctypes.Structure):
     ]
 
 
+class RelayCache(ctypes.Structure):
+    _fields_ = [
+        ("pages", _i64), ("kv_heads", _i64), ("head_dim", _i64), ("page_size", _i64),
+        ("pool", _vp),
+    ]
+
+
+class RelayCacheAppendArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", RelayCache),
+        ("n_seq", _i64), ("tokens", _i64), ("table_width", _i64), ("table_stride", _i64),
+        ("dtype", _i32),
+        ("k", _vp), ("v", _vp), ("k_stride", _i64 * 4), ("v_stride", _i64 * 4),
+        ("page_table", _vp), ("lengths", _vp), ("counts", _vp), ("new_lengths", _vp),
+    ]
+
+
+class RelayCacheReadArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", RelayCache),
+        ("n_seq", _i64), ("tokens", _i64), ("table_width", _i64), ("table_stride", _i64),
+        ("dtype", _i32),
+        ("page_table", _vp), ("lengths", _vp), ("start", _vp), ("k", _vp), ("v", _vp),
+    ]
+
+
+class RelayCacheAttentionArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", RelayCache),
+        ("n_seq", _i64), ("queries", _i64), ("heads", _i64), ("table_width", _i64), ("table_stride", _i64),
+        ("prefix_len", _i64), ("prefix_width", _i64),
+        ("dtype", _i32), ("scale", ctypes.c_float),
+        ("q", _vp), ("q_stride", _i64 * 4),
+        ("page_table", _vp), ("lengths", _vp), ("prefix_pages", _vp),
+        ("out", _vp), ("row_max", _vp), ("row_sum", _vp),
+    ]
+
+
+class RelayCachePagesArgs(ctypes.Structure):
+    _fields_ = [
+        ("cache", RelayCache),
+        ("n_seq", _i64), ("table_width", _i64), ("table_stride", _i64),
+        ("page_table", _vp), ("lengths", _vp), ("refs", _vp),
+        ("page_table_out", _vp), ("lengths_out", _vp), ("refs_out", _vp),
+    ]
+
+
 # (name, restype, argtypes) for every function in include/dbl_gdn2.h
 EXPORTS = [
     ("dbl_status_string", ctypes.c_char_p, [ctypes.c_int]),
@@ -163,6 +210,19 @@ EXPORTS = [
     ("dbl_gdn2_prefill_time_sharded", ctypes.c_int,
      [ctypes.POINTER(PrefillArgs), ctypes.c_int, ctypes.POINTER(ctypes.c_int), ctypes.POINTER(_vp), _i64,
       ctypes.POINTER(_vp), ctypes.POINTER(ctypes.c_size_t)]),
+    ("dbl_relay_cache_append", ctypes.c_int, [ctypes.POINTER(RelayCacheAppendArgs), _vp]),
+    ("dbl_relay_cache_read", ctypes.c_int, [ctypes.POINTER(RelayCacheReadArgs), _vp]),
+    ("dbl_relay_cache_attention_workspace_bytes", ctypes.c_size_t, [ctypes.POINTER(RelayCacheAttentionArgs)]),
+    ("dbl_relay_cache_attention", ctypes.c_int,
+     [ctypes.POINTER(RelayCacheAttentionArgs), _vp, ctypes.c_size_t, _vp]),
+    ("dbl_relay_cache_pages_workspace_bytes", ctypes.c_size_t, [_i64, _i64]),
+    ("dbl_relay_cache_release", ctypes.c_int, [ctypes.POINTER(RelayCachePagesArgs), _vp, _i64, _vp]),
+    ("dbl_relay_cache_fork", ctypes.c_int, [ctypes.POINTER(RelayCachePagesArgs), _vp, _vp, _i64, _vp]),
+    ("dbl_relay_cache_reserve", ctypes.c_int,
+     [ctypes.POINTER(RelayCachePagesArgs), _vp, _i64, _vp, _vp, ctypes.c_size_t, _vp]),
+    ("dbl_relay_cache_compact", ctypes.c_int,
+     [ctypes.POINTER(RelayCachePagesArgs), _vp, _vp, ctypes.c_size_t, _vp]),
+    ("dbl_relay_cache_copy_pages", ctypes.c_int, [ctypes.POINTER(RelayCache), _vp, _vp, _i64, _vp]),
 ]
 
 RELAY_NOALLOC_SCRATCH_BYTES = 16 << 20  # DBL_RELAY_NOALLOC_SCRATCH_BYTES

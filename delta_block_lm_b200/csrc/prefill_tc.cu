@@ -1102,5 +1102,9 @@ extern "C" int dbl_device_error(int* code) {
         return dbl::fail(DBL_ERR_INVALID_ARGUMENT,
                          "relay attention: a live row's document id lies outside [0, documents); its relay slots "
                          "were skipped");
+    if (host == 102)
+        return dbl::fail(DBL_ERR_INVALID_ARGUMENT,
+                         "relay cache: a token's page, or a page or sequence that a list names, does not exist; it was "
+                         "left out");
     return host ? dbl::fail(DBL_ERR_TIMEOUT, "a kernel gave up a bounded wait (site %d)", host) : DBL_OK;
 }

@@ -1,0 +1,257 @@
+"""The relay cache in 4 bits, over torch CUDA tensors: keys and values that grow by tokens, in pages
+that sequences share, copy and give back, and the attention that reads them.
+
+It serves where ``relay_merge_decode`` does, at 5 bits a value (codes and their group's scale and
+minimum) instead of 16, and without padding every sequence to one capacity.  The reference has no
+counterpart: its relay attention keeps dense keys and values.
+
+The state is four tensors that the caller owns:
+
+    pool        uint8 [pages, kv_heads, page_size / 16, 20 head_dim] (``relay_cache_pool``)
+    page_table  int32 [sequences, width]: each sequence's pages in order, -1 where it has none
+    lengths     int32 [sequences]: tokens held
+    refs        int32 [pages]: how many entries of the page table hold a page (0: free)
+
+The pool is written in place; calls that change the page table, lengths or refs return new tensors
+(``out=`` takes them to tensors of the caller, the arguments themselves included).  Nothing here
+waits for the device, so a serving loop can be captured into a CUDA graph.  A token whose page does
+not exist is left out and recorded for ``dbl_device_error`` (code 102).
+
+    relay_cache_reserve    pages for the next tokens, copy on write    relay_cache_fork     share a sequence's pages
+    relay_cache_append     write tokens                                relay_cache_release  give pages back
+    relay_cache_attention  attention of the newest tokens              relay_cache_compact  pages in use to the front
+    relay_cache_read       tokens back as values                       relay_cache_copy_pages
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+from typing import Optional
+
+import torch
+
+from . import _native as N
+from .kernels import _dtype_code, _ptr, _require_cuda, _stream
+
+TILE = 16  # tokens of one tile: page sizes are multiples of it
+
+
+def relay_cache_pool(pages: int, kv_heads: int, head_dim: int, page_size: int = 64, *, device="cuda") -> torch.Tensor:
+    """An empty pool (zeroed) of ``pages`` pages of ``page_size`` tokens (a multiple of 16)."""
+    if head_dim not in (64, 128):
+        raise ValueError(f"relay cache: head_dim must be 64 or 128, got {head_dim}")
+    if page_size <= 0 or page_size % TILE:
+        raise ValueError(f"relay cache: page_size must be a multiple of {TILE}, got {page_size}")
+    return torch.zeros((pages, kv_heads, page_size // TILE, 20 * head_dim), device=device, dtype=torch.uint8)
+
+
+def _cache(pool: torch.Tensor) -> N.RelayCache:
+    if pool.dtype != torch.uint8 or pool.dim() != 4 or not pool.is_contiguous() or pool.shape[3] not in (1280, 2560):
+        raise ValueError("relay cache: pool must be a contiguous uint8 [pages, kv_heads, page_size / 16, 20 head_dim]"
+                         f" with head_dim 64 or 128, got {pool.dtype} {list(pool.shape)}")
+    p, h, t, b = pool.shape
+    return N.RelayCache(p, h, b // 20, t * TILE, pool.data_ptr())
+
+
+def _ints(name: str, t: Optional[torch.Tensor], shape: tuple) -> Optional[torch.Tensor]:
+    if t is None:
+        return None
+    if tuple(t.shape) != shape:
+        raise ValueError(f"relay cache: {name} must be {list(shape)}, got {list(t.shape)}")
+    if t.dtype != torch.int32 or not t.is_contiguous():
+        t = t.to(torch.int32).contiguous()
+    return t
+
+
+def _list(name: str, t: torch.Tensor) -> torch.Tensor:
+    if t.dim() != 1:
+        raise ValueError(f"relay cache: {name} must be a list (one dimension), got {list(t.shape)}")
+    return _ints(name, t, tuple(t.shape))
+
+
+def relay_cache_append(pool, page_table, lengths, k, v, *, counts=None, out=None) -> torch.Tensor:
+    """Writes the tokens k, v [N, T, kv_heads, D] (f32 or bf16; any strides with unit innermost) after
+    the ``lengths`` [N] tokens that each sequence holds, and returns the new lengths.  ``counts`` [N]:
+    how many of the T tokens are real (ragged prompts).  The pages must have been reserved."""
+    dev = _require_cuda(pool, page_table, lengths, k, v, counts, out)
+    c = _cache(pool)
+    n, t = k.shape[:2] if k.dim() == 4 else (0, 0)
+    if k.dim() != 4 or tuple(k.shape[2:]) != (c.kv_heads, c.head_dim) or k.shape != v.shape:
+        raise ValueError(f"relay cache append: k and v must be [N,T,{c.kv_heads},{c.head_dim}], got {list(k.shape)} and "
+                         f"{list(v.shape)}")
+    if v.dtype != k.dtype:
+        raise ValueError("relay cache append: v must have the dtype of k")
+    if page_table.dim() != 2 or page_table.shape[0] != n:
+        raise ValueError(f"relay cache append: page_table must be [{n},width], got {list(page_table.shape)}")
+    page_table = _ints("page_table", page_table, tuple(page_table.shape))
+    lengths, counts = _ints("lengths", lengths, (n,)), _ints("counts", counts, (n,))
+    if t == 0 or n == 0:
+        return lengths.clone() if out is None else out.copy_(lengths)
+    if k.stride(3) != 1:
+        k = k.contiguous()
+    if v.stride(3) != 1:
+        v = v.contiguous()
+    with torch.cuda.device(dev):
+        new = torch.empty_like(lengths)
+        a = N.RelayCacheAppendArgs(c, n, t, page_table.shape[1], 0, _dtype_code(k), _ptr(k), _ptr(v), k.stride(),
+                                   v.stride(), _ptr(page_table), _ptr(lengths), _ptr(counts), _ptr(new))
+        N.check(N.lib().dbl_relay_cache_append(ctypes.byref(a), _stream(dev)))
+        return new if out is None else out.copy_(new)
+
+
+def relay_cache_read(pool, page_table, lengths, *, start=None, tokens: int, dtype=torch.bfloat16):
+    """Tokens start[n] .. start[n] + tokens - 1 of every sequence as the values that the cache holds:
+    (k, v) [N, tokens, kv_heads, D] in ``dtype`` (f32 or bf16); zeros at and past ``lengths``."""
+    dev = _require_cuda(pool, page_table, lengths, start)
+    c = _cache(pool)
+    if page_table.dim() != 2:
+        raise ValueError(f"relay cache read: page_table must be [N,width], got {list(page_table.shape)}")
+    n = page_table.shape[0]
+    page_table = _ints("page_table", page_table, tuple(page_table.shape))
+    lengths, start = _ints("lengths", lengths, (n,)), _ints("start", start, (n,))
+    with torch.cuda.device(dev):
+        k = torch.empty((n, tokens, c.kv_heads, c.head_dim), device=dev, dtype=dtype)
+        v = torch.empty_like(k)
+        a = N.RelayCacheReadArgs(c, n, tokens, page_table.shape[1], 0, _dtype_code(k), _ptr(page_table), _ptr(lengths),
+                                 _ptr(start), _ptr(k), _ptr(v))
+        if k.numel():
+            N.check(N.lib().dbl_relay_cache_read(ctypes.byref(a), _stream(dev)))
+    return k, v
+
+
+def relay_cache_attention(q, pool, page_table, lengths, *, prefix_pages=None, prefix_len: int = 0,
+                          scale: Optional[float] = None, out=None, workspace: Optional[torch.Tensor] = None):
+    """Attention of each sequence's newest tokens over [shared prefix ; own tokens].
+
+    q [N, heads, D], or [N, Tq, heads, D] for the last Tq tokens of each sequence, causal among
+    themselves; f32 or bf16, heads a multiple of the pool's kv heads.  ``lengths`` counts the queries'
+    own tokens (append first).  ``prefix_pages`` [width] names the pages of ``prefix_len`` tokens that
+    every sequence sees before its own.  Returns (o, row_max, row_sum) as ``relay_merge_decode``; a row
+    without keys gives o = 0 and (0, 1)."""
+    dev = _require_cuda(q, pool, page_table, lengths, prefix_pages, out, workspace)
+    c = _cache(pool)
+    if q.dim() not in (3, 4) or q.shape[-1] != c.head_dim:
+        raise ValueError(f"relay cache attention: q must be [N,heads,{c.head_dim}] or [N,Tq,heads,{c.head_dim}], got "
+                         f"{list(q.shape)}")
+    n, heads = q.shape[0], q.shape[-2]
+    tq = q.shape[1] if q.dim() == 4 else 1
+    if page_table.dim() != 2 or page_table.shape[0] != n:
+        raise ValueError(f"relay cache attention: page_table must be [{n},width], got {list(page_table.shape)}")
+    if prefix_len and (prefix_pages is None or prefix_pages.dim() != 1):
+        raise ValueError("relay cache attention: prefix_pages must be a list of pages")
+    page_table = _ints("page_table", page_table, tuple(page_table.shape))
+    lengths = _ints("lengths", lengths, (n,))
+    if prefix_len:
+        prefix_pages = _list("prefix_pages", prefix_pages)
+    if q.stride(-1) != 1:
+        q = q.contiguous()
+    if scale is None:
+        scale = 1.0 / math.sqrt(c.head_dim)
+    with torch.cuda.device(dev):
+        if out is None:
+            out = torch.empty(q.shape, device=dev, dtype=q.dtype)
+        elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+            raise ValueError("relay cache attention: out must be contiguous with the shape and dtype of q")
+        stats = torch.empty((2, *q.shape[:-1]), device=dev, dtype=torch.float32)
+        row_max, row_sum = stats
+        qs = q.stride() if q.dim() == 4 else (q.stride(0), 0, q.stride(1), 1)
+        a = N.RelayCacheAttentionArgs(c, n, tq, heads, page_table.shape[1], 0, prefix_len,
+                                      prefix_pages.shape[0] if prefix_len else 0, _dtype_code(q), scale, _ptr(q), qs,
+                                      _ptr(page_table), _ptr(lengths), _ptr(prefix_pages) if prefix_len else None,
+                                      _ptr(out), _ptr(row_max), _ptr(row_sum))
+        if q.numel():
+            need = N.lib().dbl_relay_cache_attention_workspace_bytes(ctypes.byref(a))
+            if workspace is None and need:
+                workspace = torch.zeros(need, device=dev, dtype=torch.uint8)
+            N.check(N.lib().dbl_relay_cache_attention(ctypes.byref(a), _ptr(workspace),
+                                                      workspace.numel() if workspace is not None else 0, _stream(dev)))
+    return out, row_max, row_sum
+
+
+def _pages(pool, page_table, lengths, refs, out, lists):
+    """(device, arguments, outputs) of a page operation; ``lengths`` None where it has none."""
+    dev = _require_cuda(pool, page_table, lengths, refs, *lists, *(out or ()))
+    c = _cache(pool)
+    if page_table.dim() != 2:
+        raise ValueError(f"relay cache: page_table must be [sequences,width], got {list(page_table.shape)}")
+    s, w = page_table.shape
+    state = [_ints("page_table", page_table, (s, w)), _ints("lengths", lengths, (s,)), _ints("refs", refs, (c.pages,))]
+    given = [t for t in state if t is not None]
+    if out is None:
+        after = [torch.empty_like(t) for t in given]
+    else:
+        after = list(out)
+        for t, o in zip(given, after):
+            if o.shape != t.shape or o.dtype != torch.int32 or not o.is_contiguous():
+                raise ValueError("relay cache: out must be contiguous int32 tensors shaped like the state")
+    into = after if lengths is not None else [after[0], None, after[1]]
+    a = N.RelayCachePagesArgs(c, s, w, 0, *(_ptr(t) for t in state), *(_ptr(t) for t in into))
+    return dev, a, tuple(after), state
+
+
+def _scratch(a, dev):
+    return torch.empty(N.lib().dbl_relay_cache_pages_workspace_bytes(a.cache.pages, a.n_seq), device=dev,
+                       dtype=torch.uint8)
+
+
+def relay_cache_release(pool, page_table, lengths, refs, sequences, *, out=None):
+    """Gives back the pages of ``sequences`` (a list of row numbers).  Returns (page_table, lengths, refs)."""
+    sequences = _list("sequences", sequences)
+    dev, a, after, _keep = _pages(pool, page_table, lengths, refs, out, (sequences,))
+    with torch.cuda.device(dev):
+        N.check(N.lib().dbl_relay_cache_release(ctypes.byref(a), _ptr(sequences), sequences.numel(), _stream(dev)))
+    return after
+
+
+def relay_cache_fork(pool, page_table, lengths, refs, parents, children, *, out=None):
+    """children[i] (an empty sequence, named once and no parent itself) continues from parents[i],
+    sharing its pages.  Returns (page_table, lengths, refs)."""
+    parents, children = _list("parents", parents), _list("children", children)
+    if parents.shape != children.shape:
+        raise ValueError("relay cache fork: parents and children must have the same length")
+    dev, a, after, _keep = _pages(pool, page_table, lengths, refs, out, (parents, children))
+    with torch.cuda.device(dev):
+        N.check(N.lib().dbl_relay_cache_fork(ctypes.byref(a), _ptr(parents), _ptr(children), parents.numel(),
+                                             _stream(dev)))
+    return after
+
+
+def relay_cache_reserve(pool, page_table, lengths, refs, tokens, *, out=None):
+    """Pages for the next ``tokens`` (a number, or a list of one for each sequence) tokens of every
+    sequence.  A page that others hold too is copied before it is written to.  Returns (page_table,
+    refs, missing): ``missing`` [1] is 0, or how many pages the pool lacks, and then nothing changes.
+    ``out``: (page_table, refs)."""
+    counts = None
+    if isinstance(tokens, torch.Tensor):
+        counts, tokens = _ints("tokens", tokens, tuple(lengths.shape)), 0
+    dev, a, after, _keep = _pages(pool, page_table, lengths, refs, None if out is None else (out[0], lengths, out[1]),
+                                  () if counts is None else (counts,))
+    with torch.cuda.device(dev):
+        missing = torch.empty(1, device=dev, dtype=torch.int32)
+        ws = _scratch(a, dev)
+        N.check(N.lib().dbl_relay_cache_reserve(ctypes.byref(a), _ptr(counts), tokens, _ptr(missing), _ptr(ws),
+                                                ws.numel(), _stream(dev)))
+    return after[0], after[2], missing
+
+
+def relay_cache_compact(pool, page_table, refs, *, out=None):
+    """Moves the pages in use to the front of the pool (in place) and renames them in the page table.
+    Returns (page_table, refs, used): pages 0 .. used - 1 are in use, the others free.  A shared
+    prefix's pages follow if they are a row of the page table."""
+    dev, a, after, _keep = _pages(pool, page_table, None, refs, out, ())
+    with torch.cuda.device(dev):
+        used = torch.empty(1, device=dev, dtype=torch.int32)
+        ws = _scratch(a, dev)
+        N.check(N.lib().dbl_relay_cache_compact(ctypes.byref(a), _ptr(used), _ptr(ws), ws.numel(), _stream(dev)))
+    return after[0], after[1], used
+
+
+def relay_cache_copy_pages(pool, src, dst) -> None:
+    """Copies page src[i] to page dst[i] (no page is both, none is written twice)."""
+    src, dst = _list("src", src), _list("dst", dst)
+    dev = _require_cuda(pool, src, dst)
+    if src.shape != dst.shape:
+        raise ValueError("relay cache copy: src and dst must have the same length")
+    c = _cache(pool)
+    with torch.cuda.device(dev):
+        N.check(N.lib().dbl_relay_cache_copy_pages(ctypes.byref(c), _ptr(src), _ptr(dst), src.numel(), _stream(dev)))

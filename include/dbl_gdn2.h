@@ -56,10 +56,12 @@ int dbl_abi_version(void);
  * lets the kernel run to completion (its outputs are then undefined).  The
  * tensor-core prefill also records code 100 when one of its fp16 MMA operands left fp16 range
  * (inputs far outside unit-norm keys and beta in [0, 1]; its outputs are then not valid), and
- * relay attention records code 101 when a live row's document id lies outside [0, documents).
+ * relay attention records code 101 when a live row's document id lies outside [0, documents); the
+ * relay cache records code 102 when a token's page, or a page or sequence that a list names, does
+ * not exist (the token or the list item is left out).
  * This call synchronises with the device, stores the code in *code (0 = none; code may be NULL),
  * clears the record and returns DBL_OK, DBL_ERR_UNSUPPORTED (code 100), DBL_ERR_INVALID_ARGUMENT
- * (code 101) or DBL_ERR_TIMEOUT.  No counterpart in the reference, whose kernels have no bounded
+ * (codes 101 and 102) or DBL_ERR_TIMEOUT.  No counterpart in the reference, whose kernels have no bounded
  * waits or range checks. */
 int dbl_device_error(int *code);
 
@@ -395,6 +397,129 @@ typedef struct {
 } dbl_relay_attention_args;
 
 int dbl_relay_attention_forward(const dbl_relay_attention_args *args, dbl_stream_t stream);
+
+/* =============================================================================================
+ * 6. Relay cache in 4 bits (serving).  No counterpart in the reference, whose relay attention keeps
+ * dense keys and values.
+ *
+ * A pool of pages holds the keys and values of many sequences.  A page holds page_size tokens (a
+ * multiple of 16) of every kv head as tiles of 16 tokens; a tile is 20 * head_dim bytes, with
+ * G = head_dim / 32 groups of 32 channels, two codes a byte (the lower one in the lower half):
+ *   0       8 D  key codes    [16 tokens][4 parts t][G groups j][8 codes i]             channel 32 j + 8 t + i
+ *   8 D     2 D  key groups   [16 tokens][G] (scale, minimum), bf16 each
+ *   10 D    8 D  value codes  [2 halves][8 parts g][8 tokens][G groups j][4 codes i]    channel 32 j + 4 g + i
+ *   18 D    2 D  value groups [16 tokens][G] (scale, minimum), bf16 each
+ * A channel's value is minimum + scale * code, where for the 32 values x of a group (f32 arithmetic)
+ *   minimum = min(x) rounded down to bf16,  scale = (max(x) - minimum) / 15 rounded up to bf16,
+ *   code    = the smallest c of 0 .. 15 with x - minimum <= (c + 1/2) scale;
+ * a range below 2^-100 has scale 0, and a range that is not finite makes the group NaN.
+ *
+ * The page table is int32 [sequences, table_width], rows table_stride elements apart (0 =
+ * table_width): the pages of a sequence in order, -1 where it has none.  lengths int32 [sequences]
+ * are the tokens held, refs int32 [pages] the table entries that hold each page.  They live on the
+ * device and no call waits for it, so a serving loop can be captured into a CUDA graph.
+ * ========================================================================================== */
+typedef struct {
+    int64_t pages, kv_heads, head_dim, page_size; /* head_dim 64 or 128                         */
+    void *pool;               /* u8 [pages, kv_heads, page_size / 16, 20 head_dim], 16-byte aligned */
+} dbl_relay_cache;
+
+/* Writes tokens t < counts[n] of k, v [n_seq, tokens, kv_heads, head_dim] (strides in elements,
+ * innermost 1) at positions lengths[n] + t of sequence n.  The pages must exist and be the
+ * sequence's own where it writes (dbl_relay_cache_reserve). */
+typedef struct {
+    dbl_relay_cache cache;
+    int64_t n_seq, tokens, table_width, table_stride;
+    int32_t dtype;                    /* dbl_dtype of k and v                                 */
+    const void *k, *v;
+    int64_t k_stride[4], v_stride[4];
+    const int32_t *page_table, *lengths;
+    const int32_t *counts;            /* optional [n_seq]; NULL = tokens                      */
+    int32_t *new_lengths;             /* optional [n_seq]: lengths + counts; not lengths itself */
+} dbl_relay_cache_append_args;
+
+int dbl_relay_cache_append(const dbl_relay_cache_append_args *args, dbl_stream_t stream);
+
+/* Reads tokens start[n] .. start[n] + tokens - 1 of every sequence back, as the values that the
+ * codes stand for; zeros at and past lengths[n].  k, v [n_seq, tokens, kv_heads, head_dim]
+ * contiguous, 16-byte aligned. */
+typedef struct {
+    dbl_relay_cache cache;
+    int64_t n_seq, tokens, table_width, table_stride;
+    int32_t dtype;                    /* dbl_dtype of k and v                                 */
+    const int32_t *page_table, *lengths;
+    const int32_t *start;             /* optional [n_seq]; NULL = 0                           */
+    void *k, *v;
+} dbl_relay_cache_read_args;
+
+int dbl_relay_cache_read(const dbl_relay_cache_read_args *args, dbl_stream_t stream);
+
+/* Attention of the last `queries` tokens of each sequence over a prefix that all sequences share
+ * (prefix_len tokens in the pages prefix_pages names) and the sequence's own lengths[n] tokens,
+ * which include the queries' own: query t sees own keys below lengths[n] - queries + t + 1.
+ * q [n_seq, queries, heads, head_dim] (strides in elements, innermost 1); head h reads kv head
+ * h / (heads / kv_heads).  out [n_seq, queries, heads, head_dim] in dtype and row_max, row_sum f32
+ * [n_seq, queries, heads] are contiguous; the statistics and the empty row are those of
+ * dbl_relay_merge_decode (o = 0, max = 0, sum = 1).
+ * The workspace (dbl_relay_cache_attention_workspace_bytes, 16-byte aligned; NULL where that is 0)
+ * must be zero before its first use; every call leaves its counters zero again.  Calls that overlap
+ * on the GPU must use distinct workspaces. */
+typedef struct {
+    dbl_relay_cache cache;
+    int64_t n_seq, queries, heads, table_width, table_stride, prefix_len, prefix_width;
+    int32_t dtype;                    /* dbl_dtype of q and out                               */
+    float scale;                      /* softmax scale (1/sqrt(head_dim))                     */
+    const void *q;
+    int64_t q_stride[4];
+    const int32_t *page_table, *lengths;
+    const int32_t *prefix_pages;      /* [prefix_width]; may be NULL when prefix_len is 0     */
+    void *out;
+    float *row_max, *row_sum;         /* optional                                             */
+} dbl_relay_cache_attention_args;
+
+size_t dbl_relay_cache_attention_workspace_bytes(const dbl_relay_cache_attention_args *args);
+int dbl_relay_cache_attention(const dbl_relay_cache_attention_args *args, void *workspace,
+                              size_t workspace_bytes, dbl_stream_t stream);
+
+/* Page operations.  The state after the call goes to the *_out arrays, laid out as the ones before
+ * it; they may be the same arrays.  Free pages are handed out lowest number first, in the order of
+ * sequences and slots. */
+typedef struct {
+    dbl_relay_cache cache;
+    int64_t n_seq, table_width, table_stride;
+    const int32_t *page_table, *lengths, *refs;
+    int32_t *page_table_out, *lengths_out, *refs_out;
+} dbl_relay_cache_pages_args;
+
+/* Scratch bytes of reserve and compact (16-byte aligned; need not be cleared). */
+size_t dbl_relay_cache_pages_workspace_bytes(int64_t pages, int64_t n_seq);
+
+/* Releases sequences: their rows become -1, their lengths 0, and a page is free (refs 0) once no
+ * entry holds it. */
+int dbl_relay_cache_release(const dbl_relay_cache_pages_args *args, const int32_t *sequences,
+                            int64_t count, dbl_stream_t stream);
+/* children[i] (an empty sequence, named once, not itself a parent) becomes a copy of parents[i]
+ * that shares its pages; pages reserved past the parent's length stay the parent's alone. */
+int dbl_relay_cache_fork(const dbl_relay_cache_pages_args *args, const int32_t *parents,
+                         const int32_t *children, int64_t count, dbl_stream_t stream);
+/* Gives every sequence the pages for its next counts[n] tokens (counts NULL: `tokens` each) and
+ * makes the page in which they begin its own: where others hold it too, its tiles that hold tokens
+ * are copied to a new page (if all holders of a page are about to write, the last of them keeps
+ * it).  lengths_out is not used.  *missing: 0, or, where the pool has too few free pages, how many
+ * are missing; then nothing is changed. */
+int dbl_relay_cache_reserve(const dbl_relay_cache_pages_args *args, const int32_t *counts,
+                            int64_t tokens, int32_t *missing, void *workspace,
+                            size_t workspace_bytes, dbl_stream_t stream);
+/* Moves the pages in use to the front of the pool, so that pages [0, *used) are in use and the rest
+ * free: the i-th page in use at or past *used goes to the i-th free page below it.  Every list of
+ * pages outside the table (a shared prefix's) must be a row of the table to follow.  lengths and
+ * lengths_out are not used. */
+int dbl_relay_cache_compact(const dbl_relay_cache_pages_args *args, int32_t *used, void *workspace,
+                            size_t workspace_bytes, dbl_stream_t stream);
+/* Copies page src[i] to page dst[i], i < count (lists on the device; no dst among the src, none
+ * twice). */
+int dbl_relay_cache_copy_pages(const dbl_relay_cache *cache, const int32_t *src, const int32_t *dst,
+                               int64_t count, dbl_stream_t stream);
 
 #ifdef __cplusplus
 }
