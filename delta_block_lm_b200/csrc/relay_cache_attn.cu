@@ -16,13 +16,14 @@
 //     subnormal code * 2^-24, with the code in the next 4 bits 16 times that, so one AND makes the
 //     operand register of two codes.  The powers of two go into q (keys) or the output (values).
 //     The products' sums drop what lies 24 bits below the largest operand exponent, and a
-//     subnormal's counts as 2^-14: that leaves about 17 bits, ample beside p in f16; where more are
-//     needed the codes are shifted to the top of the mantissa (code * 2^-18, 22 bits).
+//     subnormal's counts as 2^-14: that leaves about 17 bits, ample beside p in f16.  For f32 rows
+//     the keys' codes are shifted to the top of the mantissa (code * 2^-18, 22 bits) and the values'
+//     become normal numbers around zero (code - 8), so that long sums neither drop bits nor cancel.
 //   * q is held in f16 relative to a power of two of its own row (bf16 q: exact; f32 q: two f16
 //     parts, 22 bits), p scale in f16 relative to a power of two near the row's largest (f32: again
 //     two parts).  For bf16 the rounding of p scale, 2^-11, is kept off the values' mean: with r
 //     the rounded p scale, o = sum r (code - 7.5) + sum p (min + 7.5 scale), where sum r is one
-//     more product, with a row of ones.
+//     more product, with a row of ones (f32: sum r (code - 8) + sum p (min + 8 scale)).
 //   * the scores arrive with tokens in rows and have to leave with tokens along the product's
 //     inner dimension: movmatrix transposes the 8 x 8 blocks.
 // The running maximum is only raised when a score passes it by 8 (in powers of two), so a step
@@ -134,21 +135,27 @@ __device__ __forceinline__ float mult_for(float w) {
 }
 __device__ __forceinline__ float pow2_inverse(float x) { return __uint_as_float((254u << 23) - __float_as_uint(x)); }
 
-// The operand registers of the 8 codes of w, codes (0, 4), (1, 5), (2, 6), (3, 7), as f16 subnormals:
-// code * 2^-18 (PRECISE), or code * 2^-24 in registers 0 and 2 and code * 2^-20 in registers 1 and 3.
-template <bool PRECISE>
+// The operand registers of the 8 codes of w, codes (0, 4), (1, 5), (2, 6), (3, 7), and what they are
+// multiplied by to be the codes (kUnit of register i).
+enum class Codes { kLow, kHigh, kCentred };
+template <Codes C>
 __device__ __forceinline__ void code_operands(uint32_t w, uint32_t (&r)[4]) {
-    if constexpr (PRECISE) {
+    if constexpr (C == Codes::kHigh) {
         r[0] = (w << 6) & 0x03C003C0u, r[1] = (w << 2) & 0x03C003C0u;
         r[2] = (w >> 2) & 0x03C003C0u, r[3] = (w >> 6) & 0x03C003C0u;
     } else {
         r[0] = w & 0x000F000Fu, r[1] = w & 0x00F000F0u;
         r[2] = (w >> 8) & 0x000F000Fu, r[3] = (w >> 8) & 0x00F000F0u;
+        if constexpr (C == Codes::kCentred) {  // 1024 + x is the f16 with mantissa x; 1032 = 1024 + 8, 1152 = 1024 + 16 * 8
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r[i]) : "r"(r[i] | 0x64006400u), "r"(i & 1 ? 0xE480E480u : 0xE408E408u));
+        }
     }
 }
-template <bool PRECISE>
-constexpr float code_unit(int i) {  // what a register's operand is multiplied by to be the code
-    return PRECISE ? 262144.f : (i & 1) ? 1048576.f : 16777216.f;
+template <Codes C>
+constexpr float code_unit(int i) {
+    return C == Codes::kHigh ? 262144.f : (i & 1 ? 0.0625f : 1.f) * (C == Codes::kLow ? 16777216.f : 1.f);
 }
 
 template <int G>
@@ -235,7 +242,7 @@ __global__ void __launch_bounds__(W * 32) cache_attn_kernel(const AttnParams p) 
     constexpr int G = D / 32, R = 8 * NR;
     constexpr bool SPLIT = sizeof(T) == 4;
     constexpr int NP = SPLIT ? 2 : 1;  // f16 parts of q and of p
-    constexpr bool KX = SPLIT, VX = SPLIT;  // codes at the top of the mantissa
+    constexpr Codes KX = SPLIT ? Codes::kHigh : Codes::kLow, VX = SPLIT ? Codes::kCentred : Codes::kLow;
     extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     uint64_t* bar = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR) + warp * NS;
@@ -350,7 +357,7 @@ __global__ void __launch_bounds__(W * 32) cache_attn_kernel(const AttnParams p) 
         int e = (int)(__float_as_uint(top) >> 23) - 126;
         e = top == 0.f ? 0 : min(max(e, -90), 110);
         const float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
-        constexpr int unit = KX ? 18 : 24;
+        constexpr int unit = KX == Codes::kHigh ? 18 : 24;  // log2 of code_unit<KX>(0)
         const float fr = __uint_as_float((uint32_t)(127 - 14 + unit + e) << 23) * fscale;
         const float inv = __uint_as_float((uint32_t)(127 + 14 - unit - e) << 23);
         float sum[G];
@@ -574,7 +581,8 @@ __global__ void __launch_bounds__(W * 32) cache_attn_kernel(const AttnParams p) 
                     // a NaN group has a NaN minimum too; its scale must not meet the zeros of the row of ones
                     const float sa = fmaxf(group_scale(va[i].w[j]), 0.f), sb = fmaxf(group_scale(vb[i].w[j]), 0.f);
                     float ma = group_min(va[i].w[j]), mb = group_min(vb[i].w[j]);
-                    if constexpr (!SPLIT) ma = fmaf(7.5f, sa, ma), mb = fmaf(7.5f, sb, mb);
+                    constexpr float centre = SPLIT ? 8.f : 7.5f;
+                    ma = fmaf(centre, sa, ma), mb = fmaf(centre, sb, mb);
                     omin[nr][0][j] = fmaf(s[i][nr][0], ma, fmaf(s[i][nr][2], mb, omin[nr][0][j]));
                     omin[nr][1][j] = fmaf(s[i][nr][1], ma, fmaf(s[i][nr][3], mb, omin[nr][1][j]));
                     uint32_t b0[NP], b1[NP];
