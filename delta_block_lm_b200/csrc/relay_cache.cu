@@ -58,7 +58,7 @@ __device__ __forceinline__ uint32_t encode8(const float (&x)[8], uint32_t& word)
     uint32_t sb = (__float_as_uint(__fdiv_rn(span, 15.f)) + 0xFFFFu) & 0xFFFF0000u;
     if (span < 7.888609052e-31f) sb = 0;  // 2^-100
     if (bad) {
-        word = 0x7FFF7FFFu;
+        word = 0x7FFF0000u;  // scale 0, minimum NaN
         return 0;
     }
     word = (sb >> 16) | lb;

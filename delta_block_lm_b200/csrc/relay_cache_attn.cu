@@ -47,7 +47,9 @@ namespace {
 constexpr int W = 4;              // warps of a CTA
 constexpr int TS = 2;             // tiles of a step
 constexpr int STEP = TS * kCacheTile;
-constexpr int NS = 3;             // stages of a warp's ring
+constexpr int NS = 2;             // stages of a warp's ring
+constexpr int kHeld1 = 4, kHeld2 = 2;  // CTAs that an SM holds at NR = 1 and 2
+constexpr int kOverhead = 128;    // tokens
 constexpr int WIN = 32 / TS;      // steps whose page numbers the lanes of a warp hold
 constexpr int kCacheWaitFull = 40;  // wait-site code (dbl_device_error)
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
@@ -65,9 +67,11 @@ struct AttnParams {
     float *row_max, *row_sum;
     int N, Tq, H, group, prefix_len, prefix_width;
     float scale;
-    int tiles_pre, tiles_own;    // row tiles of a kv head over all sequences, of one sequence
-    int splits_pre, splits_own;  // ranges of tokens
-    int range_pre, range_own;    // tokens of a range
+    bool pre;         // this launch: the prefix, or the sequences' own tokens
+    int tiles;        // row tiles of a kv head: over all sequences, or of one sequence
+    int splits;       // ranges of tokens of the segment
+    int range;        // tokens of a range
+    int at, parts;    // first partial of the segment in a row, partials of a row
     float *part, *part_ml;       // [rows, splits, D], [rows, splits, 2]
     unsigned* counter;           // [rows]
     int* err;
@@ -79,6 +83,35 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The same from zero sums.
+__device__ __forceinline__ void mma_f16_zero(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                             uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+template <bool ZERO>
+__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+    if constexpr (ZERO)
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+            "{%10,%10,%10,%10};\n"
+            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+    else
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+            "{%0,%1,%2,%3};\n"
+            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t add_bf16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
@@ -158,6 +191,23 @@ constexpr float code_unit(int i) {
     return C == Codes::kHigh ? 262144.f : (i & 1 ? 0.0625f : 1.f) * (C == Codes::kLow ? 16777216.f : 1.f);
 }
 
+// The operand whose rows are the 2 G scales and minima of a tile's tokens (scale 0, minimum 0, scale 1,
+// ...) and whose inner dimension are its 16 tokens: registers 0 and 2 (rows 8 .. 15 are not used).
+template <int G>
+__device__ __forceinline__ void group_operands(const uint8_t* groups, int lane, uint32_t& a0, uint32_t& a2) {
+    if constexpr (G == 4) {  // a token's 8 numbers are a row of an 8 x 8 matrix
+        asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];"
+                     : "=r"(a0), "=r"(a2)
+                     : "r"(smem_u32addr(groups + (lane & 15) * 16)));
+    } else {
+        const int g = lane >> 2, t = lane & 3;
+        const uint4 x = *reinterpret_cast<const uint4*>(groups + t * 16), y = *reinterpret_cast<const uint4*>(groups + 64 + t * 16);
+        const uint32_t sel = g & 1 ? 0x7632u : 0x5410u;
+        a0 = g & 2 ? __byte_perm(x.y, x.w, sel) : __byte_perm(x.x, x.z, sel);
+        a2 = g & 2 ? __byte_perm(y.y, y.w, sel) : __byte_perm(y.x, y.z, sel);
+    }
+}
+
 template <int G>
 struct Words {  // the G words that a lane reads at once
     uint32_t w[G];
@@ -222,24 +272,30 @@ __device__ void merge_row(const AttnParams& p, int64_t row, int S) {
     }
 }
 
-template <int D, typename T, int NR>
+template <int D, typename T, int R>
 struct AttnLayout {
     static constexpr int TB = cache_tile_bytes(D), STAGE = TS * TB;
     static constexpr int RING = W * NS * STAGE;
-    static constexpr int ACC = W * 8 * NR * D * 4;  // the warps' sums, over the ring
+    static constexpr int ACC = W * R * D * 4;  // the warps' sums, over the ring
     static constexpr int OFF_BAR = RING > ACC ? RING : ACC;
     static constexpr int OFF_MASK = OFF_BAR + W * NS * 8;
     static constexpr int OFF_ML = OFF_MASK + W * NS * 4;
-    static constexpr int OFF_ROW = OFF_ML + W * 8 * NR * 8;
-    static constexpr int OFF_ERR = OFF_ROW + 8 * NR * 8;
+    static constexpr int OFF_ROW = OFF_ML + W * R * 8;
+    static constexpr int OFF_ERR = OFF_ROW + R * 8;
     static constexpr int BYTES = OFF_ERR + 16;
 };
 
-template <int D, typename T, int NR>
-__global__ void __launch_bounds__(W * 32) cache_attn_kernel(const AttnParams p) {
-    using L = AttnLayout<D, T, NR>;
+// NR groups of 8 columns; E = 2: a row in every column, E = 1 (up to 4 rows): in the even columns only,
+// which saves the arithmetic of the others (a lane holds two neighbouring columns of every product).
+template <int NR, int E>
+constexpr int rows_of_tile() { return NR * 4 * E; }
+
+template <int D, typename T, int NR, int E>
+__global__ void __launch_bounds__(W * 32, NR == 1 ? kHeld1 : kHeld2) cache_attn_kernel(const AttnParams p) {
+    constexpr int R = rows_of_tile<NR, E>();
+    using L = AttnLayout<D, T, R>;
     using At = TileAt<D>;
-    constexpr int G = D / 32, R = 8 * NR;
+    constexpr int G = D / 32;
     constexpr bool SPLIT = sizeof(T) == 4;
     constexpr int NP = SPLIT ? 2 : 1;  // f16 parts of q and of p
     constexpr Codes KX = SPLIT ? Codes::kHigh : Codes::kLow, VX = SPLIT ? Codes::kCentred : Codes::kLow;
@@ -254,16 +310,13 @@ __global__ void __launch_bounds__(W * 32) cache_attn_kernel(const AttnParams p) 
 
     // ---- the item
     const int TG = p.Tq * p.group;
+    const bool pre = p.pre;
     int item = blockIdx.x;
-    const int n_pre = p.splits_pre * p.tiles_pre * p.c.heads;
-    const bool pre = item < n_pre;
-    if (!pre) item -= n_pre;
-    const int rt = item % (pre ? p.tiles_pre : p.tiles_own);
-    item /= pre ? p.tiles_pre : p.tiles_own;
+    const int rt = item % p.tiles;
+    item /= p.tiles;
     const int h = item % p.c.heads;
     item /= p.c.heads;
-    const int split = pre ? item : item % p.splits_own;
-    const int seq = pre ? 0 : item / p.splits_own;
+    const int split = item % p.splits, seq = item / p.splits;
     const int rows = min(R, (pre ? p.N * TG : TG) - rt * R);
     // row r of the tile: sequence, query, head; the number of keys it sees in this segment
     auto row_of = [&](int r, int& n, int& q, int& hq) {
@@ -274,12 +327,12 @@ __global__ void __launch_bounds__(W * 32) cache_attn_kernel(const AttnParams p) 
         hq = h * p.group + x % p.group;
     };
     const int len = pre ? p.prefix_len : min(max(p.lengths[seq], 0), p.c.width * p.c.tiles * kCacheTile);
+    auto row_at = [&](int nr, int e) { return E == 2 ? 8 * nr + 2 * t + e : 4 * nr + t; };  // of the lane's column e
     auto limit_of = [&](int r) {
         if (r >= rows) return 0;
         return pre ? len : max(0, len - p.Tq + (rt * R + r) / p.group + 1);
     };
-    const int range = pre ? p.range_pre : p.range_own;
-    const int c0 = split * range, c1 = min(c0 + range, limit_of(rows - 1));  // later rows see more
+    const int c0 = split * p.range, c1 = min(c0 + p.range, limit_of(rows - 1));  // later rows see more
     const int all_see = limit_of(0);                                         // tokens below it need no mask
     const int steps = c1 > c0 ? (c1 - c0 + STEP - 1) / STEP : 0;
     const int mine = steps > warp ? (steps - warp + W - 1) / W : 0;
@@ -301,7 +354,7 @@ __global__ void __launch_bounds__(W * 32) cache_attn_kernel(const AttnParams p) 
         return page < p.c.pages ? page : -1;
     };
     int win = page_of(0), win_next = -1;
-    auto issue = [&](int step) {  // the warp's step'th
+    auto issue = [&](int step, int slot) {  // the warp's step'th
         if (step > 0 && step % WIN == 0) win = win_next;
         if (step % WIN == WIN / 2) win_next = page_of(step - step % WIN + WIN);
         const int page = __shfl_sync(0xffffffffu, win, (step % WIN) * TS + lane % TS);
@@ -309,7 +362,6 @@ __global__ void __launch_bounds__(W * 32) cache_attn_kernel(const AttnParams p) 
         const bool want = lane < TS && tl < tile_end, have = want && page >= 0;
         if (want && !have) atomicExch(p.err, kCacheErrorPage);
         const uint32_t m = __ballot_sync(0xffffffffu, have);
-        const int slot = step % NS;
         if (lane == 0) {
             smask[slot] = m;
             mbar_arrive_expect_tx(bar + slot, __popc(m) * L::TB);
@@ -320,20 +372,23 @@ __global__ void __launch_bounds__(W * 32) cache_attn_kernel(const AttnParams p) 
                       bar + slot);
     };
     int issued = 0;
-    for (; issued < min(NS, mine); ++issued) issue(issued);
+    for (; issued < min(NS, mine); ++issued) issue(issued, issued);
 
     // ---- q: column g of the products, channels 32 j + 8 t .. + 8 of each group j
     uint32_t qf[NR][NP][G][4];
+    // sums of q over the groups / f as three bf16 parts, in the odd places (the minima's) of the
+    // operand for the (scale, minimum) words: group t
+    uint32_t qm[NR][3];
     // the scale goes into f, which stays positive
     const float sign = p.scale > 0.f ? 1.f : p.scale < 0.f ? -1.f : 0.f;
     const float fscale = sign != 0.f ? fabsf(p.scale) * kLog2e : 1.f;
-    float qsum[NR][2][G], f[NR][2];  // of rows 2 t, 2 t + 1: sums of q over the groups / f; score = f * inner
+    float f[NR][E];  // of the columns 2 t, 2 t + 1: score = f * inner
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr) {
-        const int r = 8 * nr + g;
+        const int r = E == 2 ? 8 * nr + g : 4 * nr + g / 2;
         float x[G][8];
         float top = 0.f;
-        if (r < rows) {
+        if (r < rows && (E == 2 || g % 2 == 0)) {
             int n, q, hq;
             row_of(r, n, q, hq);
             const T* src = static_cast<const T*>(p.q) + n * p.qs[0] + q * p.qs[1] + hq * p.qs[2] + 8 * t;
@@ -360,15 +415,15 @@ __global__ void __launch_bounds__(W * 32) cache_attn_kernel(const AttnParams p) 
         constexpr int unit = KX == Codes::kHigh ? 18 : 24;  // log2 of code_unit<KX>(0)
         const float fr = __uint_as_float((uint32_t)(127 - 14 + unit + e) << 23) * fscale;
         const float inv = __uint_as_float((uint32_t)(127 + 14 - unit - e) << 23);
-        float sum[G];
+        float mine_sum = 0.f;
 #pragma unroll
         for (int j = 0; j < G; ++j) {
-            float s = 0.f;
+            float sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s += x[j][i];
-            s += __shfl_xor_sync(0xffffffffu, s, 1);
-            s += __shfl_xor_sync(0xffffffffu, s, 2);
-            sum[j] = s * inv;
+            for (int i = 0; i < 8; ++i) sum += x[j][i];
+            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+            if (t == j) mine_sum = sum * inv;
             // the operands of the two products of a group, in the order of code_operands
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -378,149 +433,168 @@ __global__ void __launch_bounds__(W * 32) cache_attn_kernel(const AttnParams p) 
             }
         }
 #pragma unroll
-        for (int e2 = 0; e2 < 2; ++e2) {
-            const int from = (2 * t + e2) * 4;
-            f[nr][e2] = __shfl_sync(0xffffffffu, fr, from);
-#pragma unroll
-            for (int j = 0; j < G; ++j) qsum[nr][e2][j] = __shfl_sync(0xffffffffu, sum[j], from);
+        for (int i = 0; i < 3; ++i) {
+            qm[nr][i] = pack_bf16x2(0.f, mine_sum);
+            mine_sum -= bf16_hi(qm[nr][i]);
         }
+#pragma unroll
+        for (int e2 = 0; e2 < E; ++e2) f[nr][e2] = __shfl_sync(0xffffffffu, fr, (2 * t + e2) * 4);
     }
 
     float acc[NR][G][2][4];  // [group][channels 4 g + 0, 1 | 2, 3]: (ch 0, row 2t), (0, 2t+1), (1, 2t), (1, 2t+1)
-    float omin[NR][2][G];    // sum p min of this lane's tokens
+    float omin[NR][E][G];    // f32: sum p (min + 8 scale) of this lane's tokens
+    float pacc[NR][4];       // bf16: sum p scale, sum p min: lanes g = 2 j, 2 j + 1 hold group j
     float racc[NR][4];       // sums of r: lanes g = j hold group j
-    float l[NR][2], top[NR][2], ref[NR][2];  // sums; largest inner score of the lane; the reference of p
-    float wtop[NR][2], mult[NR][2];          // largest p scale of the lane; r = p scale mult, a power of two
-    int lim[NR][2];
+    float l[NR][E], top[NR][E];      // sums; largest inner score of the lane
+    float ref[NR][E], bar_[NR][E];   // p = 2^(f inner - ref); the inner score at which ref is raised
+    float wtop[NR][E], mult[NR][E];  // largest p scale of the lane; r = p scale mult, a power of two
+    int lim[NR][E];
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr) {
 #pragma unroll
         for (int j = 0; j < G; ++j)
 #pragma unroll
             for (int i = 0; i < 8; ++i) acc[nr][j][i / 4][i % 4] = 0.f;
-        racc[nr][0] = racc[nr][1] = racc[nr][2] = racc[nr][3] = 0.f;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            l[nr][e] = wtop[nr][e] = 0.f;
+        for (int i = 0; i < 4; ++i) racc[nr][i] = pacc[nr][i] = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            l[nr][e] = wtop[nr][e] = ref[nr][e] = 0.f;
             mult[nr][e] = kMostMult;
-            top[nr][e] = ref[nr][e] = -INFINITY;
-            lim[nr][e] = limit_of(8 * nr + 2 * t + e);
+            top[nr][e] = bar_[nr][e] = -INFINITY;
+            lim[nr][e] = limit_of(row_at(nr, e));
 #pragma unroll
             for (int j = 0; j < G; ++j) omin[nr][e][j] = 0.f;
         }
     }
 
     // ---- the steps
-    int done = 0;
+    int done = 0, slot = 0;
+    uint32_t parity = 0;
     for (int it = 0; it < mine; ++it) {
-        const int slot = it % NS;
-        if (!__all_sync(0xffffffffu, mbar_wait(bar + slot, (uint32_t)(it / NS) & 1u, serr, kCacheWaitFull))) break;
+        if (!__all_sync(0xffffffffu, mbar_wait(bar + slot, parity, serr, kCacheWaitFull))) break;
         done = it + 1;
         const uint8_t* st = ring + slot * L::STAGE;
         const uint32_t have = smask[slot];
         const int tok0 = c0 + (it * W + warp) * STEP;
         const bool masked = tok0 + STEP > min(all_see, c1) || have != (1u << TS) - 1;
+        if (masked) {  // what the groups of tokens that are not there hold is not a number that may be used
+#pragma unroll
+            for (int i = 0; i < TS; ++i)
+                for (int w = lane; w < 2 * kCacheTile * G; w += 32) {
+                    const int tok = w / G % kCacheTile;
+                    if (!(have >> i & 1) || tok0 + i * kCacheTile + tok >= c1)
+                        *reinterpret_cast<uint32_t*>(const_cast<uint8_t*>(st) + i * L::TB +
+                                                     (w < kCacheTile * G ? At::key_group(tok, w % G) : At::value_group(tok, w % G))) = 0u;
+                }
+            fence_proxy_async_smem();  // the slot's next copy comes after these writes
+            __syncwarp();
+        }
 
-        float s[TS][NR][4];  // (token g, row 2t), (g, 2t+1), (g + 8, 2t), (g + 8, 2t+1); inner scores, then p
+        float s[TS][NR][2 * E];  // token g: columns 2t (, 2t + 1), then token g + 8; inner scores, then p
 #pragma unroll
         for (int i = 0; i < TS; ++i) {
             const uint8_t* tile = st + i * L::TB;
             const Words<G> ka = lds_words<G>(tile + At::key_word(g, t, 0)), kb = lds_words<G>(tile + At::key_word(g + 8, t, 0));
             const Words<G> pa = lds_words<G>(tile + At::key_group(g, 0)), pb = lds_words<G>(tile + At::key_group(g + 8, 0));
+            // sum_j min_j sum(q_j): the (scale, minimum) words of group t as they are
+            const uint32_t wa = *reinterpret_cast<const uint32_t*>(tile + At::key_group(g, t % G));
+            const uint32_t wb = *reinterpret_cast<const uint32_t*>(tile + At::key_group(g + 8, t % G));
 #pragma unroll
-            for (int nr = 0; nr < NR; ++nr) s[i][nr][0] = s[i][nr][1] = s[i][nr][2] = s[i][nr][3] = 0.f;
+            for (int nr = 0; nr < NR; ++nr) {
+                float c[4];
+                mma_bf16<true>(c, wa, wb, wa, wb, qm[nr][0], qm[nr][1]);
+                mma_bf16<false>(c, wa, wb, wa, wb, qm[nr][2], 0u);
+#pragma unroll
+                for (int e = 0; e < E; ++e) s[i][nr][e] = c[e], s[i][nr][E + e] = c[2 + e];
+            }
 #pragma unroll
             for (int j = 0; j < G; ++j) {
                 uint32_t a[4], b[4];
                 code_operands<KX>(ka.w[j], a);
                 code_operands<KX>(kb.w[j], b);
                 const float sa = group_scale(pa.w[j]), sb = group_scale(pb.w[j]);
-                const float ma = group_min(pa.w[j]), mb = group_min(pb.w[j]);
 #pragma unroll
                 for (int nr = 0; nr < NR; ++nr) {
-                    float c[4] = {};
-#pragma unroll
-                    for (int np = 0; np < NP; ++np) {
-                        const uint32_t* q = qf[nr][np][j];
+                    float c[4];
+                    const uint32_t* q = qf[nr][0][j];
+                    mma_f16_zero(c, a[0], b[0], a[1], b[1], q[0], q[1]);
+                    mma_f16(c, a[2], b[2], a[3], b[3], q[2], q[3]);
+                    if constexpr (SPLIT) {
+                        q = qf[nr][NP - 1][j];
                         mma_f16(c, a[0], b[0], a[1], b[1], q[0], q[1]);
                         mma_f16(c, a[2], b[2], a[3], b[3], q[2], q[3]);
                     }
-                    s[i][nr][0] = fmaf(sa, c[0], fmaf(ma, qsum[nr][0][j], s[i][nr][0]));
-                    s[i][nr][1] = fmaf(sa, c[1], fmaf(ma, qsum[nr][1][j], s[i][nr][1]));
-                    s[i][nr][2] = fmaf(sb, c[2], fmaf(mb, qsum[nr][0][j], s[i][nr][2]));
-                    s[i][nr][3] = fmaf(sb, c[3], fmaf(mb, qsum[nr][1][j], s[i][nr][3]));
+#pragma unroll
+                    for (int e = 0; e < E; ++e) {
+                        s[i][nr][e] = fmaf(sa, c[e], s[i][nr][e]);
+                        s[i][nr][E + e] = fmaf(sb, c[2 + e], s[i][nr][E + e]);
+                    }
                 }
             }
         }
-        // tokens that a row does not see, or that are not there (their scores may be anything)
+        // tokens that a row does not see, or that are not there
         if (masked) {
 #pragma unroll
             for (int i = 0; i < TS; ++i)
 #pragma unroll
                 for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int tok = tok0 + i * kCacheTile + g + 8 * (e >> 1);
-                        if (!(have >> i & 1) || tok >= min(lim[nr][e & 1], c1)) s[i][nr][e] = -INFINITY;
+                    for (int e = 0; e < 2 * E; ++e) {
+                        const int tok = tok0 + i * kCacheTile + g + 8 * (e / E);
+                        if (!(have >> i & 1) || tok >= min(lim[nr][e % E], c1)) s[i][nr][e] = -INFINITY;
                     }
         }
-        // values' groups, and each token's largest scale
-        Words<G> va[TS], vb[TS];
+        // a bound of each token's value scales: their sum
         float sa_top[TS], sb_top[TS];
 #pragma unroll
         for (int i = 0; i < TS; ++i) {
             const uint8_t* tile = st + i * L::TB;
-            va[i] = lds_words<G>(tile + At::value_group(g, 0));
-            vb[i] = lds_words<G>(tile + At::value_group(g + 8, 0));
-            if (masked) {
-                const int tok = tok0 + i * kCacheTile + g;
-                const bool in = have >> i & 1;
-#pragma unroll
-                for (int j = 0; j < G; ++j) {
-                    if (!in || tok >= c1) va[i].w[j] = 0;
-                    if (!in || tok + 8 >= c1) vb[i].w[j] = 0;
-                }
+            const Words<G> va = lds_words<G>(tile + At::value_group(g, 0)), vb = lds_words<G>(tile + At::value_group(g + 8, 0));
+            uint32_t a = add_bf16x2(va.w[0], va.w[1]), b = add_bf16x2(vb.w[0], vb.w[1]);
+            if constexpr (G == 4) {
+                a = add_bf16x2(a, add_bf16x2(va.w[2], va.w[3]));
+                b = add_bf16x2(b, add_bf16x2(vb.w[2], vb.w[3]));
             }
-            sa_top[i] = sb_top[i] = 0.f;
-#pragma unroll
-            for (int j = 0; j < G; ++j) {
-                sa_top[i] = fmaxf(sa_top[i], group_scale(va[i].w[j]));
-                sb_top[i] = fmaxf(sb_top[i], group_scale(vb[i].w[j]));
-            }
+            sa_top[i] = group_scale(a), sb_top[i] = group_scale(b);
         }
         bool raise = false;
 #pragma unroll
         for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
+            for (int e = 0; e < E; ++e) {
                 float m = top[nr][e];
 #pragma unroll
-                for (int i = 0; i < TS; ++i) m = fmaxf(m, fmaxf(s[i][nr][e], s[i][nr][e + 2]));
+                for (int i = 0; i < TS; ++i) m = fmaxf(m, fmaxf(s[i][nr][e], s[i][nr][E + e]));
                 top[nr][e] = m;
-                raise = raise || (m - ref[nr][e]) * f[nr][e] > kSlack || (ref[nr][e] == -INFINITY && m > -INFINITY);
+                raise = raise || m > bar_[nr][e];
             }
         if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
             for (int nr = 0; nr < NR; ++nr) {
-                float c[2], back[2], forth[2];
+                float c[E], back[E], forth[E];
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
+                for (int e = 0; e < E; ++e) {
                     const float m = over_g_max(top[nr][e]);
-                    c[e] = ref[nr][e] == -INFINITY ? 0.f : ex2((ref[nr][e] - m) * f[nr][e]);
-                    ref[nr][e] = m;
+                    const float to = m == -INFINITY ? 0.f : m * f[nr][e];
+                    c[e] = bar_[nr][e] == -INFINITY ? 0.f : ex2(ref[nr][e] - to);
+                    ref[nr][e] = to;
+                    bar_[nr][e] = m + kSlack / f[nr][e];
                     l[nr][e] *= c[e];
                     wtop[nr][e] *= c[e];
                     back[e] = pow2_inverse(mult[nr][e]);
                     forth[e] = mult[nr][e] = mult_for(over_g_max(wtop[nr][e]));
+                    if constexpr (SPLIT) {
 #pragma unroll
-                    for (int j = 0; j < G; ++j) omin[nr][e][j] *= c[e];
+                        for (int j = 0; j < G; ++j) omin[nr][e][j] *= c[e];
+                    }
+                    pacc[nr][e] *= c[e];
+#pragma unroll
+                    for (int j = 0; j < G; ++j)
+#pragma unroll
+                        for (int i = e; i < 8; i += 2) acc[nr][j][i / 4][i % 4] *= back[e] * c[e] * forth[e];
+                    racc[nr][e] *= back[e] * c[e] * forth[e];
                 }
-#pragma unroll
-                for (int j = 0; j < G; ++j)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) acc[nr][j][i / 4][i % 4] *= back[i & 1] * c[i & 1] * forth[i & 1];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) racc[nr][i] *= back[i] * c[i] * forth[i];
             }
         }
         // p, relative to ref
@@ -528,35 +602,32 @@ __global__ void __launch_bounds__(W * 32) cache_attn_kernel(const AttnParams p) 
 #pragma unroll
         for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const float base = ref[nr][e] == -INFINITY ? 0.f : -ref[nr][e] * f[nr][e];
+            for (int e = 0; e < E; ++e) {
                 float w = 0.f;
 #pragma unroll
                 for (int i = 0; i < TS; ++i) {
-                    s[i][nr][e] = ex2(fmaf(s[i][nr][e], f[nr][e], base));
-                    s[i][nr][e + 2] = ex2(fmaf(s[i][nr][e + 2], f[nr][e], base));
-                    l[nr][e] += s[i][nr][e] + s[i][nr][e + 2];
-                    w = fmaxf(w, fmaxf(s[i][nr][e] * sa_top[i], s[i][nr][e + 2] * sb_top[i]));
+                    s[i][nr][e] = ex2(fmaf(s[i][nr][e], f[nr][e], -ref[nr][e]));
+                    s[i][nr][E + e] = ex2(fmaf(s[i][nr][E + e], f[nr][e], -ref[nr][e]));
+                    l[nr][e] += s[i][nr][e] + s[i][nr][E + e];
+                    w = fmaxf(w, fmaxf(s[i][nr][e] * sa_top[i], s[i][nr][E + e] * sb_top[i]));
                 }
                 wtop[nr][e] = fmaxf(wtop[nr][e], w);
                 raise = raise || w * mult[nr][e] > kMostF16;
             }
         if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
-            for (int nr = 0; nr < NR; ++nr) {
-                float c[2];
+            for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
+                for (int e = 0; e < E; ++e) {
                     const float m = fminf(mult[nr][e], mult_for(over_g_max(wtop[nr][e])));
-                    c[e] = pow2_inverse(mult[nr][e]) * m;
+                    const float c = pow2_inverse(mult[nr][e]) * m;
                     mult[nr][e] = m;
+#pragma unroll
+                    for (int j = 0; j < G; ++j)
+#pragma unroll
+                        for (int i = e; i < 8; i += 2) acc[nr][j][i / 4][i % 4] *= c;
+                    racc[nr][e] *= c;
                 }
-#pragma unroll
-                for (int j = 0; j < G; ++j)
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) acc[nr][j][i / 4][i % 4] *= c[i & 1];
-                racc[nr][0] *= c[0], racc[nr][1] *= c[1];
-            }
         }
 #pragma unroll
         for (int i = 0; i < TS; ++i) {
@@ -572,42 +643,63 @@ __global__ void __launch_bounds__(W * 32) cache_attn_kernel(const AttnParams p) 
                     x[u][j + 1] = __byte_perm(w.w[j / 2], w.w[G / 2 + j / 2], 0x7632);
                 }
             }
+            const Words<G> va = lds_words<G>(tile + At::value_group(g, 0)), vb = lds_words<G>(tile + At::value_group(g + 8, 0));
+            if constexpr (!SPLIT) {  // p in two bf16 parts
+                uint32_t w0, w2;
+                group_operands<G>(tile + At::value_group(0, 0), lane, w0, w2);
 #pragma unroll
-            for (int nr = 0; nr < NR; ++nr) {
-                const float p0 = s[i][nr][0] * mult[nr][0], p1 = s[i][nr][1] * mult[nr][1];
-                const float p2 = s[i][nr][2] * mult[nr][0], p3 = s[i][nr][3] * mult[nr][1];
+                for (int nr = 0; nr < NR; ++nr) {
+                    float a0 = s[i][nr][0], a1 = E == 2 ? s[i][nr][E - 1] : 0.f, b0 = s[i][nr][E], b1 = E == 2 ? s[i][nr][2 * E - 1] : 0.f;
+                    const uint32_t ha = pack_bf16x2(a0, a1), hb = pack_bf16x2(b0, b1);
+                    mma_bf16<false>(pacc[nr], w0, 0u, w2, 0u, transpose8x8(ha), transpose8x8(hb));
+                    a0 -= bf16_lo(ha), b0 -= bf16_lo(hb);
+                    if constexpr (E == 2) a1 -= bf16_hi(ha), b1 -= bf16_hi(hb);
+                    mma_bf16<false>(pacc[nr], w0, 0u, w2, 0u, transpose8x8(pack_bf16x2(a0, a1)), transpose8x8(pack_bf16x2(b0, b1)));
+                }
+            }
+            float pm[NR][2 * E];
 #pragma unroll
-                for (int j = 0; j < G; ++j) {
-                    // a NaN group has a NaN minimum too; its scale must not meet the zeros of the row of ones
-                    const float sa = fmaxf(group_scale(va[i].w[j]), 0.f), sb = fmaxf(group_scale(vb[i].w[j]), 0.f);
-                    float ma = group_min(va[i].w[j]), mb = group_min(vb[i].w[j]);
-                    constexpr float centre = SPLIT ? 8.f : 7.5f;
-                    ma = fmaf(centre, sa, ma), mb = fmaf(centre, sb, mb);
-                    omin[nr][0][j] = fmaf(s[i][nr][0], ma, fmaf(s[i][nr][2], mb, omin[nr][0][j]));
-                    omin[nr][1][j] = fmaf(s[i][nr][1], ma, fmaf(s[i][nr][3], mb, omin[nr][1][j]));
+            for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+                for (int e = 0; e < 2 * E; ++e) pm[nr][e] = s[i][nr][e] * mult[nr][e % E];
+#pragma unroll
+            for (int j = 0; j < G; ++j) {
+                uint32_t y[4], z[4];
+                code_operands<VX>(x[0][j], y);
+                code_operands<VX>(x[1][j], z);
+                const float sa = group_scale(va.w[j]), sb = group_scale(vb.w[j]);
+                const uint32_t one = g == j ? kOnes : 0u;
+#pragma unroll
+                for (int nr = 0; nr < NR; ++nr) {
+                    if constexpr (SPLIT) {
+                        const float ma = fmaf(8.f, sa, group_min(va.w[j])), mb = fmaf(8.f, sb, group_min(vb.w[j]));
+#pragma unroll
+                        for (int e = 0; e < E; ++e)
+                            omin[nr][e][j] = fmaf(s[i][nr][e], ma, fmaf(s[i][nr][E + e], mb, omin[nr][e][j]));
+                    }
+                    const float r0 = pm[nr][0] * sa, r1 = E == 2 ? pm[nr][E - 1] * sa : 0.f;
+                    const float r2 = pm[nr][E] * sb, r3 = E == 2 ? pm[nr][2 * E - 1] * sb : 0.f;
                     uint32_t b0[NP], b1[NP];
                     if constexpr (SPLIT) {
-                        split_f16x2(p0 * sa, p1 * sa, b0[0], b0[NP - 1]);
-                        split_f16x2(p2 * sb, p3 * sb, b1[0], b1[NP - 1]);
+                        split_f16x2(r0, r1, b0[0], b0[NP - 1]);
+                        split_f16x2(r2, r3, b1[0], b1[NP - 1]);
                     } else {
-                        b0[0] = pack_f16x2(p0 * sa, p1 * sa);
-                        b1[0] = pack_f16x2(p2 * sb, p3 * sb);
+                        b0[0] = pack_f16x2(r0, r1);
+                        b1[0] = pack_f16x2(r2, r3);
                     }
-                    uint32_t y[4], z[4];
-                    code_operands<VX>(x[0][j], y);
-                    code_operands<VX>(x[1][j], z);
 #pragma unroll
                     for (int np = 0; np < NP; ++np) {
                         const uint32_t c0_ = transpose8x8(b0[np]), c1_ = transpose8x8(b1[np]);
                         mma_f16(acc[nr][j][0], y[0], y[1], z[0], z[1], c0_, c1_);
-                        if constexpr (!SPLIT) mma_f16(racc[nr], g == j ? kOnes : 0u, 0u, g == j ? kOnes : 0u, 0u, c0_, c1_);
+                        if constexpr (!SPLIT) mma_f16(racc[nr], one, 0u, one, 0u, c0_, c1_);
                         mma_f16(acc[nr][j][1], y[2], y[3], z[2], z[3], c0_, c1_);
                     }
                 }
             }
         }
         __syncwarp();  // the slot has been read
-        if (issued < mine) issue(issued), ++issued;
+        if (issued < mine) issue(issued, slot), ++issued;
+        if (++slot == NS) slot = 0, parity ^= 1u;
     }
     // A warp that gave up at a wait still owns the copies it issued: let them land first.
     for (int i = done; i < issued; ++i) mbar_drain(bar + i % NS, (uint32_t)(i / NS) & 1u);
@@ -619,20 +711,25 @@ __global__ void __launch_bounds__(W * 32) cache_attn_kernel(const AttnParams p) 
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-            const int r = 8 * nr + 2 * t + e;
-            const float m = over_g_max(top[nr][e]);
-            const float c = ref[nr][e] == -INFINITY ? 0.f : ex2((ref[nr][e] - m) * f[nr][e]);
+        for (int e = 0; e < E; ++e) {
+            const int r = row_at(nr, e);
+            const float m = over_g_max(top[nr][e]) * f[nr][e];  // -inf: nothing seen
+            const float c = m == -INFINITY ? 0.f : ex2(ref[nr][e] - m);
             const float sum = over_g_sum(l[nr][e]) * c;
             const float v = pow2_inverse(mult[nr][e]);
             float om[G], rs[G];
 #pragma unroll
             for (int j = 0; j < G; ++j) {
-                om[j] = over_g_sum(omin[nr][e][j]);
-                rs[j] = SPLIT ? 0.f : -7.5f * __shfl_sync(0xffffffffu, racc[nr][e], j * 4 + t);
+                if constexpr (SPLIT) {
+                    om[j] = over_g_sum(omin[nr][e][j]);
+                    rs[j] = 0.f;
+                } else {
+                    om[j] = fmaf(7.5f, __shfl_sync(0xffffffffu, pacc[nr][e], 8 * j + t), __shfl_sync(0xffffffffu, pacc[nr][e], 8 * j + 4 + t));
+                    rs[j] = -7.5f * __shfl_sync(0xffffffffu, racc[nr][e], 4 * j + t);
+                }
             }
             if (r < rows) {
-                if (g == 0) sml[warp * R + r] = make_float2(m == -INFINITY ? m : m * f[nr][e], sum);
+                if (g == 0) sml[warp * R + r] = make_float2(m, sum);
 #pragma unroll
                 for (int j = 0; j < G; ++j) {
                     float4 o;
@@ -652,7 +749,7 @@ __global__ void __launch_bounds__(W * 32) cache_attn_kernel(const AttnParams p) 
     __syncthreads();
 
     // ---- the CTA's sums: the output, or a partial
-    const int S = p.splits_pre + p.splits_own, at = pre ? split : p.splits_pre + split;
+    const int S = p.parts, at = p.at + split;
     const float* all = reinterpret_cast<const float*>(smem);
     for (int i = threadIdx.x; i < rows * (D / 4); i += W * 32) {
         const int r = i / (D / 4), d = i % (D / 4) * 4;
@@ -706,42 +803,54 @@ __global__ void __launch_bounds__(W * 32) cache_attn_kernel(const AttnParams p) 
         if (last >> r & 1) merge_row<D, T>(p, srow[r], S);
 }
 
+struct Segment {
+    int nr, e, tiles, splits, range;
+    int64_t grid;
+};
 struct Plan {
-    int nr, tiles_pre, tiles_own, splits_pre, splits_own, range_pre, range_own;
-    int64_t rows, grid;
+    Segment own, pre;
+    int64_t rows;
+    int parts;
     size_t off_ml, off_cnt, bytes;
 };
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// A segment of `tokens` tokens that `rows` rows of a kv head share, `items` times.
+Segment segment_of(int64_t rows, int64_t items, int64_t tokens, bool bf16) {
+    Segment s{};
+    s.e = rows <= 4 ? 1 : 2;
+    s.nr = bf16 && rows > 8 ? 2 : 1;
+    s.tiles = (int)ceil_div(rows, 4 * s.e * s.nr);
+    items *= s.tiles;
+    // The cut that takes the fewest tokens one after another: rounds of CTAs that the GPU holds at a
+    // time, each the tokens of a range and a start and end that cost about as much as kOverhead.
+    const int64_t held = 148 * (s.nr == 2 ? kHeld2 : kHeld1), unit = W * STEP;
+    int64_t best = -1;
+    for (int64_t n = 1; n <= ceil_div(tokens, unit) && (n == 1 || items * n <= 4 * held); ++n) {
+        const int64_t range = ceil_div(ceil_div(tokens, n), unit) * unit, splits = ceil_div(tokens, range);
+        const int64_t cost = ceil_div(items * splits, held) * (range + kOverhead);
+        if (best < 0 || cost < best) {
+            best = cost;
+            s.range = (int)range;
+            s.splits = (int)splits;
+        }
+    }
+    s.grid = items * s.splits;
+    return s;
+}
+
 Plan plan_of(const dbl_relay_cache_attention_args* a) {
     Plan L{};
-    const int64_t G = a->heads / a->cache.kv_heads, TG = a->queries * G, H = a->cache.kv_heads, N = a->n_seq;
-    const int64_t max_own = a->table_width * a->cache.page_size;
-    L.nr = a->dtype == DBL_BF16 && (TG > 8 || (a->prefix_len > 0 && N * TG > 8)) ? 2 : 1;
-    const int64_t R = 8 * L.nr;
-    L.tiles_own = (int)ceil_div(TG, R);
-    L.tiles_pre = a->prefix_len > 0 ? (int)ceil_div(N * TG, R) : 0;
-    // CTAs enough for every SM to hold four, twice over; ranges of at least 256 tokens
-    const int64_t want = 148 * 8;
-    auto cut = [&](int64_t items, int64_t tokens, int& splits, int& range) {
-        int64_t s = ceil_div(want, items);
-        if (s > ceil_div(tokens, 256)) s = ceil_div(tokens, 256);
-        if (s < 1) s = 1;
-        int64_t r = ceil_div(ceil_div(tokens, s), W * STEP) * W * STEP;
-        if (r < W * STEP) r = W * STEP;
-        range = (int)r;
-        splits = (int)ceil_div(tokens, r);
-        if (splits < 1) splits = 1;
-    };
-    cut(N * H * L.tiles_own, max_own, L.splits_own, L.range_own);
-    if (L.tiles_pre) cut(H * L.tiles_pre, a->prefix_len, L.splits_pre, L.range_pre);
+    const int64_t TG = a->queries * (a->heads / a->cache.kv_heads), H = a->cache.kv_heads, N = a->n_seq;
+    const bool bf16 = a->dtype == DBL_BF16;
+    L.own = segment_of(TG, N * H, a->table_width * a->cache.page_size, bf16);
+    if (a->prefix_len > 0) L.pre = segment_of(N * TG, H, a->prefix_len, bf16);
     L.rows = N * a->queries * a->heads;
-    L.grid = (int64_t)L.splits_pre * L.tiles_pre * H + (int64_t)L.splits_own * L.tiles_own * H * N;
-    const int64_t S = L.splits_pre + L.splits_own;
-    if (S > 1) {
-        L.off_ml = (size_t)(L.rows * S * a->cache.head_dim) * 4;
-        L.off_cnt = L.off_ml + (size_t)(L.rows * S) * 8;
+    L.parts = L.pre.splits + L.own.splits;
+    if (L.parts > 1) {
+        L.off_ml = (size_t)(L.rows * L.parts * a->cache.head_dim) * 4;
+        L.off_cnt = L.off_ml + (size_t)(L.rows * L.parts) * 8;
         L.bytes = L.off_cnt + (size_t)L.rows * 4;
     }
     return L;
@@ -769,17 +878,31 @@ int attn_validate(const dbl_relay_cache_attention_args* a) {
     return DBL_OK;
 }
 
-template <int D, typename T, int NR>
+template <int D, typename T, int NR, int E>
 int launch_attn(const AttnParams& p, int64_t grid, cudaStream_t st) {
-    constexpr int smem = AttnLayout<D, T, NR>::BYTES;
+    constexpr int smem = AttnLayout<D, T, rows_of_tile<NR, E>()>::BYTES;
     static std::atomic<uint64_t> done{0};
     const int rc = once_per_device(done, [] {
-        return cuda_status(cudaFuncSetAttribute(cache_attn_kernel<D, T, NR>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
-                           "relay cache attention: cudaFuncSetAttribute");
+        return cuda_status(
+            cudaFuncSetAttribute(cache_attn_kernel<D, T, NR, E>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
+            "relay cache attention: cudaFuncSetAttribute");
     });
     if (rc != DBL_OK) return rc;
-    cache_attn_kernel<D, T, NR><<<(unsigned)grid, W * 32, smem, st>>>(p);
+    cache_attn_kernel<D, T, NR, E><<<(unsigned)grid, W * 32, smem, st>>>(p);
     return launch_status("cache_attn_kernel");
+}
+
+template <int D>
+int launch_segment(AttnParams p, const Segment& s, bool pre, int at, bool bf16, cudaStream_t st) {
+    p.pre = pre;
+    p.tiles = s.tiles;
+    p.splits = s.splits;
+    p.range = s.range;
+    p.at = at;
+    if (!bf16) return s.e == 1 ? launch_attn<D, float, 1, 1>(p, s.grid, st) : launch_attn<D, float, 1, 2>(p, s.grid, st);
+    if (s.nr == 2) return launch_attn<D, __nv_bfloat16, 2, 2>(p, s.grid, st);
+    return s.e == 1 ? launch_attn<D, __nv_bfloat16, 1, 1>(p, s.grid, st)
+                    : launch_attn<D, __nv_bfloat16, 1, 2>(p, s.grid, st);
 }
 
 }  // namespace
@@ -803,7 +926,7 @@ extern "C" int dbl_relay_cache_attention(const dbl_relay_cache_attention_args* a
     resolve_strides(a->q_stride, dims, 4, qs);
     if (qs[3] != 1) return fail(DBL_ERR_INVALID_ARGUMENT, "relay cache attention: the innermost stride of q must be 1");
     const Plan L = plan_of(a);
-    if (L.grid > 0x7fffffff) return fail(DBL_ERR_UNSUPPORTED, "relay cache attention: grid too large");
+    if (L.own.grid > 0x7fffffff || L.pre.grid > 0x7fffffff) return fail(DBL_ERR_UNSUPPORTED, "relay cache attention: grid too large");
     if (L.bytes && (!workspace || workspace_bytes < L.bytes))
         return fail(DBL_ERR_WORKSPACE, "relay cache attention: workspace of %zu bytes required (got %zu)", L.bytes,
                     workspace_bytes);
@@ -825,12 +948,7 @@ extern "C" int dbl_relay_cache_attention(const dbl_relay_cache_attention_args* a
     p.prefix_len = (int)a->prefix_len;
     p.prefix_width = (int)a->prefix_width;
     p.scale = a->scale;
-    p.tiles_pre = L.tiles_pre;
-    p.tiles_own = L.tiles_own;
-    p.splits_pre = L.splits_pre;
-    p.splits_own = L.splits_own;
-    p.range_pre = L.range_pre;
-    p.range_own = L.range_own;
+    p.parts = L.parts;
     uint8_t* ws = static_cast<uint8_t*>(workspace);
     p.part = reinterpret_cast<float*>(ws);
     p.part_ml = reinterpret_cast<float*>(ws + L.off_ml);
@@ -838,11 +956,11 @@ extern "C" int dbl_relay_cache_attention(const dbl_relay_cache_attention_args* a
     rc = device_error_record(&p.err);
     if (rc != DBL_OK) return rc;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    if (a->dtype == DBL_F32)
-        return D == 128 ? launch_attn<128, float, 1>(p, L.grid, st) : launch_attn<64, float, 1>(p, L.grid, st);
-    if (L.nr == 1)
-        return D == 128 ? launch_attn<128, __nv_bfloat16, 1>(p, L.grid, st)
-                        : launch_attn<64, __nv_bfloat16, 1>(p, L.grid, st);
-    return D == 128 ? launch_attn<128, __nv_bfloat16, 2>(p, L.grid, st)
-                    : launch_attn<64, __nv_bfloat16, 2>(p, L.grid, st);
+    const bool bf16 = a->dtype == DBL_BF16;
+    if (L.pre.splits) {
+        rc = D == 128 ? launch_segment<128>(p, L.pre, true, 0, bf16, st) : launch_segment<64>(p, L.pre, true, 0, bf16, st);
+        if (rc != DBL_OK) return rc;
+    }
+    return D == 128 ? launch_segment<128>(p, L.own, false, L.pre.splits, bf16, st)
+                    : launch_segment<64>(p, L.own, false, L.pre.splits, bf16, st);
 }

@@ -412,7 +412,8 @@ int dbl_relay_attention_forward(const dbl_relay_attention_args *args, dbl_stream
  * A channel's value is minimum + scale * code, where for the 32 values x of a group (f32 arithmetic)
  *   minimum = min(x) rounded down to bf16,  scale = (max(x) - minimum) / 15 rounded up to bf16,
  *   code    = the smallest c of 0 .. 15 with x - minimum <= (c + 1/2) scale;
- * a range below 2^-100 has scale 0, and a range that is not finite makes the group NaN.
+ * a range below 2^-100 has scale 0, and a range that is not finite makes the group NaN (scale 0,
+ * minimum NaN).
  *
  * The page table is int32 [sequences, table_width], rows table_stride elements apart (0 =
  * table_width): the pages of a sequence in order, -1 where it has none.  lengths int32 [sequences]
