@@ -220,7 +220,7 @@ int cache_validate(const dbl_relay_cache* c, const char* what) {
     if (c->page_size <= 0 || c->page_size % kCacheTile || c->page_size > 4096)
         return fail(DBL_ERR_UNSUPPORTED, "%s: page_size must be a multiple of 16 up to 4096 (got %lld)", what,
                     (long long)c->page_size);
-    if (c->pages > 0x7fffffff || c->kv_heads > 65535)
+    if (c->pages > 0x7fffffff || c->kv_heads > 65535 || c->pages * c->kv_heads > 0x7fffffff / (c->page_size / kCacheTile))
         return fail(DBL_ERR_UNSUPPORTED, "%s: sizes exceed 32-bit limits", what);
     if (!c->pool) return fail(DBL_ERR_INVALID_ARGUMENT, "%s: pool is required", what);
     if (!aligned(c->pool, 16)) return fail(DBL_ERR_INVALID_ARGUMENT, "%s: pool must be 16-byte aligned", what);

@@ -16,14 +16,16 @@
 //     subnormal code * 2^-24, with the code in the next 4 bits 16 times that, so one AND makes the
 //     operand register of two codes.  The powers of two go into q (keys) or the output (values).
 //     The products' sums drop what lies 24 bits below the largest operand exponent, and a
-//     subnormal's counts as 2^-14: that leaves about 17 bits, ample beside p in f16.  For f32 rows
-//     the keys' codes are shifted to the top of the mantissa (code * 2^-18, 22 bits) and the values'
-//     become normal numbers around zero (code - 8), so that long sums neither drop bits nor cancel.
+//     subnormal's counts as 2^-14, which leaves about 17 bits: for f32 rows the keys' codes are
+//     shifted to the top of the mantissa (code * 2^-18, 22 bits).  The values' codes become normal
+//     numbers around zero (code - 8), so that long sums neither drop bits nor cancel:
+//     o = sum r (code - 8) + sum p (min + 8 scale), r the rounded p scale.
 //   * q is held in f16 relative to a power of two of its own row (bf16 q: exact; f32 q: two f16
 //     parts, 22 bits), p scale in f16 relative to a power of two near the row's largest (f32: again
-//     two parts).  For bf16 the rounding of p scale, 2^-11, is kept off the values' mean: with r
-//     the rounded p scale, o = sum r (code - 7.5) + sum p (min + 7.5 scale), where sum r is one
-//     more product, with a row of ones (f32: sum r (code - 8) + sum p (min + 8 scale)).
+//     two parts).
+//   * the minima are operands as they lie in memory: a token's (scale, minimum) words are the bf16
+//     pairs of a row, met by zeros in the scales' places (keys), or read by a transposing ldmatrix
+//     (values, which also gives the sums of p scale); sum(q) and p are given in bf16 parts.
 //   * the scores arrive with tokens in rows and have to leave with tokens along the product's
 //     inner dimension: movmatrix transposes the 8 x 8 blocks.
 // The running maximum is only raised when a score passes it by 8 (in powers of two), so a step
@@ -52,11 +54,13 @@ constexpr int kHeld1 = 4, kHeld2 = 2;  // CTAs that an SM holds at NR = 1 and 2
 constexpr int kOverhead = 128;    // tokens
 constexpr int WIN = 32 / TS;      // steps whose page numbers the lanes of a warp hold
 constexpr int kCacheWaitFull = 40;  // wait-site code (dbl_device_error)
+constexpr int kNoPage = -1, kPast = -2;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+// Tokens of a segment: tile * tiles_inv has its exact quotient below 2^32 / 256 tiles.
+constexpr int64_t kMostTokens = (int64_t)1 << 27;
 constexpr float kSlack = 8.f;     // how far a score may pass the running maximum (powers of two)
 constexpr float kMostF16 = 60000.f;             // p scale mult stays below it
 constexpr float kMostMult = 1.2676506e30f;      // 2^100
-constexpr uint32_t kOnes = 0x3C003C00u;         // two f16 ones
 
 struct AttnParams {
     CacheView c;
@@ -67,6 +71,7 @@ struct AttnParams {
     float *row_max, *row_sum;
     int N, Tq, H, group, prefix_len, prefix_width;
     float scale;
+    uint32_t tiles_inv;  // ceil(2^32 / tiles of a page), 0 for 1: tile / tiles is the high word of a product
     bool pre;         // this launch: the prefix, or the sequences' own tokens
     int tiles;        // row tiles of a kv head: over all sequences, or of one sequence
     int splits;       // ranges of tokens of the segment
@@ -79,7 +84,7 @@ struct AttnParams {
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -87,26 +92,26 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
 // The same from zero sums.
 __device__ __forceinline__ void mma_f16_zero(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                              uint32_t b0, uint32_t b1) {
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
         : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
-template <bool ZERO>
-__device__ __forceinline__ void mma_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1) {
-    if constexpr (ZERO)
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-            "{%10,%10,%10,%10};\n"
-            : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
-            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
-    else
-        asm volatile(
-            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-            "{%0,%1,%2,%3};\n"
-            : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Inner dimension 8.
+__device__ __forceinline__ void mma_bf16_k8(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t b) {
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%0,%1,%2,%3};\n"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a0), "r"(a1), "r"(b));
+}
+__device__ __forceinline__ void mma_bf16_k8_zero(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t b) {
+    asm("mma.sync.aligned.m16n8k8.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5}, {%6}, {%7,%7,%7,%7};\n"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a0), "r"(a1), "r"(b), "f"(0.f));
 }
 __device__ __forceinline__ uint32_t add_bf16x2(uint32_t a, uint32_t b) {
     uint32_t r;
@@ -115,7 +120,7 @@ __device__ __forceinline__ uint32_t add_bf16x2(uint32_t a, uint32_t b) {
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
 __device__ __forceinline__ float ex2(float x) {
@@ -192,19 +197,19 @@ constexpr float code_unit(int i) {
 }
 
 // The operand whose rows are the 2 G scales and minima of a tile's tokens (scale 0, minimum 0, scale 1,
-// ...) and whose inner dimension are its 16 tokens: registers 0 and 2 (rows 8 .. 15 are not used).
+// ...) and whose inner dimension are its 16 tokens (rows 8 .. 15 hold anything).
 template <int G>
-__device__ __forceinline__ void group_operands(const uint8_t* groups, int lane, uint32_t& a0, uint32_t& a2) {
+__device__ __forceinline__ void group_operands(const uint8_t* groups, int lane, uint32_t (&a)[4]) {
     if constexpr (G == 4) {  // a token's 8 numbers are a row of an 8 x 8 matrix
-        asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0,%1}, [%2];"
-                     : "=r"(a0), "=r"(a2)
-                     : "r"(smem_u32addr(groups + (lane & 15) * 16)));
+        asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                     : "=r"(a[0]), "=r"(a[1]), "=r"(a[2]), "=r"(a[3])
+                     : "r"(smem_u32addr(groups + (lane & 7) * 16 + (lane & 16) * 8)));
     } else {
         const int g = lane >> 2, t = lane & 3;
         const uint4 x = *reinterpret_cast<const uint4*>(groups + t * 16), y = *reinterpret_cast<const uint4*>(groups + 64 + t * 16);
         const uint32_t sel = g & 1 ? 0x7632u : 0x5410u;
-        a0 = g & 2 ? __byte_perm(x.y, x.w, sel) : __byte_perm(x.x, x.z, sel);
-        a2 = g & 2 ? __byte_perm(y.y, y.w, sel) : __byte_perm(y.x, y.z, sel);
+        a[0] = a[1] = g & 2 ? __byte_perm(x.y, x.w, sel) : __byte_perm(x.x, x.z, sel);
+        a[2] = a[3] = g & 2 ? __byte_perm(y.y, y.w, sel) : __byte_perm(y.x, y.z, sel);
     }
 }
 
@@ -278,8 +283,7 @@ struct AttnLayout {
     static constexpr int RING = W * NS * STAGE;
     static constexpr int ACC = W * R * D * 4;  // the warps' sums, over the ring
     static constexpr int OFF_BAR = RING > ACC ? RING : ACC;
-    static constexpr int OFF_MASK = OFF_BAR + W * NS * 8;
-    static constexpr int OFF_ML = OFF_MASK + W * NS * 4;
+    static constexpr int OFF_ML = OFF_BAR + W * NS * 8;
     static constexpr int OFF_ROW = OFF_ML + W * R * 8;
     static constexpr int OFF_ERR = OFF_ROW + R * 8;
     static constexpr int BYTES = OFF_ERR + 16;
@@ -298,11 +302,10 @@ __global__ void __launch_bounds__(W * 32, NR == 1 ? kHeld1 : kHeld2) cache_attn_
     constexpr int G = D / 32;
     constexpr bool SPLIT = sizeof(T) == 4;
     constexpr int NP = SPLIT ? 2 : 1;  // f16 parts of q and of p
-    constexpr Codes KX = SPLIT ? Codes::kHigh : Codes::kLow, VX = SPLIT ? Codes::kCentred : Codes::kLow;
+    constexpr Codes KX = SPLIT ? Codes::kHigh : Codes::kLow, VX = Codes::kCentred;
     extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     uint64_t* bar = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR) + warp * NS;
-    uint32_t* smask = reinterpret_cast<uint32_t*>(smem + L::OFF_MASK) + warp * NS;
     float2* sml = reinterpret_cast<float2*>(smem + L::OFF_ML);      // [W][R]
     int64_t* srow = reinterpret_cast<int64_t*>(smem + L::OFF_ROW);  // output rows
     int* serr = reinterpret_cast<int*>(smem + L::OFF_ERR);
@@ -344,32 +347,46 @@ __global__ void __launch_bounds__(W * 32, NR == 1 ? kHeld1 : kHeld2) cache_attn_
     fence_mbar_init();
     __syncthreads();
 
-    // ---- copies.  Lane l holds the page of tile l % TS of the warp's step (window) + l / TS.
-    auto page_of = [&](int step) -> int {  // of this lane's tile, for the window that begins at `step`
+    // ---- copies.  Lane l holds the place of tile l % TS of the warp's step (window) + l / TS in the
+    // pool: kNoPage where the table has no page for it, kPast where the range has no such tile.
+    auto place_of = [&](int step) -> int {
         const int tl = c0 / kCacheTile + ((step + lane / TS) * W + warp) * TS + lane % TS;
-        if (tl >= tile_end) return -1;
-        if (!pre) return cache_page(p.c, seq, tl);
-        const int slot = tl / p.c.tiles;
-        const int page = slot < p.prefix_width ? p.prefix_pages[slot] : -1;
-        return page < p.c.pages ? page : -1;
+        if (tl >= tile_end) return kPast;
+        const int slot = p.tiles_inv ? (int)__umulhi((uint32_t)tl, p.tiles_inv) : tl;
+        int page = -1;
+        if (slot < (pre ? p.prefix_width : p.c.width))
+            page = pre ? p.prefix_pages[slot] : p.c.table[seq * p.c.table_stride + slot];
+        return page >= 0 && page < p.c.pages ? (page * p.c.heads + h) * p.c.tiles + tl - slot * p.c.tiles : kNoPage;
     };
-    int win = page_of(0), win_next = -1;
+    int win = place_of(0), win_next = kPast;
+    uint32_t have_of = 0;  // TS bits for each slot: the tiles that its copy brings
     auto issue = [&](int step, int slot) {  // the warp's step'th
         if (step > 0 && step % WIN == 0) win = win_next;
-        if (step % WIN == WIN / 2) win_next = page_of(step - step % WIN + WIN);
-        const int page = __shfl_sync(0xffffffffu, win, (step % WIN) * TS + lane % TS);
-        const int tl = c0 / kCacheTile + (step * W + warp) * TS + lane;
-        const bool want = lane < TS && tl < tile_end, have = want && page >= 0;
-        if (want && !have) atomicExch(p.err, kCacheErrorPage);
-        const uint32_t m = __ballot_sync(0xffffffffu, have);
+        if (step % WIN == WIN / 2) win_next = place_of(step - step % WIN + WIN);
+        int at[TS];
+        uint32_t m = 0;
+        bool row = true;  // the tiles are neighbours
+#pragma unroll
+        for (int i = 0; i < TS; ++i) {
+            at[i] = __shfl_sync(0xffffffffu, win, (step % WIN) * TS + i);
+            m |= (uint32_t)(at[i] >= 0) << i;
+            row = row && at[i] == at[0] + i;
+        }
+        have_of = (have_of & ~(((1u << TS) - 1) << (slot * TS))) | m << (slot * TS);
         if (lane == 0) {
-            smask[slot] = m;
+            uint8_t* dst = ring + slot * L::STAGE;
             mbar_arrive_expect_tx(bar + slot, __popc(m) * L::TB);
+            if (row && m) {
+                bulk_load(dst, p.c.pool + (int64_t)at[0] * L::TB, TS * L::TB, bar + slot);
+            } else {
+#pragma unroll
+                for (int i = 0; i < TS; ++i) {
+                    if (at[i] >= 0) bulk_load(dst + i * L::TB, p.c.pool + (int64_t)at[i] * L::TB, L::TB, bar + slot);
+                    if (at[i] == kNoPage) atomicExch(p.err, kCacheErrorPage);
+                }
+            }
         }
         __syncwarp();
-        if (have)
-            bulk_load(ring + slot * L::STAGE + lane * L::TB, cache_tile<D>(p.c, page, h, tl % p.c.tiles), L::TB,
-                      bar + slot);
     };
     int issued = 0;
     for (; issued < min(NS, mine); ++issued) issue(issued, issued);
@@ -444,7 +461,6 @@ __global__ void __launch_bounds__(W * 32, NR == 1 ? kHeld1 : kHeld2) cache_attn_
     float acc[NR][G][2][4];  // [group][channels 4 g + 0, 1 | 2, 3]: (ch 0, row 2t), (0, 2t+1), (1, 2t), (1, 2t+1)
     float omin[NR][E][G];    // f32: sum p (min + 8 scale) of this lane's tokens
     float pacc[NR][4];       // bf16: sum p scale, sum p min: lanes g = 2 j, 2 j + 1 hold group j
-    float racc[NR][4];       // sums of r: lanes g = j hold group j
     float l[NR][E], top[NR][E];      // sums; largest inner score of the lane
     float ref[NR][E], bar_[NR][E];   // p = 2^(f inner - ref); the inner score at which ref is raised
     float wtop[NR][E], mult[NR][E];  // largest p scale of the lane; r = p scale mult, a power of two
@@ -456,7 +472,7 @@ __global__ void __launch_bounds__(W * 32, NR == 1 ? kHeld1 : kHeld2) cache_attn_
 #pragma unroll
             for (int i = 0; i < 8; ++i) acc[nr][j][i / 4][i % 4] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) racc[nr][i] = pacc[nr][i] = 0.f;
+        for (int i = 0; i < 4; ++i) pacc[nr][i] = 0.f;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             l[nr][e] = wtop[nr][e] = ref[nr][e] = 0.f;
@@ -475,7 +491,7 @@ __global__ void __launch_bounds__(W * 32, NR == 1 ? kHeld1 : kHeld2) cache_attn_
         if (!__all_sync(0xffffffffu, mbar_wait(bar + slot, parity, serr, kCacheWaitFull))) break;
         done = it + 1;
         const uint8_t* st = ring + slot * L::STAGE;
-        const uint32_t have = smask[slot];
+        const uint32_t have = have_of >> (slot * TS) & ((1u << TS) - 1);
         const int tok0 = c0 + (it * W + warp) * STEP;
         const bool masked = tok0 + STEP > min(all_see, c1) || have != (1u << TS) - 1;
         if (masked) {  // what the groups of tokens that are not there hold is not a number that may be used
@@ -503,8 +519,9 @@ __global__ void __launch_bounds__(W * 32, NR == 1 ? kHeld1 : kHeld2) cache_attn_
 #pragma unroll
             for (int nr = 0; nr < NR; ++nr) {
                 float c[4];
-                mma_bf16<true>(c, wa, wb, wa, wb, qm[nr][0], qm[nr][1]);
-                mma_bf16<false>(c, wa, wb, wa, wb, qm[nr][2], 0u);
+                mma_bf16_k8_zero(c, wa, wb, qm[nr][0]);
+                mma_bf16_k8(c, wa, wb, qm[nr][1]);
+                mma_bf16_k8(c, wa, wb, qm[nr][2]);
 #pragma unroll
                 for (int e = 0; e < E; ++e) s[i][nr][e] = c[e], s[i][nr][E + e] = c[2 + e];
             }
@@ -593,7 +610,6 @@ __global__ void __launch_bounds__(W * 32, NR == 1 ? kHeld1 : kHeld2) cache_attn_
                     for (int j = 0; j < G; ++j)
 #pragma unroll
                         for (int i = e; i < 8; i += 2) acc[nr][j][i / 4][i % 4] *= back[e] * c[e] * forth[e];
-                    racc[nr][e] *= back[e] * c[e] * forth[e];
                 }
             }
         }
@@ -626,7 +642,6 @@ __global__ void __launch_bounds__(W * 32, NR == 1 ? kHeld1 : kHeld2) cache_attn_
                     for (int j = 0; j < G; ++j)
 #pragma unroll
                         for (int i = e; i < 8; i += 2) acc[nr][j][i / 4][i % 4] *= c;
-                    racc[nr][e] *= c;
                 }
         }
 #pragma unroll
@@ -645,16 +660,16 @@ __global__ void __launch_bounds__(W * 32, NR == 1 ? kHeld1 : kHeld2) cache_attn_
             }
             const Words<G> va = lds_words<G>(tile + At::value_group(g, 0)), vb = lds_words<G>(tile + At::value_group(g + 8, 0));
             if constexpr (!SPLIT) {  // p in two bf16 parts
-                uint32_t w0, w2;
-                group_operands<G>(tile + At::value_group(0, 0), lane, w0, w2);
+                uint32_t w[4];
+                group_operands<G>(tile + At::value_group(0, 0), lane, w);
 #pragma unroll
                 for (int nr = 0; nr < NR; ++nr) {
                     float a0 = s[i][nr][0], a1 = E == 2 ? s[i][nr][E - 1] : 0.f, b0 = s[i][nr][E], b1 = E == 2 ? s[i][nr][2 * E - 1] : 0.f;
                     const uint32_t ha = pack_bf16x2(a0, a1), hb = pack_bf16x2(b0, b1);
-                    mma_bf16<false>(pacc[nr], w0, 0u, w2, 0u, transpose8x8(ha), transpose8x8(hb));
+                    mma_bf16(pacc[nr], w, transpose8x8(ha), transpose8x8(hb));
                     a0 -= bf16_lo(ha), b0 -= bf16_lo(hb);
                     if constexpr (E == 2) a1 -= bf16_hi(ha), b1 -= bf16_hi(hb);
-                    mma_bf16<false>(pacc[nr], w0, 0u, w2, 0u, transpose8x8(pack_bf16x2(a0, a1)), transpose8x8(pack_bf16x2(b0, b1)));
+                    mma_bf16(pacc[nr], w, transpose8x8(pack_bf16x2(a0, a1)), transpose8x8(pack_bf16x2(b0, b1)));
                 }
             }
             float pm[NR][2 * E];
@@ -668,7 +683,6 @@ __global__ void __launch_bounds__(W * 32, NR == 1 ? kHeld1 : kHeld2) cache_attn_
                 code_operands<VX>(x[0][j], y);
                 code_operands<VX>(x[1][j], z);
                 const float sa = group_scale(va.w[j]), sb = group_scale(vb.w[j]);
-                const uint32_t one = g == j ? kOnes : 0u;
 #pragma unroll
                 for (int nr = 0; nr < NR; ++nr) {
                     if constexpr (SPLIT) {
@@ -691,7 +705,6 @@ __global__ void __launch_bounds__(W * 32, NR == 1 ? kHeld1 : kHeld2) cache_attn_
                     for (int np = 0; np < NP; ++np) {
                         const uint32_t c0_ = transpose8x8(b0[np]), c1_ = transpose8x8(b1[np]);
                         mma_f16(acc[nr][j][0], y[0], y[1], z[0], z[1], c0_, c1_);
-                        if constexpr (!SPLIT) mma_f16(racc[nr], one, 0u, one, 0u, c0_, c1_);
                         mma_f16(acc[nr][j][1], y[2], y[3], z[2], z[3], c0_, c1_);
                     }
                 }
@@ -717,26 +730,22 @@ __global__ void __launch_bounds__(W * 32, NR == 1 ? kHeld1 : kHeld2) cache_attn_
             const float c = m == -INFINITY ? 0.f : ex2(ref[nr][e] - m);
             const float sum = over_g_sum(l[nr][e]) * c;
             const float v = pow2_inverse(mult[nr][e]);
-            float om[G], rs[G];
+            float om[G];
 #pragma unroll
             for (int j = 0; j < G; ++j) {
-                if constexpr (SPLIT) {
-                    om[j] = over_g_sum(omin[nr][e][j]);
-                    rs[j] = 0.f;
-                } else {
-                    om[j] = fmaf(7.5f, __shfl_sync(0xffffffffu, pacc[nr][e], 8 * j + t), __shfl_sync(0xffffffffu, pacc[nr][e], 8 * j + 4 + t));
-                    rs[j] = -7.5f * __shfl_sync(0xffffffffu, racc[nr][e], 4 * j + t);
-                }
+                if constexpr (SPLIT) om[j] = over_g_sum(omin[nr][e][j]);
+                else om[j] = fmaf(8.f, __shfl_sync(0xffffffffu, pacc[nr][e], 8 * j + t),
+                                  __shfl_sync(0xffffffffu, pacc[nr][e], 8 * j + 4 + t));
             }
             if (r < rows) {
                 if (g == 0) sml[warp * R + r] = make_float2(m, sum);
 #pragma unroll
                 for (int j = 0; j < G; ++j) {
                     float4 o;
-                    o.x = fmaf(fmaf(acc[nr][j][0][e], code_unit<VX>(0), rs[j]), v, om[j]) * c;
-                    o.y = fmaf(fmaf(acc[nr][j][0][e + 2], code_unit<VX>(1), rs[j]), v, om[j]) * c;
-                    o.z = fmaf(fmaf(acc[nr][j][1][e], code_unit<VX>(2), rs[j]), v, om[j]) * c;
-                    o.w = fmaf(fmaf(acc[nr][j][1][e + 2], code_unit<VX>(3), rs[j]), v, om[j]) * c;
+                    o.x = fmaf(acc[nr][j][0][e] * code_unit<VX>(0), v, om[j]) * c;
+                    o.y = fmaf(acc[nr][j][0][e + 2] * code_unit<VX>(1), v, om[j]) * c;
+                    o.z = fmaf(acc[nr][j][1][e] * code_unit<VX>(2), v, om[j]) * c;
+                    o.w = fmaf(acc[nr][j][1][e + 2] * code_unit<VX>(3), v, om[j]) * c;
                     *reinterpret_cast<float4*>(sacc + r * D + 32 * j + 4 * g) = o;
                 }
             }
@@ -868,12 +877,12 @@ int attn_validate(const dbl_relay_cache_attention_args* a) {
         return fail(DBL_ERR_INVALID_ARGUMENT, "relay cache attention: heads must be a multiple of kv_heads");
     if (a->dtype != DBL_F32 && a->dtype != DBL_BF16)
         return fail(DBL_ERR_INVALID_ARGUMENT, "relay cache attention: dtype must be f32 or bf16");
-    if (a->prefix_len < 0 || a->prefix_len > 0x3fffffff || a->prefix_width < 0 || a->prefix_width > 0x7fffffff)
+    if (a->prefix_len < 0 || a->prefix_len > kMostTokens || a->prefix_width < 0 || a->prefix_width > 0x7fffffff)
         return fail(DBL_ERR_INVALID_ARGUMENT, "relay cache attention: prefix_len out of range");
     if (a->prefix_len > 0 && (!a->prefix_pages || a->prefix_width * a->cache.page_size < a->prefix_len))
         return fail(DBL_ERR_INVALID_ARGUMENT, "relay cache attention: prefix_pages must hold prefix_len tokens");
     if (a->queries > 0x7fffffff || a->heads > 0x7fffffff || a->n_seq * a->queries > 0x7fffffff / a->heads ||
-        a->table_width * a->cache.page_size > 0x3fffffff)
+        a->table_width * a->cache.page_size > kMostTokens)
         return fail(DBL_ERR_UNSUPPORTED, "relay cache attention: sizes exceed 32-bit limits");
     return DBL_OK;
 }
@@ -945,6 +954,7 @@ extern "C" int dbl_relay_cache_attention(const dbl_relay_cache_attention_args* a
     p.Tq = (int)a->queries;
     p.H = (int)a->heads;
     p.group = (int)(a->heads / a->cache.kv_heads);
+    p.tiles_inv = p.c.tiles == 1 ? 0u : (uint32_t)(((1ull << 32) + p.c.tiles - 1) / p.c.tiles);
     p.prefix_len = (int)a->prefix_len;
     p.prefix_width = (int)a->prefix_width;
     p.scale = a->scale;
