@@ -176,18 +176,28 @@ __device__ __forceinline__ float pow2_inverse(float x) { return __uint_as_float(
 // The operand registers of the 8 codes of w, codes (0, 4), (1, 5), (2, 6), (3, 7), and what they are
 // multiplied by to be the codes (kUnit of register i).
 enum class Codes { kLow, kHigh, kCentred };
+// (x & mask) | bits in one instruction, which takes one constant: the other one stays in a register.
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {
+    uint32_t r;
+    asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(x), "r"(mask), "r"(bits));
+    return r;
+}
 template <Codes C>
 __device__ __forceinline__ void code_operands(uint32_t w, uint32_t (&r)[4]) {
     if constexpr (C == Codes::kHigh) {
         r[0] = (w << 6) & 0x03C003C0u, r[1] = (w << 2) & 0x03C003C0u;
         r[2] = (w >> 2) & 0x03C003C0u, r[3] = (w >> 6) & 0x03C003C0u;
     } else {
-        r[0] = w & 0x000F000Fu, r[1] = w & 0x00F000F0u;
-        r[2] = (w >> 8) & 0x000F000Fu, r[3] = (w >> 8) & 0x00F000F0u;
-        if constexpr (C == Codes::kCentred) {  // 1024 + x is the f16 with mantissa x; 1032 = 1024 + 8, 1152 = 1024 + 16 * 8
+        const uint32_t v = w >> 8;
+        if constexpr (C == Codes::kLow) {
+            r[0] = w & 0x000F000Fu, r[1] = w & 0x00F000F0u;
+            r[2] = v & 0x000F000Fu, r[3] = v & 0x00F000F0u;
+        } else {  // 1024 + x is the f16 with mantissa x; 1032 = 1024 + 8, 1152 = 1024 + 16 * 8
+            r[0] = and_or(w, 0x000F000Fu, 0x64006400u), r[1] = and_or(w, 0x00F000F0u, 0x64006400u);
+            r[2] = and_or(v, 0x000F000Fu, 0x64006400u), r[3] = and_or(v, 0x00F000F0u, 0x64006400u);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r[i]) : "r"(r[i] | 0x64006400u), "r"(i & 1 ? 0xE480E480u : 0xE408E408u));
+                asm("add.rn.f16x2 %0, %0, %1;" : "+r"(r[i]) : "r"(i & 1 ? 0xE480E480u : 0xE408E408u));
         }
     }
 }
