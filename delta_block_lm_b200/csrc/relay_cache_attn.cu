@@ -386,7 +386,7 @@ __global__ void __launch_bounds__(W * 32, NR == 1 ? kHeld1 : kHeld2) cache_attn_
         if (lane == 0) {
             uint8_t* dst = ring + slot * L::STAGE;
             mbar_arrive_expect_tx(bar + slot, __popc(m) * L::TB);
-            if (row && m) {
+            if (row && m == (1u << TS) - 1) {
                 bulk_load(dst, p.c.pool + (int64_t)at[0] * L::TB, TS * L::TB, bar + slot);
             } else {
 #pragma unroll
