@@ -226,6 +226,7 @@ EXPORTS = [
 ]
 
 RELAY_NOALLOC_SCRATCH_BYTES = 16 << 20  # DBL_RELAY_NOALLOC_SCRATCH_BYTES
+RELAY_CACHE_COUNTER_BYTES = 8192  # DBL_RELAY_CACHE_COUNTER_BYTES
 
 _lib = None
 _lock = threading.Lock()

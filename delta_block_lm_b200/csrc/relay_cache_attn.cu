@@ -31,10 +31,14 @@
 // The running maximum is only raised when a score passes it by 8 (in powers of two), so a step
 // usually costs one vote instead of the shuffles of a maximum and the rescaling of the sums.
 //
-// Work: a CTA takes (kv head, up to 8 NR rows, a range of tokens) of the prefix -- rows of all
-// sequences, so that it is read once per head for 8 NR sequences -- or of one sequence.  Its four
-// warps take turns at steps of 32 tokens, each with a ring of its own that bulk copies fill.  The
-// partial sums of the CTAs of a row go to the workspace, and the one that arrives last merges them.
+// Work: an item is (sequence, kv head, up to 8 NR rows), or (kv head, up to 8 NR rows of all
+// sequences) of the prefix, which is thus read once per head for 8 NR rows.  Items are cut into units
+// of 128 tokens, and the units of all items, one after another, are dealt to the CTAs that the GPU
+// holds in equal runs, whatever the lengths are: a CTA finds its run in the lengths, so the host does
+// not need them.  A CTA's four warps take turns at steps of 32 tokens, each with a ring of its own that
+// bulk copies fill.  An item that one CTA holds whole is finished there; the others' sums go to the
+// workspace, and the CTA that arrives last at an item joins them.  The prefix is a launch of its own
+// before the sequences' launch, which joins its sums to every item's.
 #include <float.h>
 
 #include "relay_cache.cuh"
@@ -51,7 +55,10 @@ constexpr int TS = 2;             // tiles of a step
 constexpr int STEP = TS * kCacheTile;
 constexpr int NS = 2;             // stages of a warp's ring
 constexpr int kHeld1 = 4, kHeld2 = 2;  // CTAs that an SM holds at NR = 1 and 2
-constexpr int kOverhead = 128;    // tokens
+constexpr int UNIT = W * STEP;    // tokens of a unit
+constexpr int kApartTokens = 512, kApartSequences = 8;  // of a prefix with a launch of its own
+constexpr int kLeast = 2;         // units of a CTA's run at least
+constexpr int kCounterBytes = DBL_RELAY_CACHE_COUNTER_BYTES;
 constexpr int WIN = 32 / TS;      // steps whose page numbers the lanes of a warp hold
 constexpr int kCacheWaitFull = 40;  // wait-site code (dbl_device_error)
 constexpr int kNoPage = -1, kPast = -2;
@@ -66,19 +73,20 @@ struct AttnParams {
     CacheView c;
     const void* q;
     int64_t qs[3];  // strides of sequence, query and head
+    bool q_vec;     // 16-byte loads
     const int32_t *lengths, *prefix_pages;
     void* out;
     float *row_max, *row_sum;
     int N, Tq, H, group, prefix_len, prefix_width;
     float scale;
     uint32_t tiles_inv;  // ceil(2^32 / tiles of a page), 0 for 1: tile / tiles is the high word of a product
-    bool pre;         // this launch: the prefix, or the sequences' own tokens
-    int tiles;        // row tiles of a kv head: over all sequences, or of one sequence
-    int splits;       // ranges of tokens of the segment
-    int range;        // tokens of a range
-    int at, parts;    // first partial of the segment in a row, partials of a row
-    float *part, *part_ml;       // [rows, splits, D], [rows, splits, 2]
-    unsigned* counter;           // [rows]
+    bool pre;       // this launch: the prefix, or the sequences' own tokens
+    int lead;       // tokens of the prefix's tiles where the sequences' launch reads them itself, 0 where not
+    int tiles;      // row tiles: of a kv head over all sequences, or of a kv head and sequence
+    int pre_tiles, pre_rows, pre_units, pre_run, pre_parts;  // the prefix: row tiles of a head, rows of a tile, units,
+                                                             // units of a run, partials of a row at most
+    unsigned* counter;     // [CTAs]: of the item that begins in a CTA's run and ends in another's
+    float *part, *pre_part;  // rows of D sums, maximum, sum (D + 4 floats): [CTAs][2][R]; [heads, tiles, R][pre_parts]
     int* err;
 };
 
@@ -240,51 +248,57 @@ __device__ __forceinline__ Words<G> lds_words(const uint8_t* p) {
     return r;
 }
 
-// Merges the S partials of output row `row`; one warp.
-template <int D, typename T>
-__device__ void merge_row(const AttnParams& p, int64_t row, int S) {
+constexpr int kPartPad = 4;  // floats of a partial row after its D sums: maximum, sum, two unused
+
+// Joins partial rows to the warp's own rows acc [rows][D] with (maximum, sum) ml [rows], in shared
+// memory.  Lane r says where the partials of row r lie: the i-th of its `count` at from + off + i * stride,
+// the first one `extra` further; the warp takes every W-th.
+template <int D, int R>
+__device__ __forceinline__ void fold_rows(float* acc, float2* ml, int rows, int warp, int lane, const float* from,
+                                          int off, int stride, int extra, int count) {
     constexpr int V = D / 32;  // channels of a lane, neighbouring
-    const int lane = threadIdx.x & 31;
-    const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + row * S;
-    float m = -INFINITY;
-    for (int i = lane; i < S; i += 32) m = fmaxf(m, __ldcg(ml + i).x);
+    if (lane >= rows) count = 0;
+    const int most = __reduce_max_sync(0xffffffffu, count);
+    const float2 own = lane < rows ? ml[lane] : make_float2(-INFINITY, 0.f);
+    float m = own.x;
+#pragma unroll 4
+    for (int i = warp; i < most; i += W)
+        if (i < count) m = fmaxf(m, __ldcg(from + off + i * stride + (i ? 0 : extra) + D));
+    const float c = own.x == -INFINITY ? 0.f : ex2(own.x - m);
+    float l = own.y * c, o[R][V];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    float l = 0.f, acc[V] = {};
-    for (int base = 0; base < S; base += 32) {
-        float w = 0.f, li = 0.f;
-        if (base + lane < S) {
-            const float2 x = __ldcg(ml + base + lane);
-            w = x.x == -INFINITY ? 0.f : ex2(x.x - m);
-            li = x.y;
-        }
-        l += w * li;
-        const int n = min(32, S - base);
-        for (int i = 0; i < n; ++i) {
-            const float wi = __shfl_sync(0xffffffffu, w, i);
-            if (wi == 0.f) continue;
-            const float* a = p.part + (row * S + base + i) * D + lane * V;
+    for (int r = 0; r < R; ++r) {
+        const float cr = __shfl_sync(0xffffffffu, c, r);
+#pragma unroll
+        for (int v = 0; v < V; ++v) o[r][v] = r < rows ? acc[r * D + lane * V + v] * cr : 0.f;
+    }
+#pragma unroll 2
+    for (int i = warp; i < most; i += W) {
+        const int at = off + i * stride + (i ? 0 : extra);
+        const float2 x = i < count ? __ldcg(reinterpret_cast<const float2*>(from + at + D)) : make_float2(-INFINITY, 0.f);
+        const float w = x.x == -INFINITY ? 0.f : ex2(x.x - m);
+        l = fmaf(w, x.y, l);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            const float wr = __shfl_sync(0xffffffffu, w, r);
+            const float* a = from + __shfl_sync(0xffffffffu, at, r) + lane * V;
+            if (wr == 0.f) continue;
             if constexpr (V == 4) {
-                const float4 x = __ldcg(reinterpret_cast<const float4*>(a));
-                acc[0] = fmaf(wi, x.x, acc[0]), acc[1] = fmaf(wi, x.y, acc[1]);
-                acc[2] = fmaf(wi, x.z, acc[2]), acc[3] = fmaf(wi, x.w, acc[3]);
+                const float4 y = __ldcg(reinterpret_cast<const float4*>(a));
+                o[r][0] = fmaf(wr, y.x, o[r][0]), o[r][1] = fmaf(wr, y.y, o[r][1]);
+                o[r][2] = fmaf(wr, y.z, o[r][2]), o[r][3] = fmaf(wr, y.w, o[r][3]);
             } else {
-                const float2 x = __ldcg(reinterpret_cast<const float2*>(a));
-                acc[0] = fmaf(wi, x.x, acc[0]), acc[1] = fmaf(wi, x.y, acc[1]);
+                const float2 y = __ldcg(reinterpret_cast<const float2*>(a));
+                o[r][0] = fmaf(wr, y.x, o[r][0]), o[r][1] = fmaf(wr, y.y, o[r][1]);
             }
         }
     }
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    const bool empty = l == 0.f;
-    const float inv = empty ? 0.f : 1.f / l;
-    T* out = static_cast<T*>(p.out) + row * D + lane * V;
+    for (int r = 0; r < R; ++r)
+        if (r < rows)
 #pragma unroll
-    for (int i = 0; i < V; ++i) out[i] = from_f32<T>(acc[i] * inv);
-    if (lane == 0) {
-        if (p.row_max) p.row_max[row] = empty ? 0.f : m * kLn2;
-        if (p.row_sum) p.row_sum[row] = empty ? 1.f : l;
-    }
+            for (int v = 0; v < V; ++v) acc[r * D + lane * V + v] = o[r][v];
+    if (lane < rows) ml[lane] = make_float2(m, l);
 }
 
 template <int D, typename T, int R>
@@ -294,9 +308,8 @@ struct AttnLayout {
     static constexpr int ACC = W * R * D * 4;  // the warps' sums, over the ring
     static constexpr int OFF_BAR = RING > ACC ? RING : ACC;
     static constexpr int OFF_ML = OFF_BAR + W * NS * 8;
-    static constexpr int OFF_ROW = OFF_ML + W * R * 8;
-    static constexpr int OFF_ERR = OFF_ROW + R * 8;
-    static constexpr int BYTES = OFF_ERR + 16;
+    static constexpr int OFF_SCAN = OFF_ML + W * R * 8;  // error word, last-arrival flag, start of the run, warps' totals
+    static constexpr int BYTES = OFF_SCAN + 32 + W * 4;
 };
 
 // NR groups of 8 columns; E = 2: a row in every column, E = 1 (up to 4 rows): in the even columns only,
@@ -312,24 +325,82 @@ __global__ void __launch_bounds__(W * 32, NR == 1 ? kHeld1 : kHeld2) cache_attn_
     constexpr int G = D / 32;
     constexpr bool SPLIT = sizeof(T) == 4;
     constexpr int NP = SPLIT ? 2 : 1;  // f16 parts of q and of p
+    constexpr int PER = 16 / sizeof(T);
     constexpr Codes KX = SPLIT ? Codes::kHigh : Codes::kLow, VX = Codes::kCentred;
     extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     uint64_t* bar = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR) + warp * NS;
     float2* sml = reinterpret_cast<float2*>(smem + L::OFF_ML);      // [W][R]
-    int64_t* srow = reinterpret_cast<int64_t*>(smem + L::OFF_ROW);  // output rows
-    int* serr = reinterpret_cast<int*>(smem + L::OFF_ERR);
+    int* sint = reinterpret_cast<int*>(smem + L::OFF_SCAN);
+    int* serr = sint;
     uint8_t* ring = smem + warp * NS * L::STAGE;
-
-    // ---- the item
-    const int TG = p.Tq * p.group;
+    const int TG = p.Tq * p.group, HT = p.c.heads * p.tiles;
     const bool pre = p.pre;
-    int item = blockIdx.x;
-    const int rt = item % p.tiles;
-    item /= p.tiles;
-    const int h = item % p.c.heads;
-    item /= p.c.heads;
-    const int split = item % p.splits, seq = item / p.splits;
+    if (lane == 0)
+        for (int i = 0; i < NS; ++i) mbar_init(bar + i, 1);
+    if (threadIdx.x == 0) *serr = 0;
+    fence_mbar_init();
+
+    // ---- the run: units [pos, end) of the items in the order (sequence, kv head, row tile)
+    // An item's tokens: the prefix's where it has no launch of its own, to the end of their last tile, then
+    // the sequence's.
+    const int lead = p.lead, lead_end = lead ? p.prefix_len : 0;
+    auto length_of = [&](int n) {
+        return pre ? p.prefix_len : lead + min(max(p.lengths[n], 0), p.c.width * p.c.tiles * kCacheTile);
+    };
+    auto units_of = [&](int n) { return max(1, (length_of(n) + UNIT - 1) / UNIT); };
+    int run, pos, end, seq = 0, base = 0;  // base: units before sequence seq
+    if (pre) {
+        run = p.pre_run;
+        pos = blockIdx.x * run;
+        end = min(pos + run, HT * p.pre_units);
+        __syncthreads();
+    } else {
+        const int each = (p.N + W * 32 - 1) / (W * 32), n0 = min(p.N, (int)threadIdx.x * each), n1 = min(p.N, n0 + each);
+        int sum = 0;
+        for (int n = n0; n < n1; ++n) sum += units_of(n);
+        int upto = sum;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += x;
+        }
+        if (lane == 31) sint[8 + warp] = upto;
+        __syncthreads();
+        int total = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            if (w < warp) upto += sint[8 + w];
+            total += sint[8 + w];
+        }
+        total *= HT;
+        run = max((total + (int)gridDim.x - 1) / (int)gridDim.x, kLeast);
+        pos = blockIdx.x * run;
+        end = min(pos + run, total);
+        upto *= HT;
+        int before = upto - sum * HT;
+        if (pos >= before && pos < upto) {  // one thread holds the sequence in which the run begins
+            int n = n0;
+            for (int u; pos >= before + (u = units_of(n) * HT); ++n) before += u;
+            sint[2] = n;
+            sint[3] = before;
+        }
+        __syncthreads();
+        seq = sint[2];
+        base = sint[3];
+    }
+    if (pos >= end) return;
+    int slot = 0;  // of the warp's ring, and the parity of its phase
+    uint32_t parity = 0;
+    while (pos < end) {
+    // ---- the item, and what the run holds of it
+    int units = pre ? p.pre_units : units_of(seq);
+    while (!pre && pos >= base + HT * units) base += HT * units, ++seq, units = units_of(seq);
+    const int item = (pos - base) / units, item_pos = base + item * units;
+    const int h = item / p.tiles, rt = item % p.tiles;
+    const int u0 = pos - item_pos, u1 = min(units, u0 + end - pos);
+    const int cta_first = item_pos / run, cta_last = (item_pos + units - 1) / run;
+    pos += u1 - u0;
     const int rows = min(R, (pre ? p.N * TG : TG) - rt * R);
     // row r of the tile: sequence, query, head; the number of keys it sees in this segment
     auto row_of = [&](int r, int& n, int& q, int& hq) {
@@ -339,34 +410,30 @@ __global__ void __launch_bounds__(W * 32, NR == 1 ? kHeld1 : kHeld2) cache_attn_
         q = x / p.group;
         hq = h * p.group + x % p.group;
     };
-    const int len = pre ? p.prefix_len : min(max(p.lengths[seq], 0), p.c.width * p.c.tiles * kCacheTile);
+    const int len = length_of(seq);
     auto row_at = [&](int nr, int e) { return E == 2 ? 8 * nr + 2 * t + e : 4 * nr + t; };  // of the lane's column e
     auto limit_of = [&](int r) {
         if (r >= rows) return 0;
-        return pre ? len : max(0, len - p.Tq + (rt * R + r) / p.group + 1);
+        return pre ? len : max(lead, len - p.Tq + (rt * R + r) / p.group + 1);
     };
-    const int c0 = split * p.range, c1 = min(c0 + p.range, limit_of(rows - 1));  // later rows see more
+    const int c0 = u0 * UNIT, c1 = min(u1 * UNIT, limit_of(rows - 1));  // later rows see more
     const int all_see = limit_of(0);                                         // tokens below it need no mask
     const int steps = c1 > c0 ? (c1 - c0 + STEP - 1) / STEP : 0;
     const int mine = steps > warp ? (steps - warp + W - 1) / W : 0;
     const int tile_end = (c1 + kCacheTile - 1) / kCacheTile;
-
-    if (lane == 0)
-        for (int i = 0; i < NS; ++i) mbar_init(bar + i, 1);
-    if (threadIdx.x == 0) *serr = 0;
-    fence_mbar_init();
-    __syncthreads();
 
     // ---- copies.  Lane l holds the place of tile l % TS of the warp's step (window) + l / TS in the
     // pool: kNoPage where the table has no page for it, kPast where the range has no such tile.
     auto place_of = [&](int step) -> int {
         const int tl = c0 / kCacheTile + ((step + lane / TS) * W + warp) * TS + lane % TS;
         if (tl >= tile_end) return kPast;
-        const int slot = p.tiles_inv ? (int)__umulhi((uint32_t)tl, p.tiles_inv) : tl;
+        const bool shared = pre || tl * kCacheTile < lead;
+        const int at = shared ? tl : tl - lead / kCacheTile;
+        const int slot = p.tiles_inv ? (int)__umulhi((uint32_t)at, p.tiles_inv) : at;
         int page = -1;
-        if (slot < (pre ? p.prefix_width : p.c.width))
-            page = pre ? p.prefix_pages[slot] : p.c.table[seq * p.c.table_stride + slot];
-        return page >= 0 && page < p.c.pages ? (page * p.c.heads + h) * p.c.tiles + tl - slot * p.c.tiles : kNoPage;
+        if (slot < (shared ? p.prefix_width : p.c.width))
+            page = shared ? p.prefix_pages[slot] : p.c.table[seq * p.c.table_stride + slot];
+        return page >= 0 && page < p.c.pages ? (page * p.c.heads + h) * p.c.tiles + at - slot * p.c.tiles : kNoPage;
     };
     int win = place_of(0), win_next = kPast;
     uint32_t have_of = 0;  // TS bits for each slot: the tiles that its copy brings
@@ -399,7 +466,7 @@ __global__ void __launch_bounds__(W * 32, NR == 1 ? kHeld1 : kHeld2) cache_attn_
         __syncwarp();
     };
     int issued = 0;
-    for (; issued < min(NS, mine); ++issued) issue(issued, issued);
+    for (; issued < min(NS, mine); ++issued) issue(issued, slot + issued < NS ? slot + issued : slot + issued - NS);
 
     // ---- q: column g of the products, channels 32 j + 8 t .. + 8 of each group j
     uint32_t qf[NR][NP][G][4];
@@ -420,9 +487,25 @@ __global__ void __launch_bounds__(W * 32, NR == 1 ? kHeld1 : kHeld2) cache_attn_
             row_of(r, n, q, hq);
             const T* src = static_cast<const T*>(p.q) + n * p.qs[0] + q * p.qs[1] + hq * p.qs[2] + 8 * t;
 #pragma unroll
-            for (int j = 0; j < G; ++j)
+            for (int j = 0; j < G; ++j) {
+                if (p.q_vec) {  // every row starts on 16 bytes
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[j][i] = to_f32<T>(src[32 * j + i]) * sign;
+                    for (int i = 0; i < 8 / PER; ++i) {
+                        const uint4 w = __ldg(reinterpret_cast<const uint4*>(src + 32 * j) + i);
+                        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            if constexpr (SPLIT) x[j][4 * i + k] = __uint_as_float(u[k]);
+                            else x[j][2 * k] = bf16_lo(u[k]), x[j][2 * k + 1] = bf16_hi(u[k]);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) x[j][i] = to_f32<T>(src[32 * j + i]);
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[j][i] *= sign;
+            }
         } else {
 #pragma unroll
             for (int j = 0; j < G; ++j)
@@ -495,21 +578,21 @@ __global__ void __launch_bounds__(W * 32, NR == 1 ? kHeld1 : kHeld2) cache_attn_
     }
 
     // ---- the steps
-    int done = 0, slot = 0;
-    uint32_t parity = 0;
-    for (int it = 0; it < mine; ++it) {
+    int done = 0;
+    for (; done < mine; ++done) {
         if (!__all_sync(0xffffffffu, mbar_wait(bar + slot, parity, serr, kCacheWaitFull))) break;
-        done = it + 1;
         const uint8_t* st = ring + slot * L::STAGE;
         const uint32_t have = have_of >> (slot * TS) & ((1u << TS) - 1);
-        const int tok0 = c0 + (it * W + warp) * STEP;
-        const bool masked = tok0 + STEP > min(all_see, c1) || have != (1u << TS) - 1;
+        const int tok0 = c0 + (done * W + warp) * STEP;
+        const bool gap = tok0 < lead && tok0 + STEP > lead_end;  // holds the end of the prefix's last tile
+        const bool masked = tok0 + STEP > min(all_see, c1) || have != (1u << TS) - 1 || gap;
         if (masked) {  // what the groups of tokens that are not there hold is not a number that may be used
 #pragma unroll
             for (int i = 0; i < TS; ++i)
                 for (int w = lane; w < 2 * kCacheTile * G; w += 32) {
                     const int tok = w / G % kCacheTile;
-                    if (!(have >> i & 1) || tok0 + i * kCacheTile + tok >= c1)
+                    const int at = tok0 + i * kCacheTile + tok;
+                    if (!(have >> i & 1) || at >= c1 || (at >= lead_end && at < lead))
                         *reinterpret_cast<uint32_t*>(const_cast<uint8_t*>(st) + i * L::TB +
                                                      (w < kCacheTile * G ? At::key_group(tok, w % G) : At::value_group(tok, w % G))) = 0u;
                 }
@@ -569,7 +652,7 @@ __global__ void __launch_bounds__(W * 32, NR == 1 ? kHeld1 : kHeld2) cache_attn_
 #pragma unroll
                     for (int e = 0; e < 2 * E; ++e) {
                         const int tok = tok0 + i * kCacheTile + g + 8 * (e / E);
-                        if (!(have >> i & 1) || tok >= min(lim[nr][e % E], c1)) s[i][nr][e] = -INFINITY;
+                        if (!(have >> i & 1) || tok >= min(lim[nr][e % E], c1) || (tok >= lead_end && tok < lead)) s[i][nr][e] = -INFINITY;
                     }
         }
         // a bound of each token's value scales: their sum
@@ -725,9 +808,11 @@ __global__ void __launch_bounds__(W * 32, NR == 1 ? kHeld1 : kHeld2) cache_attn_
         if (++slot == NS) slot = 0, parity ^= 1u;
     }
     // A warp that gave up at a wait still owns the copies it issued: let them land first.
-    for (int i = done; i < issued; ++i) mbar_drain(bar + i % NS, (uint32_t)(i / NS) & 1u);
+    for (; done < issued; ++done) {
+        mbar_drain(bar + slot, parity);
+        if (++slot == NS) slot = 0, parity ^= 1u;
+    }
     __syncthreads();
-    if (threadIdx.x == 0 && *serr != 0) atomicExch(p.err, *serr);
 
     // ---- the warps' sums, relative to the largest score of the warp, to shared memory
     float* sacc = reinterpret_cast<float*>(smem) + warp * R * D;
@@ -760,22 +845,15 @@ __global__ void __launch_bounds__(W * 32, NR == 1 ? kHeld1 : kHeld2) cache_attn_
                 }
             }
         }
-    if (threadIdx.x < rows) {
-        int n, q, hq;
-        row_of(threadIdx.x, n, q, hq);
-        srow[threadIdx.x] = ((int64_t)n * p.Tq + q) * p.H + hq;
-    }
     __syncthreads();
 
-    // ---- the CTA's sums: the output, or a partial
-    const int S = p.parts, at = p.at + split;
+    // ---- the CTA's sums
     const float* all = reinterpret_cast<const float*>(smem);
-    for (int i = threadIdx.x; i < rows * (D / 4); i += W * 32) {
-        const int r = i / (D / 4), d = i % (D / 4) * 4;
-        float m = -INFINITY;
+    auto joined = [&](int r, int d, float& m, float& sum) {  // of the warps, row r, channels d .. d + 3
+        m = -INFINITY;
 #pragma unroll
         for (int w = 0; w < W; ++w) m = fmaxf(m, sml[w * R + r].x);
-        float sum = 0.f;
+        sum = 0.f;
         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < W; ++w) {
@@ -785,11 +863,61 @@ __global__ void __launch_bounds__(W * 32, NR == 1 ? kHeld1 : kHeld2) cache_attn_
             sum = fmaf(c, ml.y, sum);
             o.x = fmaf(c, a.x, o.x), o.y = fmaf(c, a.y, o.y), o.z = fmaf(c, a.z, o.z), o.w = fmaf(c, a.w, o.w);
         }
-        const int64_t row = srow[r];
-        if (S > 1) {
-            *reinterpret_cast<float4*>(p.part + (row * S + at) * D + d) = o;
-            if (d == 0) reinterpret_cast<float2*>(p.part_ml)[row * S + at] = make_float2(m, sum);
-        } else {
+        return o;
+    };
+    constexpr int PR = D + kPartPad;
+    auto own_part = [&](int cta, int r) {  // an item begins as the last of a run and goes on as the first of others
+        return p.part + ((int64_t)(cta * 2 + (cta == cta_first ? 1 : 0)) * R + r) * PR;
+    };
+    const bool whole = cta_first == cta_last;
+    if (pre || !whole) {
+        for (int i = threadIdx.x; i < rows * (D / 4); i += W * 32) {
+            const int r = i / (D / 4), d = i % (D / 4) * 4;
+            float m, sum;
+            const float4 o = joined(r, d, m, sum);
+            float* to = pre ? p.pre_part + ((int64_t)(item * R + r) * p.pre_parts + blockIdx.x - cta_first) * PR
+                            : own_part(blockIdx.x, r);
+            *reinterpret_cast<float4*>(to + d) = o;
+            if (d == 0) *reinterpret_cast<float2*>(to + D) = make_float2(m, sum);
+        }
+    }
+    bool finish = !pre && whole;
+    if (!pre && !whole) {  // the CTA that arrives last at the item joins its parts, and leaves the counter at zero
+        __threadfence();
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            const bool last = atomicAdd(p.counter + cta_first, 1u) == (unsigned)(cta_last - cta_first);
+            if (last) p.counter[cta_first] = 0;
+            sint[1] = last;
+        }
+        __syncthreads();
+        finish = sint[1];
+        if (finish) {
+            __threadfence();
+            for (int i = lane; i < rows * D; i += 32) sacc[i] = 0.f;
+            if (lane < rows) sml[warp * R + lane] = make_float2(-INFINITY, 0.f);
+            __syncwarp();
+            fold_rows<D, R>(sacc, sml + warp * R, rows, warp, lane, p.part, (cta_first * 2 * R + lane) * PR, 2 * R * PR,
+                            R * PR, cta_last - cta_first + 1);
+            __syncthreads();
+        }
+    }
+    if (finish) {
+        if (p.pre_units) {  // the prefix's launch has ended
+            const int x = seq * TG + rt * R + min(lane, rows - 1), it = h * p.pre_tiles + x / p.pre_rows;
+            const int first = it * p.pre_units / p.pre_run, last = ((it + 1) * p.pre_units - 1) / p.pre_run;
+            __syncwarp();
+            fold_rows<D, R>(sacc, sml + warp * R, rows, warp, lane, p.pre_part,
+                            (it * p.pre_rows + x % p.pre_rows) * p.pre_parts * PR, PR, 0, last - first + 1);
+            __syncthreads();
+        }
+        for (int i = threadIdx.x; i < rows * (D / 4); i += W * 32) {
+            const int r = i / (D / 4), d = i % (D / 4) * 4;
+            float m, sum;
+            const float4 o = joined(r, d, m, sum);
+            int n, q, hq;
+            row_of(r, n, q, hq);
+            const int64_t row = ((int64_t)n * p.Tq + q) * p.H + hq;
             const bool empty = sum == 0.f;
             const float inv = empty ? 0.f : 1.f / sum;
             T* out = static_cast<T*>(p.out) + row * D + d;
@@ -801,76 +929,58 @@ __global__ void __launch_bounds__(W * 32, NR == 1 ? kHeld1 : kHeld2) cache_attn_
             }
         }
     }
-    if (S == 1) return;
-    // ---- the CTA that arrives last at a row merges it, and leaves its counter at zero
-    __shared__ uint32_t s_last;
-    if (threadIdx.x == 0) s_last = 0;
-    __threadfence();
+    fence_proxy_async_smem();  // the sums lie where the next item's copies go
     __syncthreads();
-    if (threadIdx.x < rows) {
-        const unsigned before = atomicAdd(p.counter + srow[threadIdx.x], 1u);
-        if (before == (unsigned)S - 1) {
-            p.counter[srow[threadIdx.x]] = 0;
-            atomicOr(&s_last, 1u << threadIdx.x);
-        }
     }
-    __syncthreads();
-    const uint32_t last = s_last;
-    if (last == 0) return;
-    __threadfence();
-    for (int r = warp; r < rows; r += W)
-        if (last >> r & 1) merge_row<D, T>(p, srow[r], S);
+    if (threadIdx.x == 0 && *serr != 0) atomicExch(p.err, *serr);
 }
-
-struct Segment {
-    int nr, e, tiles, splits, range;
-    int64_t grid;
-};
-struct Plan {
-    Segment own, pre;
-    int64_t rows;
-    int parts;
-    size_t off_ml, off_cnt, bytes;
-};
 
 int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// A segment of `tokens` tokens that `rows` rows of a kv head share, `items` times.
+struct Segment {  // the prefix, or the sequences' own tokens
+    int nr, e, rows, tiles;
+    int64_t units, grid;  // of all items, at most
+};
+
+// `rows` rows share the tokens of an item.
 Segment segment_of(int64_t rows, int64_t items, int64_t tokens, bool bf16) {
     Segment s{};
     s.e = rows <= 4 ? 1 : 2;
     s.nr = bf16 && rows > 8 ? 2 : 1;
-    s.tiles = (int)ceil_div(rows, 4 * s.e * s.nr);
-    items *= s.tiles;
-    // The cut that takes the fewest tokens one after another: rounds of CTAs that the GPU holds at a
-    // time, each the tokens of a range and a start and end that cost about as much as kOverhead.
-    const int64_t held = 148 * (s.nr == 2 ? kHeld2 : kHeld1), unit = W * STEP;
-    int64_t best = -1;
-    for (int64_t n = 1; n <= ceil_div(tokens, unit) && (n == 1 || items * n <= 4 * held); ++n) {
-        const int64_t range = ceil_div(ceil_div(tokens, n), unit) * unit, splits = ceil_div(tokens, range);
-        const int64_t cost = ceil_div(items * splits, held) * (range + kOverhead);
-        if (best < 0 || cost < best) {
-            best = cost;
-            s.range = (int)range;
-            s.splits = (int)splits;
-        }
-    }
-    s.grid = items * s.splits;
+    s.rows = 4 * s.e * s.nr;
+    s.tiles = (int)ceil_div(rows, s.rows);
+    s.units = items * s.tiles * (tokens > UNIT ? ceil_div(tokens, UNIT) : 1);
+    const int64_t held = 148 * (s.nr == 2 ? kHeld2 : kHeld1), runs = ceil_div(s.units, kLeast);
+    s.grid = runs < held ? runs : held;
     return s;
 }
+
+struct Plan {
+    Segment own, pre;
+    int lead, pre_units, pre_run, pre_parts;
+    size_t off_part, off_pre, bytes;
+};
 
 Plan plan_of(const dbl_relay_cache_attention_args* a) {
     Plan L{};
     const int64_t TG = a->queries * (a->heads / a->cache.kv_heads), H = a->cache.kv_heads, N = a->n_seq;
     const bool bf16 = a->dtype == DBL_BF16;
-    L.own = segment_of(TG, N * H, a->table_width * a->cache.page_size, bf16);
-    if (a->prefix_len > 0) L.pre = segment_of(N * TG, H, a->prefix_len, bf16);
-    L.rows = N * a->queries * a->heads;
-    L.parts = L.pre.splits + L.own.splits;
-    if (L.parts > 1) {
-        L.off_ml = (size_t)(L.rows * L.parts * a->cache.head_dim) * 4;
-        L.off_cnt = L.off_ml + (size_t)(L.rows * L.parts) * 8;
-        L.bytes = L.off_cnt + (size_t)L.rows * 4;
+    const size_t row = (size_t)(a->cache.head_dim + kPartPad) * 4;
+    // A prefix is worth a launch of its own where many sequences share it and it is long.
+    const bool apart = a->prefix_len >= kApartTokens && N >= kApartSequences;
+    L.lead = a->prefix_len > 0 && !apart ? (int)(ceil_div(a->prefix_len, kCacheTile) * kCacheTile) : 0;
+    L.own = segment_of(TG, N * H, L.lead + a->table_width * a->cache.page_size, bf16);
+    L.off_part = kCounterBytes;
+    L.off_pre = L.off_part + (size_t)(L.own.grid * 2 * L.own.rows) * row;
+    L.bytes = L.off_pre;
+    if (apart) {
+        L.pre = segment_of(N * TG, H, a->prefix_len, bf16);
+        L.pre_units = (int)ceil_div(a->prefix_len, UNIT);
+        L.pre_run = (int)ceil_div(L.pre.units, L.pre.grid);
+        if (L.pre_run < kLeast) L.pre_run = kLeast;
+        L.pre.grid = ceil_div(L.pre.units, L.pre_run);
+        L.pre_parts = (L.pre_units + L.pre_run - 2) / L.pre_run + 1;
+        L.bytes += (size_t)(H * L.pre.tiles * L.pre.rows * L.pre_parts) * row;
     }
     return L;
 }
@@ -912,12 +1022,9 @@ int launch_attn(const AttnParams& p, int64_t grid, cudaStream_t st) {
 }
 
 template <int D>
-int launch_segment(AttnParams p, const Segment& s, bool pre, int at, bool bf16, cudaStream_t st) {
+int launch_segment(AttnParams p, const Segment& s, bool pre, bool bf16, cudaStream_t st) {
     p.pre = pre;
     p.tiles = s.tiles;
-    p.splits = s.splits;
-    p.range = s.range;
-    p.at = at;
     if (!bf16) return s.e == 1 ? launch_attn<D, float, 1, 1>(p, s.grid, st) : launch_attn<D, float, 1, 2>(p, s.grid, st);
     if (s.nr == 2) return launch_attn<D, __nv_bfloat16, 2, 2>(p, s.grid, st);
     return s.e == 1 ? launch_attn<D, __nv_bfloat16, 1, 1>(p, s.grid, st)
@@ -945,16 +1052,22 @@ extern "C" int dbl_relay_cache_attention(const dbl_relay_cache_attention_args* a
     resolve_strides(a->q_stride, dims, 4, qs);
     if (qs[3] != 1) return fail(DBL_ERR_INVALID_ARGUMENT, "relay cache attention: the innermost stride of q must be 1");
     const Plan L = plan_of(a);
-    if (L.own.grid > 0x7fffffff || L.pre.grid > 0x7fffffff) return fail(DBL_ERR_UNSUPPORTED, "relay cache attention: grid too large");
-    if (L.bytes && (!workspace || workspace_bytes < L.bytes))
+    if (L.own.units > 0x3fffffff || L.pre.units > 0x3fffffff || L.bytes > ((size_t)1 << 32))
+        return fail(DBL_ERR_UNSUPPORTED, "relay cache attention: sizes exceed 32-bit limits");
+    if (!workspace || workspace_bytes < L.bytes)
         return fail(DBL_ERR_WORKSPACE, "relay cache attention: workspace of %zu bytes required (got %zu)", L.bytes,
                     workspace_bytes);
-    if (L.bytes && !aligned(workspace, 16))
+    if (!aligned(workspace, 16))
         return fail(DBL_ERR_INVALID_ARGUMENT, "relay cache attention: workspace must be 16-byte aligned");
     AttnParams p{};
     p.c = cache_view(&a->cache, a->page_table, a->table_width, a->table_stride);
     p.q = a->q;
-    for (int i = 0; i < 3; ++i) p.qs[i] = qs[i];
+    const int64_t per = 16 / (int64_t)dtype_size(a->dtype);
+    p.q_vec = aligned(a->q, 16);
+    for (int i = 0; i < 3; ++i) {
+        p.qs[i] = qs[i];
+        p.q_vec = p.q_vec && qs[i] % per == 0;
+    }
     p.lengths = a->lengths;
     p.prefix_pages = a->prefix_pages;
     p.out = a->out;
@@ -968,19 +1081,23 @@ extern "C" int dbl_relay_cache_attention(const dbl_relay_cache_attention_args* a
     p.prefix_len = (int)a->prefix_len;
     p.prefix_width = (int)a->prefix_width;
     p.scale = a->scale;
-    p.parts = L.parts;
+    p.lead = L.lead;
+    p.pre_tiles = L.pre.tiles;
+    p.pre_rows = L.pre.rows;
+    p.pre_units = L.pre_units;
+    p.pre_run = L.pre_run;
+    p.pre_parts = L.pre_parts;
     uint8_t* ws = static_cast<uint8_t*>(workspace);
-    p.part = reinterpret_cast<float*>(ws);
-    p.part_ml = reinterpret_cast<float*>(ws + L.off_ml);
-    p.counter = reinterpret_cast<unsigned*>(ws + L.off_cnt);
+    p.counter = reinterpret_cast<unsigned*>(ws);
+    p.part = reinterpret_cast<float*>(ws + L.off_part);
+    p.pre_part = reinterpret_cast<float*>(ws + L.off_pre);
     rc = device_error_record(&p.err);
     if (rc != DBL_OK) return rc;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     const bool bf16 = a->dtype == DBL_BF16;
-    if (L.pre.splits) {
-        rc = D == 128 ? launch_segment<128>(p, L.pre, true, 0, bf16, st) : launch_segment<64>(p, L.pre, true, 0, bf16, st);
+    if (L.pre_units) {
+        rc = D == 128 ? launch_segment<128>(p, L.pre, true, bf16, st) : launch_segment<64>(p, L.pre, true, bf16, st);
         if (rc != DBL_OK) return rc;
     }
-    return D == 128 ? launch_segment<128>(p, L.own, false, L.pre.splits, bf16, st)
-                    : launch_segment<64>(p, L.own, false, L.pre.splits, bf16, st);
+    return D == 128 ? launch_segment<128>(p, L.own, false, bf16, st) : launch_segment<64>(p, L.own, false, bf16, st);
 }

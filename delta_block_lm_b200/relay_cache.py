@@ -119,6 +119,22 @@ def relay_cache_read(pool, page_table, lengths, *, start=None, tokens: int, dtyp
     return k, v
 
 
+_workspaces: dict = {}  # (device, stream): the attention's workspace, kept from call to call
+
+
+def _workspace(need: int, dev: torch.device, stream: int) -> torch.Tensor:
+    """A workspace whose counters are zero.  Calls on one stream follow one another, so each stream keeps
+    one; a graph that is being captured gets its own (it may be replayed beside other calls)."""
+    capturing = torch.cuda.is_current_stream_capturing()
+    ws = None if capturing else _workspaces.get((dev.index, stream))
+    if ws is None or ws.numel() < need:
+        ws = torch.empty(need, device=dev, dtype=torch.uint8)
+        ws[:N.RELAY_CACHE_COUNTER_BYTES].zero_()
+        if not capturing:
+            _workspaces[dev.index, stream] = ws
+    return ws
+
+
 def relay_cache_attention(q, pool, page_table, lengths, *, prefix_pages=None, prefix_len: int = 0,
                           scale: Optional[float] = None, out=None, workspace: Optional[torch.Tensor] = None):
     """Attention of each sequence's newest tokens over [shared prefix ; own tokens].
@@ -126,7 +142,8 @@ def relay_cache_attention(q, pool, page_table, lengths, *, prefix_pages=None, pr
     q [N, heads, D], or [N, Tq, heads, D] for the last Tq tokens of each sequence, causal among
     themselves; f32 or bf16, heads a multiple of the pool's kv heads.  ``lengths`` counts the queries'
     own tokens (append first).  ``prefix_pages`` [width] names the pages of ``prefix_len`` tokens that
-    every sequence sees before its own.  Returns (o, row_max, row_sum) as ``relay_merge_decode``; a row
+    every sequence sees before its own.  ``workspace``: a uint8 tensor whose first
+    ``RELAY_CACHE_COUNTER_BYTES`` bytes are zero before its first use (by default each stream keeps one).  Returns (o, row_max, row_sum) as ``relay_merge_decode``; a row
     without keys gives o = 0 and (0, 1)."""
     dev = _require_cuda(q, pool, page_table, lengths, prefix_pages, out, workspace)
     c = _cache(pool)
@@ -160,11 +177,10 @@ def relay_cache_attention(q, pool, page_table, lengths, *, prefix_pages=None, pr
                                       _ptr(page_table), _ptr(lengths), _ptr(prefix_pages) if prefix_len else None,
                                       _ptr(out), _ptr(row_max), _ptr(row_sum))
         if q.numel():
-            need = N.lib().dbl_relay_cache_attention_workspace_bytes(ctypes.byref(a))
-            if workspace is None and need:
-                workspace = torch.zeros(need, device=dev, dtype=torch.uint8)
-            N.check(N.lib().dbl_relay_cache_attention(ctypes.byref(a), _ptr(workspace),
-                                                      workspace.numel() if workspace is not None else 0, _stream(dev)))
+            stream = _stream(dev)
+            if workspace is None:
+                workspace = _workspace(N.lib().dbl_relay_cache_attention_workspace_bytes(ctypes.byref(a)), dev, stream)
+            N.check(N.lib().dbl_relay_cache_attention(ctypes.byref(a), _ptr(workspace), workspace.numel(), stream))
     return out, row_max, row_sum
 
 

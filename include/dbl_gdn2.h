@@ -462,9 +462,10 @@ int dbl_relay_cache_read(const dbl_relay_cache_read_args *args, dbl_stream_t str
  * h / (heads / kv_heads).  out [n_seq, queries, heads, head_dim] in dtype and row_max, row_sum f32
  * [n_seq, queries, heads] are contiguous; the statistics and the empty row are those of
  * dbl_relay_merge_decode (o = 0, max = 0, sum = 1).
- * The workspace (dbl_relay_cache_attention_workspace_bytes, 16-byte aligned; NULL where that is 0)
- * must be zero before its first use; every call leaves its counters zero again.  Calls that overlap
- * on the GPU must use distinct workspaces. */
+ * The workspace (dbl_relay_cache_attention_workspace_bytes, 16-byte aligned) holds counters in its
+ * first DBL_RELAY_CACHE_COUNTER_BYTES bytes, which must be zero before its first use; every call leaves them
+ * zero again.  Calls that overlap on the GPU must use distinct workspaces. */
+#define DBL_RELAY_CACHE_COUNTER_BYTES 8192
 typedef struct {
     dbl_relay_cache cache;
     int64_t n_seq, queries, heads, table_width, table_stride, prefix_len, prefix_width;
