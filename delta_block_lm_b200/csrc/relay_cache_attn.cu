@@ -54,10 +54,10 @@ constexpr int W = 4;              // warps of a CTA
 constexpr int TS = 2;             // tiles of a step
 constexpr int STEP = TS * kCacheTile;
 constexpr int NS = 2;             // stages of a warp's ring
-constexpr int kHeld1 = 4, kHeld2 = 2;  // CTAs that an SM holds at NR = 1 and 2
 constexpr int UNIT = W * STEP;    // tokens of a unit
 constexpr int kApartTokens = 512, kApartSequences = 8;  // of a prefix with a launch of its own
-constexpr int kLeast = 2;         // units of a CTA's run at least
+constexpr int kStart = 3;         // units that the start and end of an item cost (about 6 us, a unit 2 us)
+constexpr int kLeast = 4;         // units of a CTA's run at least
 constexpr int kCounterBytes = DBL_RELAY_CACHE_COUNTER_BYTES;
 constexpr int WIN = 32 / TS;      // steps whose page numbers the lanes of a warp hold
 constexpr int kCacheWaitFull = 40;  // wait-site code (dbl_device_error)
@@ -261,7 +261,7 @@ __device__ __forceinline__ void fold_rows(float* acc, float2* ml, int rows, int 
     const int most = __reduce_max_sync(0xffffffffu, count);
     const float2 own = lane < rows ? ml[lane] : make_float2(-INFINITY, 0.f);
     float m = own.x;
-#pragma unroll 4
+#pragma unroll 8
     for (int i = warp; i < most; i += W)
         if (i < count) m = fmaxf(m, __ldcg(from + off + i * stride + (i ? 0 : extra) + D));
     const float c = own.x == -INFINITY ? 0.f : ex2(own.x - m);
@@ -272,26 +272,39 @@ __device__ __forceinline__ void fold_rows(float* acc, float2* ml, int rows, int 
 #pragma unroll
         for (int v = 0; v < V; ++v) o[r][v] = r < rows ? acc[r * D + lane * V + v] * cr : 0.f;
     }
-#pragma unroll 2
-    for (int i = warp; i < most; i += W) {
-        const int at = off + i * stride + (i ? 0 : extra);
-        const float2 x = i < count ? __ldcg(reinterpret_cast<const float2*>(from + at + D)) : make_float2(-INFINITY, 0.f);
-        const float w = x.x == -INFINITY ? 0.f : ex2(x.x - m);
-        l = fmaf(w, x.y, l);
+    constexpr int AT_ONCE = R == 1 ? 8 : R <= 4 ? 2 : 1;  // parts whose loads are on their way together
+    for (int i0 = warp; i0 < most; i0 += W * AT_ONCE) {
+        float w[AT_ONCE];
+        float4 y[AT_ONCE][R];
 #pragma unroll
-        for (int r = 0; r < R; ++r) {
-            const float wr = __shfl_sync(0xffffffffu, w, r);
-            const float* a = from + __shfl_sync(0xffffffffu, at, r) + lane * V;
-            if (wr == 0.f) continue;
-            if constexpr (V == 4) {
-                const float4 y = __ldcg(reinterpret_cast<const float4*>(a));
-                o[r][0] = fmaf(wr, y.x, o[r][0]), o[r][1] = fmaf(wr, y.y, o[r][1]);
-                o[r][2] = fmaf(wr, y.z, o[r][2]), o[r][3] = fmaf(wr, y.w, o[r][3]);
-            } else {
-                const float2 y = __ldcg(reinterpret_cast<const float2*>(a));
-                o[r][0] = fmaf(wr, y.x, o[r][0]), o[r][1] = fmaf(wr, y.y, o[r][1]);
+        for (int k = 0; k < AT_ONCE; ++k) {
+            const int i = i0 + k * W, at = off + i * stride + (i ? 0 : extra);
+            const float2 x = i < count ? __ldcg(reinterpret_cast<const float2*>(from + at + D)) : make_float2(-INFINITY, 0.f);
+            w[k] = x.x == -INFINITY ? 0.f : ex2(x.x - m);
+            l = fmaf(w[k], x.y, l);
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const float* a = from + __shfl_sync(0xffffffffu, at, r) + lane * V;
+                const bool in = __shfl_sync(0xffffffffu, i < count, r);
+                y[k][r] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if constexpr (V == 4) {
+                    if (in) y[k][r] = __ldcg(reinterpret_cast<const float4*>(a));
+                } else {
+                    if (in) {
+                        const float2 z = __ldcg(reinterpret_cast<const float2*>(a));
+                        y[k][r].x = z.x, y[k][r].y = z.y;
+                    }
+                }
             }
         }
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k)
+#pragma unroll
+            for (int r = 0; r < R; ++r) {
+                const float wr = __shfl_sync(0xffffffffu, w[k], r);
+                o[r][0] = fmaf(wr, y[k][r].x, o[r][0]), o[r][1] = fmaf(wr, y[k][r].y, o[r][1]);
+                if constexpr (V == 4) o[r][2] = fmaf(wr, y[k][r].z, o[r][2]), o[r][3] = fmaf(wr, y[k][r].w, o[r][3]);
+            }
     }
 #pragma unroll
     for (int r = 0; r < R; ++r)
@@ -314,11 +327,13 @@ struct AttnLayout {
 
 // NR groups of 8 columns; E = 2: a row in every column, E = 1 (up to 4 rows): in the even columns only,
 // which saves the arithmetic of the others (a lane holds two neighbouring columns of every product).
+// CTAs that an SM holds, by the registers that a tile's sums take.
+constexpr int held_at(int nr, int e) { return nr == 2 ? 2 : e == 2 ? 3 : 4; }
 template <int NR, int E>
 constexpr int rows_of_tile() { return NR * 4 * E; }
 
 template <int D, typename T, int NR, int E>
-__global__ void __launch_bounds__(W * 32, NR == 1 ? kHeld1 : kHeld2) cache_attn_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(W * 32, held_at(NR, E)) cache_attn_kernel(const AttnParams p) {
     constexpr int R = rows_of_tile<NR, E>();
     using L = AttnLayout<D, T, R>;
     using At = TileAt<D>;
@@ -341,14 +356,16 @@ __global__ void __launch_bounds__(W * 32, NR == 1 ? kHeld1 : kHeld2) cache_attn_
     if (threadIdx.x == 0) *serr = 0;
     fence_mbar_init();
 
-    // ---- the run: units [pos, end) of the items in the order (sequence, kv head, row tile)
+    // ---- the run: units [pos, end) of the items in the order (sequence, kv head, row tile); each item begins
+    // with `start` units that stand for no tokens
     // An item's tokens: the prefix's where it has no launch of its own, to the end of their last tile, then
     // the sequence's.
     const int lead = p.lead, lead_end = lead ? p.prefix_len : 0;
     auto length_of = [&](int n) {
         return pre ? p.prefix_len : lead + min(max(p.lengths[n], 0), p.c.width * p.c.tiles * kCacheTile);
     };
-    auto units_of = [&](int n) { return max(1, (length_of(n) + UNIT - 1) / UNIT); };
+    const int start = pre ? 0 : kStart;
+    auto units_of = [&](int n) { return start + max(1, (length_of(n) + UNIT - 1) / UNIT); };
     int run, pos, end, seq = 0, base = 0;  // base: units before sequence seq
     if (pre) {
         run = p.pre_run;
@@ -398,8 +415,10 @@ __global__ void __launch_bounds__(W * 32, NR == 1 ? kHeld1 : kHeld2) cache_attn_
     while (!pre && pos >= base + HT * units) base += HT * units, ++seq, units = units_of(seq);
     const int item = (pos - base) / units, item_pos = base + item * units;
     const int h = item / p.tiles, rt = item % p.tiles;
-    const int u0 = pos - item_pos, u1 = min(units, u0 + end - pos);
-    const int cta_first = item_pos / run, cta_last = (item_pos + units - 1) / run;
+    pos = max(pos, item_pos + start);
+    if (pos >= end) break;
+    const int u0 = pos - item_pos - start, u1 = min(units - start, u0 + end - pos);
+    const int cta_first = (item_pos + start) / run, cta_last = (item_pos + units - 1) / run;
     pos += u1 - u0;
     const int rows = min(R, (pre ? p.N * TG : TG) - rt * R);
     // row r of the tile: sequence, query, head; the number of keys it sees in this segment
@@ -421,6 +440,37 @@ __global__ void __launch_bounds__(W * 32, NR == 1 ? kHeld1 : kHeld2) cache_attn_
     const int steps = c1 > c0 ? (c1 - c0 + STEP - 1) / STEP : 0;
     const int mine = steps > warp ? (steps - warp + W - 1) / W : 0;
     const int tile_end = (c1 + kCacheTile - 1) / kCacheTile;
+
+    // ---- q: column g of the products, channels 32 j + 8 t .. + 8 of each group j, as it lies in memory;
+    // asked for before the copies, whose bytes would be ahead of it
+    uint4 raw[NR][G][8 / PER];
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr) {
+        const int r = E == 2 ? 8 * nr + g : 4 * nr + g / 2;
+        const bool live = r < rows && (E == 2 || g % 2 == 0);
+        int n = 0, q = 0, hq = 0;
+        if (live) row_of(r, n, q, hq);
+        const T* src = static_cast<const T*>(p.q) + n * p.qs[0] + q * p.qs[1] + hq * p.qs[2] + 8 * t;
+#pragma unroll
+        for (int j = 0; j < G; ++j)
+#pragma unroll
+            for (int i = 0; i < 8 / PER; ++i) {
+                uint4 w = make_uint4(0, 0, 0, 0);
+                if (live && p.q_vec) {  // every row starts on 16 bytes
+                    w = __ldg(reinterpret_cast<const uint4*>(src + 32 * j) + i);
+                } else if (live) {
+                    const T* e = src + 32 * j + PER * i;
+                    if constexpr (SPLIT) {
+                        w = make_uint4(__float_as_uint(e[0]), __float_as_uint(e[1]), __float_as_uint(e[2]), __float_as_uint(e[3]));
+                    } else {
+                        const uint16_t* b = reinterpret_cast<const uint16_t*>(e);
+                        w = make_uint4(b[0] | (uint32_t)b[1] << 16, b[2] | (uint32_t)b[3] << 16, b[4] | (uint32_t)b[5] << 16,
+                                       b[6] | (uint32_t)b[7] << 16);
+                    }
+                }
+                raw[nr][j][i] = w;
+            }
+    }
 
     // ---- copies.  Lane l holds the place of tile l % TS of the warp's step (window) + l / TS in the
     // pool: kNoPage where the table has no page for it, kPast where the range has no such tile.
@@ -468,7 +518,7 @@ __global__ void __launch_bounds__(W * 32, NR == 1 ? kHeld1 : kHeld2) cache_attn_
     int issued = 0;
     for (; issued < min(NS, mine); ++issued) issue(issued, slot + issued < NS ? slot + issued : slot + issued - NS);
 
-    // ---- q: column g of the products, channels 32 j + 8 t .. + 8 of each group j
+    // ---- q as operands
     uint32_t qf[NR][NP][G][4];
     // sums of q over the groups / f as three bf16 parts, in the odd places (the minima's) of the
     // operand for the (scale, minimum) words: group t
@@ -479,39 +529,19 @@ __global__ void __launch_bounds__(W * 32, NR == 1 ? kHeld1 : kHeld2) cache_attn_
     float f[NR][E];  // of the columns 2 t, 2 t + 1: score = f * inner
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr) {
-        const int r = E == 2 ? 8 * nr + g : 4 * nr + g / 2;
         float x[G][8];
         float top = 0.f;
-        if (r < rows && (E == 2 || g % 2 == 0)) {
-            int n, q, hq;
-            row_of(r, n, q, hq);
-            const T* src = static_cast<const T*>(p.q) + n * p.qs[0] + q * p.qs[1] + hq * p.qs[2] + 8 * t;
 #pragma unroll
-            for (int j = 0; j < G; ++j) {
-                if (p.q_vec) {  // every row starts on 16 bytes
+        for (int j = 0; j < G; ++j)
 #pragma unroll
-                    for (int i = 0; i < 8 / PER; ++i) {
-                        const uint4 w = __ldg(reinterpret_cast<const uint4*>(src + 32 * j) + i);
-                        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+            for (int i = 0; i < 8 / PER; ++i) {
+                const uint32_t u[4] = {raw[nr][j][i].x, raw[nr][j][i].y, raw[nr][j][i].z, raw[nr][j][i].w};
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            if constexpr (SPLIT) x[j][4 * i + k] = __uint_as_float(u[k]);
-                            else x[j][2 * k] = bf16_lo(u[k]), x[j][2 * k + 1] = bf16_hi(u[k]);
-                        }
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) x[j][i] = to_f32<T>(src[32 * j + i]);
+                for (int k = 0; k < 4; ++k) {
+                    if constexpr (SPLIT) x[j][4 * i + k] = __uint_as_float(u[k]) * sign;
+                    else x[j][2 * k] = bf16_lo(u[k]) * sign, x[j][2 * k + 1] = bf16_hi(u[k]) * sign;
                 }
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[j][i] *= sign;
             }
-        } else {
-#pragma unroll
-            for (int j = 0; j < G; ++j)
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[j][i] = 0.f;
-        }
 #pragma unroll
         for (int j = 0; j < G; ++j)
 #pragma unroll
@@ -869,6 +899,10 @@ __global__ void __launch_bounds__(W * 32, NR == 1 ? kHeld1 : kHeld2) cache_attn_
     auto own_part = [&](int cta, int r) {  // an item begins as the last of a run and goes on as the first of others
         return p.part + ((int64_t)(cta * 2 + (cta == cta_first ? 1 : 0)) * R + r) * PR;
     };
+    auto fold = [&](const float* from, int off, int stride, int extra, int count) {
+        if (R <= 4 && rows == 1) fold_rows<D, 1>(sacc, sml + warp * R, 1, warp, lane, from, off, stride, extra, count);
+        else fold_rows<D, R>(sacc, sml + warp * R, rows, warp, lane, from, off, stride, extra, count);
+    };
     const bool whole = cta_first == cta_last;
     if (pre || !whole) {
         for (int i = threadIdx.x; i < rows * (D / 4); i += W * 32) {
@@ -897,7 +931,7 @@ __global__ void __launch_bounds__(W * 32, NR == 1 ? kHeld1 : kHeld2) cache_attn_
             for (int i = lane; i < rows * D; i += 32) sacc[i] = 0.f;
             if (lane < rows) sml[warp * R + lane] = make_float2(-INFINITY, 0.f);
             __syncwarp();
-            fold_rows<D, R>(sacc, sml + warp * R, rows, warp, lane, p.part, (cta_first * 2 * R + lane) * PR, 2 * R * PR,
+            fold(p.part, (cta_first * 2 * R + lane) * PR, 2 * R * PR,
                             R * PR, cta_last - cta_first + 1);
             __syncthreads();
         }
@@ -907,7 +941,7 @@ __global__ void __launch_bounds__(W * 32, NR == 1 ? kHeld1 : kHeld2) cache_attn_
             const int x = seq * TG + rt * R + min(lane, rows - 1), it = h * p.pre_tiles + x / p.pre_rows;
             const int first = it * p.pre_units / p.pre_run, last = ((it + 1) * p.pre_units - 1) / p.pre_run;
             __syncwarp();
-            fold_rows<D, R>(sacc, sml + warp * R, rows, warp, lane, p.pre_part,
+            fold(p.pre_part,
                             (it * p.pre_rows + x % p.pre_rows) * p.pre_parts * PR, PR, 0, last - first + 1);
             __syncthreads();
         }
@@ -943,14 +977,14 @@ struct Segment {  // the prefix, or the sequences' own tokens
 };
 
 // `rows` rows share the tokens of an item.
-Segment segment_of(int64_t rows, int64_t items, int64_t tokens, bool bf16) {
+Segment segment_of(int64_t rows, int64_t items, int64_t tokens, int start, bool bf16) {
     Segment s{};
     s.e = rows <= 4 ? 1 : 2;
     s.nr = bf16 && rows > 8 ? 2 : 1;
     s.rows = 4 * s.e * s.nr;
     s.tiles = (int)ceil_div(rows, s.rows);
-    s.units = items * s.tiles * (tokens > UNIT ? ceil_div(tokens, UNIT) : 1);
-    const int64_t held = 148 * (s.nr == 2 ? kHeld2 : kHeld1), runs = ceil_div(s.units, kLeast);
+    s.units = items * s.tiles * (start + (tokens > UNIT ? ceil_div(tokens, UNIT) : 1));
+    const int64_t held = 148 * held_at(s.nr, s.e), runs = ceil_div(s.units, kLeast);
     s.grid = runs < held ? runs : held;
     return s;
 }
@@ -969,12 +1003,12 @@ Plan plan_of(const dbl_relay_cache_attention_args* a) {
     // A prefix is worth a launch of its own where many sequences share it and it is long.
     const bool apart = a->prefix_len >= kApartTokens && N >= kApartSequences;
     L.lead = a->prefix_len > 0 && !apart ? (int)(ceil_div(a->prefix_len, kCacheTile) * kCacheTile) : 0;
-    L.own = segment_of(TG, N * H, L.lead + a->table_width * a->cache.page_size, bf16);
+    L.own = segment_of(TG, N * H, L.lead + a->table_width * a->cache.page_size, kStart, bf16);
     L.off_part = kCounterBytes;
     L.off_pre = L.off_part + (size_t)(L.own.grid * 2 * L.own.rows) * row;
     L.bytes = L.off_pre;
     if (apart) {
-        L.pre = segment_of(N * TG, H, a->prefix_len, bf16);
+        L.pre = segment_of(N * TG, H, a->prefix_len, 0, bf16);
         L.pre_units = (int)ceil_div(a->prefix_len, UNIT);
         L.pre_run = (int)ceil_div(L.pre.units, L.pre.grid);
         if (L.pre_run < kLeast) L.pre_run = kLeast;
