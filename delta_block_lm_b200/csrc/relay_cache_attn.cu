@@ -38,7 +38,7 @@
 // not need them.  A CTA's four warps take turns at steps of 32 tokens, each with a ring of its own that
 // bulk copies fill.  An item that one CTA holds whole is finished there; the others' sums go to the
 // workspace, and the CTA that arrives last at an item joins them.  The prefix is a launch of its own
-// before the sequences' launch, which joins its sums to every item's.
+// before the sequences' launch, which starts beside it and joins its sums to every item's.
 #include <float.h>
 
 #include "relay_cache.cuh"
@@ -355,6 +355,8 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E)) cache_attn_kernel(cons
         for (int i = 0; i < NS; ++i) mbar_init(bar + i, 1);
     if (threadIdx.x == 0) *serr = 0;
     fence_mbar_init();
+
+    if (pre) asm volatile("griddepcontrol.launch_dependents;");  // the sequences' launch may fill what this one leaves free
 
     // ---- the run: units [pos, end) of the items in the order (sequence, kv head, row tile); each item begins
     // with `start` units that stand for no tokens
@@ -937,7 +939,8 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E)) cache_attn_kernel(cons
         }
     }
     if (finish) {
-        if (p.pre_units) {  // the prefix's launch has ended
+        if (p.pre_units) {
+            asm volatile("griddepcontrol.wait;" ::: "memory");  // the prefix's launch has ended
             const int x = seq * TG + rt * R + min(lane, rows - 1), it = h * p.pre_tiles + x / p.pre_rows;
             const int first = it * p.pre_units / p.pre_run, last = ((it + 1) * p.pre_units - 1) / p.pre_run;
             __syncwarp();
@@ -1051,8 +1054,18 @@ int launch_attn(const AttnParams& p, int64_t grid, cudaStream_t st) {
             "relay cache attention: cudaFuncSetAttribute");
     });
     if (rc != DBL_OK) return rc;
-    cache_attn_kernel<D, T, NR, E><<<(unsigned)grid, W * 32, smem, st>>>(p);
-    return launch_status("cache_attn_kernel");
+    // The sequences' launch after the prefix's starts without waiting for it, and waits where it joins its sums.
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)grid);
+    cfg.blockDim = dim3(W * 32);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = p.pre_units && !p.pre ? 1 : 0;
+    return cuda_status(cudaLaunchKernelEx(&cfg, cache_attn_kernel<D, T, NR, E>, p), "cache_attn_kernel");
 }
 
 template <int D>
