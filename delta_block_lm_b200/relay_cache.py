@@ -31,9 +31,30 @@ from typing import Optional
 import torch
 
 from . import _native as N
-from .kernels import _dtype_code, _ptr, _require_cuda, _stream
+from .kernels import _dtype_code, _ptr, _require_cuda
 
 TILE = 16  # tokens of one tile: page sizes are multiples of it
+
+
+class _Here:
+    """The context of a call whose device is the current one already."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *_):
+        return None
+
+
+_here = _Here()
+
+
+def _on(dev: torch.device):
+    return _here if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
+def _stream(dev: torch.device) -> int:  # a decode step makes several of these calls: the short way
+    return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
 def relay_cache_pool(pages: int, kv_heads: int, head_dim: int, page_size: int = 64, *, device="cuda") -> torch.Tensor:
@@ -56,7 +77,7 @@ def _cache(pool: torch.Tensor) -> N.RelayCache:
 def _ints(name: str, t: Optional[torch.Tensor], shape: tuple) -> Optional[torch.Tensor]:
     if t is None:
         return None
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"relay cache: {name} must be {list(shape)}, got {list(t.shape)}")
     if t.dtype != torch.int32 or not t.is_contiguous():
         t = t.to(torch.int32).contiguous()
@@ -91,7 +112,7 @@ def relay_cache_append(pool, page_table, lengths, k, v, *, counts=None, out=None
         k = k.contiguous()
     if v.stride(3) != 1:
         v = v.contiguous()
-    with torch.cuda.device(dev):
+    with _on(dev):
         new = torch.empty_like(lengths)
         a = N.RelayCacheAppendArgs(c, n, t, page_table.shape[1], 0, _dtype_code(k), _ptr(k), _ptr(v), k.stride(),
                                    v.stride(), _ptr(page_table), _ptr(lengths), _ptr(counts), _ptr(new))
@@ -109,7 +130,7 @@ def relay_cache_read(pool, page_table, lengths, *, start=None, tokens: int, dtyp
     n = page_table.shape[0]
     page_table = _ints("page_table", page_table, tuple(page_table.shape))
     lengths, start = _ints("lengths", lengths, (n,)), _ints("start", start, (n,))
-    with torch.cuda.device(dev):
+    with _on(dev):
         k = torch.empty((n, tokens, c.kv_heads, c.head_dim), device=dev, dtype=dtype)
         v = torch.empty_like(k)
         a = N.RelayCacheReadArgs(c, n, tokens, page_table.shape[1], 0, _dtype_code(k), _ptr(page_table), _ptr(lengths),
@@ -119,19 +140,20 @@ def relay_cache_read(pool, page_table, lengths, *, start=None, tokens: int, dtyp
     return k, v
 
 
-_workspaces: dict = {}  # (device, stream): the attention's workspace, kept from call to call
+_workspaces: dict = {}  # (what for, device, stream): a workspace kept from call to call
 
 
-def _workspace(need: int, dev: torch.device, stream: int) -> torch.Tensor:
-    """A workspace whose counters are zero.  Calls on one stream follow one another, so each stream keeps
-    one; a graph that is being captured gets its own (it may be replayed beside other calls)."""
+def _workspace(what: str, need: int, dev: torch.device, stream: int) -> torch.Tensor:
+    """A workspace whose counters (the attention's) are zero.  Calls on one stream follow one another, so
+    each stream keeps one; a graph that is being captured gets its own (it may be replayed beside other
+    calls)."""
     capturing = torch.cuda.is_current_stream_capturing()
-    ws = None if capturing else _workspaces.get((dev.index, stream))
+    ws = None if capturing else _workspaces.get((what, dev.index, stream))
     if ws is None or ws.numel() < need:
         ws = torch.empty(need, device=dev, dtype=torch.uint8)
         ws[:N.RELAY_CACHE_COUNTER_BYTES].zero_()
         if not capturing:
-            _workspaces[dev.index, stream] = ws
+            _workspaces[what, dev.index, stream] = ws
     return ws
 
 
@@ -164,13 +186,13 @@ def relay_cache_attention(q, pool, page_table, lengths, *, prefix_pages=None, pr
         q = q.contiguous()
     if scale is None:
         scale = 1.0 / math.sqrt(c.head_dim)
-    with torch.cuda.device(dev):
+    with _on(dev):
         if out is None:
-            out = torch.empty(q.shape, device=dev, dtype=q.dtype)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
             raise ValueError("relay cache attention: out must be contiguous with the shape and dtype of q")
-        stats = torch.empty((2, *q.shape[:-1]), device=dev, dtype=torch.float32)
-        row_max, row_sum = stats
+        rows = q.shape[:-1]
+        row_max, row_sum = q.new_empty(rows, dtype=torch.float32), q.new_empty(rows, dtype=torch.float32)
         qs = q.stride() if q.dim() == 4 else (q.stride(0), 0, q.stride(1), 1)
         a = N.RelayCacheAttentionArgs(c, n, tq, heads, page_table.shape[1], 0, prefix_len,
                                       prefix_pages.shape[0] if prefix_len else 0, _dtype_code(q), scale, _ptr(q), qs,
@@ -179,42 +201,45 @@ def relay_cache_attention(q, pool, page_table, lengths, *, prefix_pages=None, pr
         if q.numel():
             stream = _stream(dev)
             if workspace is None:
-                workspace = _workspace(N.lib().dbl_relay_cache_attention_workspace_bytes(ctypes.byref(a)), dev, stream)
+                workspace = _workspace("attention", N.lib().dbl_relay_cache_attention_workspace_bytes(ctypes.byref(a)), dev, stream)
             N.check(N.lib().dbl_relay_cache_attention(ctypes.byref(a), _ptr(workspace), workspace.numel(), stream))
     return out, row_max, row_sum
 
 
-def _pages(pool, page_table, lengths, refs, out, lists):
-    """(device, arguments, outputs) of a page operation; ``lengths`` None where it has none."""
+def _pages(pool, page_table, lengths, refs, out, lists, new_lengths=True):
+    """(device, arguments, outputs, tensors to keep) of a page operation; lengths None: it has none."""
     dev = _require_cuda(pool, page_table, lengths, refs, *lists, *(out or ()))
     c = _cache(pool)
     if page_table.dim() != 2:
         raise ValueError(f"relay cache: page_table must be [sequences,width], got {list(page_table.shape)}")
     s, w = page_table.shape
-    state = [_ints("page_table", page_table, (s, w)), _ints("lengths", lengths, (s,)), _ints("refs", refs, (c.pages,))]
-    given = [t for t in state if t is not None]
+    page_table, refs = _ints("page_table", page_table, (s, w)), _ints("refs", refs, (c.pages,))
+    lengths = _ints("lengths", lengths, (s,))
+    new_lengths = new_lengths and lengths is not None
+    given = (page_table, lengths, refs) if new_lengths else (page_table, refs)
     if out is None:
-        after = [torch.empty_like(t) for t in given]
+        after = tuple([torch.empty_like(t) for t in given])
     else:
-        after = list(out)
+        after = tuple(out)
+        if len(after) != len(given):
+            raise ValueError(f"relay cache: out must be {len(given)} tensors")
         for t, o in zip(given, after):
             if o.shape != t.shape or o.dtype != torch.int32 or not o.is_contiguous():
                 raise ValueError("relay cache: out must be contiguous int32 tensors shaped like the state")
-    into = after if lengths is not None else [after[0], None, after[1]]
-    a = N.RelayCachePagesArgs(c, s, w, 0, *(_ptr(t) for t in state), *(_ptr(t) for t in into))
-    return dev, a, tuple(after), state
+    a = N.RelayCachePagesArgs(c, s, w, 0, page_table.data_ptr(), _ptr(lengths), refs.data_ptr(), after[0].data_ptr(),
+                              after[1].data_ptr() if new_lengths else None, after[-1].data_ptr())
+    return dev, a, after, (page_table, lengths, refs)
 
 
-def _scratch(a, dev):
-    return torch.empty(N.lib().dbl_relay_cache_pages_workspace_bytes(a.cache.pages, a.n_seq), device=dev,
-                       dtype=torch.uint8)
+def _scratch(a, dev, stream):
+    return _workspace("pages", N.lib().dbl_relay_cache_pages_workspace_bytes(a.cache.pages, a.n_seq), dev, stream)
 
 
 def relay_cache_release(pool, page_table, lengths, refs, sequences, *, out=None):
     """Gives back the pages of ``sequences`` (a list of row numbers).  Returns (page_table, lengths, refs)."""
     sequences = _list("sequences", sequences)
     dev, a, after, _keep = _pages(pool, page_table, lengths, refs, out, (sequences,))
-    with torch.cuda.device(dev):
+    with _on(dev):
         N.check(N.lib().dbl_relay_cache_release(ctypes.byref(a), _ptr(sequences), sequences.numel(), _stream(dev)))
     return after
 
@@ -226,7 +251,7 @@ def relay_cache_fork(pool, page_table, lengths, refs, parents, children, *, out=
     if parents.shape != children.shape:
         raise ValueError("relay cache fork: parents and children must have the same length")
     dev, a, after, _keep = _pages(pool, page_table, lengths, refs, out, (parents, children))
-    with torch.cuda.device(dev):
+    with _on(dev):
         N.check(N.lib().dbl_relay_cache_fork(ctypes.byref(a), _ptr(parents), _ptr(children), parents.numel(),
                                              _stream(dev)))
     return after
@@ -240,14 +265,13 @@ def relay_cache_reserve(pool, page_table, lengths, refs, tokens, *, out=None):
     counts = None
     if isinstance(tokens, torch.Tensor):
         counts, tokens = _ints("tokens", tokens, tuple(lengths.shape)), 0
-    dev, a, after, _keep = _pages(pool, page_table, lengths, refs, None if out is None else (out[0], lengths, out[1]),
-                                  () if counts is None else (counts,))
-    with torch.cuda.device(dev):
-        missing = torch.empty(1, device=dev, dtype=torch.int32)
-        ws = _scratch(a, dev)
+    dev, a, after, _keep = _pages(pool, page_table, lengths, refs, out, () if counts is None else (counts,), False)
+    with _on(dev):
+        missing, stream = refs.new_empty(1), _stream(dev)
+        ws = _scratch(a, dev, stream)
         N.check(N.lib().dbl_relay_cache_reserve(ctypes.byref(a), _ptr(counts), tokens, _ptr(missing), _ptr(ws),
-                                                ws.numel(), _stream(dev)))
-    return after[0], after[2], missing
+                                                ws.numel(), stream))
+    return after[0], after[1], missing
 
 
 def relay_cache_compact(pool, page_table, refs, *, out=None):
@@ -255,10 +279,10 @@ def relay_cache_compact(pool, page_table, refs, *, out=None):
     Returns (page_table, refs, used): pages 0 .. used - 1 are in use, the others free.  A shared
     prefix's pages follow if they are a row of the page table."""
     dev, a, after, _keep = _pages(pool, page_table, None, refs, out, ())
-    with torch.cuda.device(dev):
-        used = torch.empty(1, device=dev, dtype=torch.int32)
-        ws = _scratch(a, dev)
-        N.check(N.lib().dbl_relay_cache_compact(ctypes.byref(a), _ptr(used), _ptr(ws), ws.numel(), _stream(dev)))
+    with _on(dev):
+        used, stream = refs.new_empty(1, dtype=torch.int32), _stream(dev)
+        ws = _scratch(a, dev, stream)
+        N.check(N.lib().dbl_relay_cache_compact(ctypes.byref(a), _ptr(used), _ptr(ws), ws.numel(), stream))
     return after[0], after[1], used
 
 
@@ -269,5 +293,5 @@ def relay_cache_copy_pages(pool, src, dst) -> None:
     if src.shape != dst.shape:
         raise ValueError("relay cache copy: src and dst must have the same length")
     c = _cache(pool)
-    with torch.cuda.device(dev):
+    with _on(dev):
         N.check(N.lib().dbl_relay_cache_copy_pages(ctypes.byref(c), _ptr(src), _ptr(dst), src.numel(), _stream(dev)))
