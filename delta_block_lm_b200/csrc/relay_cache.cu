@@ -8,6 +8,8 @@
 // has 13 significant bits and is exact.  A range below 2^-100 has scale 0 (1 / scale must be
 // finite); a range that is not finite (an infinity or NaN among the values) makes the group NaN, so
 // that it shows in what is computed from the token and from no other.
+#include <type_traits>
+
 #include "relay_cache.cuh"
 #include "tc_ptx.cuh"
 
@@ -20,7 +22,8 @@ struct AppendParams {
     int64_t ks[3], vs[3];  // strides of sequence, token and head
     const int32_t *lengths, *counts;
     int32_t* new_lengths;
-    int N, T;
+    int N, T, tiles;  // tiles: that T tokens can touch
+    bool vec;         // 16-byte loads
     int* err;
 };
 
@@ -32,49 +35,53 @@ struct ReadParams {
     int* err;
 };
 
-// Codes of 8 channels of a group of which four neighbouring lanes hold 8 each.  Returns the eight
-// codes (the first in the lowest four bits) and the group's (scale, minimum) word.
-__device__ __forceinline__ uint32_t encode8(const float (&x)[8], uint32_t& word) {
+// Codes of NC channels of a group, of which 32 / NC neighbouring lanes hold NC each: 8 to a word, the
+// first in the lowest four bits.  Returns the group's (scale, minimum) word.
+//
+// The code of d = x - minimum is the nearest integer to d / scale, ties down.  The guess, d times a
+// reciprocal that is 2^-21 too small (rcp.approx is off by 2^-23 at most), rounded to an integer by adding
+// 1.5 * 2^23, is the code or one less; d - guess * scale is exact (a multiple of d's last place, less than
+// 2^24 of them) and says which.
+template <int NC>
+__device__ __forceinline__ uint32_t encode(const float (&x)[NC], uint32_t (&codes)[NC / 8]) {
     // fminf and fmaxf pass over a NaN, the sum does not
     float lo = x[0], hi = x[0], sum = x[0];
 #pragma unroll
-    for (int i = 1; i < 8; ++i) {
+    for (int i = 1; i < NC; ++i) {
         lo = fminf(lo, x[i]);
         hi = fmaxf(hi, x[i]);
         sum += x[i];
     }
-    bool bad = sum != sum;
 #pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {
+    for (int o = 1; o < 32 / NC; o <<= 1) {
         lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
         hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        bad = bad | (__shfl_xor_sync(0xffffffffu, (int)bad, o) != 0);
+        sum += __shfl_xor_sync(0xffffffffu, sum, o);
     }
     uint32_t lb = __float_as_uint(lo);
     lb = (lb & 0x80000000u) ? (lb + 0xFFFFu) & 0xFFFF0000u : lb & 0xFFFF0000u;
     const float base = __uint_as_float(lb);
     const float span = hi - base;
-    bad = bad || !(span <= 3.402823466e38f);
     uint32_t sb = (__float_as_uint(__fdiv_rn(span, 15.f)) + 0xFFFFu) & 0xFFFF0000u;
     if (span < 7.888609052e-31f) sb = 0;  // 2^-100
-    if (bad) {
-        word = 0x7FFF0000u;  // scale 0, minimum NaN
-        return 0;
-    }
-    word = (sb >> 16) | lb;
-    if (sb == 0) return 0;
-    const float s = __uint_as_float(sb), inv = __fdiv_rn(1.f, s);
-    uint32_t codes = 0;
+    const bool bad = sum != sum || !(span <= 3.402823466e38f);
+    const float s = __uint_as_float(sb), half = 0.5f * s;
+    float inv;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+    inv *= 0.9999995232f;
+    constexpr float kRound = 12582912.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float d = x[i] - base;
-        // a first guess within one of the code, then the definition
-        int c = __float2int_ru(fmaf(d, inv, -0.5f));
-        c += d > ((float)c + 0.5f) * s ? 1 : 0;
-        c -= d <= ((float)c - 0.5f) * s ? 1 : 0;
-        codes |= (uint32_t)min(max(c, 0), 15) << (4 * i);
+    for (int w = 0; w < NC / 8; ++w) {
+        uint32_t word = 0;
+#pragma unroll
+        for (int i = 7; i >= 0; --i) {
+            const float d = x[8 * w + i] - base, t = fmaf(d, inv, kRound);
+            const uint32_t more = fmaf(kRound - t, s, d) > half ? 1u : 0u;
+            word = word * 16u + (__float_as_uint(t) + more - __float_as_uint(kRound));
+        }
+        codes[w] = bad || sb == 0 ? 0u : word;
     }
-    return codes;
+    return bad ? 0x7FFF0000u /* scale 0, minimum NaN */ : (sb >> 16) | lb;
 }
 
 template <typename T>
@@ -102,10 +109,10 @@ __device__ __forceinline__ void load8<float>(const float* p, bool vec, float (&x
     }
 }
 
-// One thread: 8 channels of one (token, head), of the key and then of the value; four neighbouring
-// lanes are a group.
+// Single tokens.  One thread: 8 channels of one (token, head), of the key and then of the value; four
+// neighbouring lanes are a group.
 template <int D, typename T>
-__global__ void __launch_bounds__(256) cache_append_kernel(const AppendParams p, bool vec) {
+__global__ void __launch_bounds__(256) cache_append_kernel(const AppendParams p) {
     using At = TileAt<D>;
     constexpr int LPT = D / 8;  // lanes of a token and head
     const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
@@ -116,34 +123,130 @@ __global__ void __launch_bounds__(256) cache_append_kernel(const AppendParams p,
         const int cnt = p.counts ? min(max(p.counts[i], 0), p.T) : p.T;
         p.new_lengths[i] = p.lengths[i] + cnt;
     }
-    // whole groups of lanes leave or stay, and the shuffles are among the four lanes of a group
+    // lanes past the end go along with the first row and write nothing: the shuffles need whole groups
     const bool inside = row < rows;
     const int h = inside ? (int)(row % p.c.heads) : 0;
     const int64_t nt = inside ? row / p.c.heads : 0;
     const int t = (int)(nt % p.T);
     const int64_t n = nt / p.T;
+    float x[8], y[8];
+    load8<T>(static_cast<const T*>(p.k) + n * p.ks[0] + t * p.ks[1] + h * p.ks[2] + part * 8, p.vec, x);
+    load8<T>(static_cast<const T*>(p.v) + n * p.vs[0] + t * p.vs[1] + h * p.vs[2] + part * 8, p.vec, y);
     const int count = p.counts ? min(max(p.counts[n], 0), p.T) : p.T;
     const bool live = inside && t < count;
     const int pos = p.lengths[n] + t;
     const int page = live && pos >= 0 ? cache_page(p.c, n, pos / kCacheTile) : -1;
     if (live && page < 0) atomicExch(p.err, kCacheErrorPage);
     const int k = pos & (kCacheTile - 1);
-    uint8_t* tile = cache_tile<D>(p.c, max(page, 0), h, (pos / kCacheTile) % p.c.tiles);
+    uint8_t* tile = cache_tile<D>(p.c, max(page, 0), h, max(pos, 0) / kCacheTile % p.c.tiles);
     const int j = part / 4, q = part % 4;  // group, quarter of the group
-    float x[8];
-    uint32_t word;
-    load8<T>(static_cast<const T*>(p.k) + n * p.ks[0] + t * p.ks[1] + h * p.ks[2] + part * 8, vec, x);
-    uint32_t codes = encode8(x, word);
-    if (page >= 0) {
-        *reinterpret_cast<uint32_t*>(tile + At::key_word(k, q, j)) = codes;
-        if (q == 0) *reinterpret_cast<uint32_t*>(tile + At::key_group(k, j)) = word;
+    uint32_t kc[1], vc[1];
+    const uint32_t kw = encode<8>(x, kc), vw = encode<8>(y, vc);
+    if (page < 0) return;
+    *reinterpret_cast<uint32_t*>(tile + At::key_word(k, q, j)) = kc[0];
+    *reinterpret_cast<uint16_t*>(tile + At::value_half(k, 2 * q, j)) = (uint16_t)vc[0];
+    *reinterpret_cast<uint16_t*>(tile + At::value_half(k, 2 * q + 1, j)) = (uint16_t)(vc[0] >> 16);
+    if (q == 0) {
+        *reinterpret_cast<uint32_t*>(tile + At::key_group(k, j)) = kw;
+        *reinterpret_cast<uint32_t*>(tile + At::value_group(k, j)) = vw;
     }
-    load8<T>(static_cast<const T*>(p.v) + n * p.vs[0] + t * p.vs[1] + h * p.vs[2] + part * 8, vec, x);
-    codes = encode8(x, word);
-    if (page >= 0) {
-        *reinterpret_cast<uint16_t*>(tile + At::value_half(k, 2 * q, j)) = (uint16_t)codes;
-        *reinterpret_cast<uint16_t*>(tile + At::value_half(k, 2 * q + 1, j)) = (uint16_t)(codes >> 16);
-        if (q == 0) *reinterpret_cast<uint32_t*>(tile + At::value_group(k, j)) = word;
+}
+
+// Prompts.  A CTA writes one tile of positions for kTileHeads heads: the tile is put together in shared
+// memory and leaves in 16-byte words (in the pieces of single tokens where it is not written whole).  One
+// thread: 16 channels of one token's key or value, two neighbouring lanes a group; its next head's
+// values are on their way while it encodes.
+constexpr int kTileHeads = 4;
+constexpr int kTileTokens = 8;  // calls of at least so many tokens a sequence go by tiles
+
+template <int D, typename T>
+__global__ void __launch_bounds__(256) cache_append_tiles_kernel(const AppendParams p) {
+    using At = TileAt<D>;
+    constexpr int TB = cache_tile_bytes(D), LPT = D / 16, HP = 128 / D;  // lanes of a token, heads of a pass
+    constexpr int NW = 16 / (16 / (int)sizeof(T));                       // 16-byte words of 16 channels
+    __shared__ __align__(16) uint8_t image[2][HP * TB];
+    const int hg = (p.c.heads + kTileHeads - 1) / kTileHeads;
+    int64_t b = blockIdx.x;
+    const int h0 = (int)(b % hg) * kTileHeads, h1 = min(h0 + kTileHeads, p.c.heads);
+    b /= hg;
+    const int64_t n = b / p.tiles;
+    const int count = p.counts ? min(max(p.counts[n], 0), p.T) : p.T, len = p.lengths[n];
+    if (p.new_lengths && b % p.tiles == 0 && h0 == 0 && threadIdx.x == 0) p.new_lengths[n] = len + count;
+    const int tl = max(len, 0) / kCacheTile + (int)(b % p.tiles), t0 = tl * kCacheTile - len;  // token of place 0
+    if (t0 >= count || len < 0) return;
+    const int page = cache_page(p.c, n, tl);
+    if (page < 0) {
+        if (threadIdx.x == 0) atomicExch(p.err, kCacheErrorPage);
+        return;
+    }
+    const int i = threadIdx.x, hp = i / (2 * D), which = i / D % 2, k = i / LPT % kCacheTile, part = i % LPT;
+    const int t = t0 + k, j = part / 2, q = part % 2;
+    const bool live = t >= 0 && t < count;
+    const bool whole = t0 >= 0 && t0 + kCacheTile <= count;
+    const T* src = static_cast<const T*>(which ? p.v : p.k) + n * (which ? p.vs[0] : p.ks[0]) +
+                   (live ? t : max(0, -t0)) * (which ? p.vs[1] : p.ks[1]) + part * 16;
+    const int64_t hs = which ? p.vs[2] : p.ks[2];
+    uint4 raw[NW];
+    auto load = [&](int h) {
+        const T* at = src + min(h, h1 - 1) * hs;
+        if (p.vec) {
+#pragma unroll
+            for (int w = 0; w < NW; ++w) raw[w] = __ldg(reinterpret_cast<const uint4*>(at) + w);
+        } else {
+            T v[16];
+#pragma unroll
+            for (int w = 0; w < 16; ++w) v[w] = at[w];
+#pragma unroll
+            for (int w = 0; w < NW; ++w) raw[w] = reinterpret_cast<const uint4*>(v)[w];
+        }
+    };
+    load(h0 + hp);
+    int buf = 0;
+    for (int h = h0; h < h1; h += HP, buf ^= 1) {
+        float x[16];
+#pragma unroll
+        for (int w = 0; w < NW; ++w) {
+            const uint32_t u[4] = {raw[w].x, raw[w].y, raw[w].z, raw[w].w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if constexpr (sizeof(T) == 4) x[4 * w + e] = __uint_as_float(u[e]);
+                else x[8 * w + 2 * e] = bf16_lo(u[e]), x[8 * w + 2 * e + 1] = bf16_hi(u[e]);
+            }
+        }
+        if (h + HP < h1) load(h + HP + hp);
+        uint32_t codes[2];
+        const uint32_t word = encode<16>(x, codes);
+        uint8_t* img = image[buf] + hp * TB;
+        if (which) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                *reinterpret_cast<uint16_t*>(img + At::value_half(k, 4 * q + e, j)) = (uint16_t)(codes[e / 2] >> (16 * (e % 2)));
+            if (q == 0) *reinterpret_cast<uint32_t*>(img + At::value_group(k, j)) = word;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) *reinterpret_cast<uint32_t*>(img + At::key_word(k, 2 * q + e, j)) = codes[e];
+            if (q == 0) *reinterpret_cast<uint32_t*>(img + At::key_group(k, j)) = word;
+        }
+        __syncthreads();  // the image is complete; the other one has been written out (two images, one barrier each)
+        const int heads = min(HP, h1 - h);
+        uint8_t* to = cache_tile<D>(p.c, page, h, tl % p.c.tiles);
+        const int64_t per = (int64_t)p.c.tiles * TB;  // from head to head
+        if (whole) {
+            for (int w = i; w < heads * (TB / 16); w += 256) {
+                const int hh = w / (TB / 16), at = w % (TB / 16);
+                reinterpret_cast<uint4*>(to + hh * per)[at] = reinterpret_cast<const uint4*>(image[buf] + hh * TB)[at];
+            }
+        } else {  // pieces of D / 16 bytes, each of one token
+            using Piece = typename std::conditional<D == 128, uint2, uint32_t>::type;
+            constexpr int NPC = TB / (int)sizeof(Piece), ROW = 8;
+            for (int w = i; w < heads * NPC; w += 256) {
+                const int hh = w / NPC, at = w % NPC, in = at % (NPC / 2);  // codes: 16 rows of 8 pieces, groups: 2 pieces
+                int kk = in >= 16 * ROW ? (in - 16 * ROW) / 2 : at < NPC / 2 ? in / ROW : in / 64 * 8 + in % 8;
+                const int tt = t0 + kk;
+                if (tt >= 0 && tt < count)
+                    reinterpret_cast<Piece*>(to + hh * per)[at] = reinterpret_cast<const Piece*>(image[buf] + hh * TB)[at];
+            }
+        }
     }
 }
 
@@ -163,7 +266,8 @@ __device__ __forceinline__ void store8<float>(float* p, const float (&x)[8]) {
 __device__ __forceinline__ void decode8(uint32_t codes, uint32_t word, float (&x)[8]) {
     const float s = group_scale(word), m = group_min(word);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = fmaf(s, (float)((codes >> (4 * i)) & 15u), m);  // the product is exact
+    for (int i = 0; i < 8; ++i)  // 2^23 + code as bits; the product is exact
+        x[i] = fmaf(s, __uint_as_float((codes >> (4 * i) & 15u) | 0x4B000000u) - 8388608.f, m);
 }
 
 template <int D, typename T>
@@ -269,16 +373,21 @@ extern "C" int dbl_relay_cache_append(const dbl_relay_cache_append_args* a, dbl_
     if (rc != DBL_OK) return rc;
     // 16-byte loads where every row of k and v starts on 16 bytes
     const int64_t per = 16 / (int64_t)dtype_size(a->dtype);
-    bool vec = aligned(a->k, 16) && aligned(a->v, 16);
-    for (int i = 0; i < 3; ++i) vec = vec && ks[i] % per == 0 && vs[i] % per == 0;
-    const unsigned grid = blocks_for(threads > p.N ? threads : p.N, 256);
+    p.vec = aligned(a->k, 16) && aligned(a->v, 16);
+    for (int i = 0; i < 3; ++i) p.vec = p.vec && ks[i] % per == 0 && vs[i] % per == 0;
+    p.tiles = (int)((a->tokens + 2 * kCacheTile - 2) / kCacheTile);
+    const int64_t ctas = a->n_seq * p.tiles * ((a->cache.kv_heads + kTileHeads - 1) / kTileHeads);
+    const bool tiles = a->tokens >= kTileTokens;
+    if (tiles && ctas > 0x7fffffff) return fail(DBL_ERR_UNSUPPORTED, "relay cache append: grid too large");
+    const unsigned grid = tiles ? (unsigned)ctas : blocks_for(threads, 256);
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    const auto launch = [&](auto kernel) { kernel<<<grid, 256, 0, st>>>(p); };
     if (a->dtype == DBL_BF16) {
-        if (D == 128) cache_append_kernel<128, __nv_bfloat16><<<grid, 256, 0, st>>>(p, vec);
-        else cache_append_kernel<64, __nv_bfloat16><<<grid, 256, 0, st>>>(p, vec);
+        if (D == 128) launch(tiles ? cache_append_tiles_kernel<128, __nv_bfloat16> : cache_append_kernel<128, __nv_bfloat16>);
+        else launch(tiles ? cache_append_tiles_kernel<64, __nv_bfloat16> : cache_append_kernel<64, __nv_bfloat16>);
     } else {
-        if (D == 128) cache_append_kernel<128, float><<<grid, 256, 0, st>>>(p, vec);
-        else cache_append_kernel<64, float><<<grid, 256, 0, st>>>(p, vec);
+        if (D == 128) launch(tiles ? cache_append_tiles_kernel<128, float> : cache_append_kernel<128, float>);
+        else launch(tiles ? cache_append_tiles_kernel<64, float> : cache_append_kernel<64, float>);
     }
     return launch_status("cache_append_kernel");
 }

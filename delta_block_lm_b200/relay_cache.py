@@ -188,11 +188,12 @@ def relay_cache_attention(q, pool, page_table, lengths, *, prefix_pages=None, pr
         scale = 1.0 / math.sqrt(c.head_dim)
     with _on(dev):
         if out is None:
-            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            out = torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, device=dev, dtype=q.dtype)
         elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
             raise ValueError("relay cache attention: out must be contiguous with the shape and dtype of q")
-        rows = q.shape[:-1]
-        row_max, row_sum = q.new_empty(rows, dtype=torch.float32), q.new_empty(rows, dtype=torch.float32)
+        rows, steps = q.shape[:-1], (heads, 1) if q.dim() == 3 else (tq * heads, heads, 1)
+        row_max = torch.empty_strided(rows, steps, device=dev, dtype=torch.float32)
+        row_sum = torch.empty_strided(rows, steps, device=dev, dtype=torch.float32)
         qs = q.stride() if q.dim() == 4 else (q.stride(0), 0, q.stride(1), 1)
         a = N.RelayCacheAttentionArgs(c, n, tq, heads, page_table.shape[1], 0, prefix_len,
                                       prefix_pages.shape[0] if prefix_len else 0, _dtype_code(q), scale, _ptr(q), qs,
