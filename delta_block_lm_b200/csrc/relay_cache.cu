@@ -22,8 +22,8 @@ struct AppendParams {
     int64_t ks[3], vs[3];  // strides of sequence, token and head
     const int32_t *lengths, *counts;
     int32_t* new_lengths;
-    int N, T, tiles;  // tiles: that T tokens can touch
-    bool vec;         // 16-byte loads
+    int T, tiles, blocks;  // tiles that T tokens can touch; blocks of a sequence
+    bool vec;              // 16-byte loads
     int* err;
 };
 
@@ -31,7 +31,7 @@ struct ReadParams {
     CacheView c;
     void *k, *v;
     const int32_t *lengths, *start;
-    int N, T;
+    int T, tiles, blocks;
     int* err;
 };
 
@@ -115,26 +115,18 @@ template <int D, typename T>
 __global__ void __launch_bounds__(256) cache_append_kernel(const AppendParams p) {
     using At = TileAt<D>;
     constexpr int LPT = D / 8;  // lanes of a token and head
-    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    const int64_t row = i / LPT;  // (sequence, token, head)
-    const int part = (int)(i % LPT);
-    const int64_t rows = (int64_t)p.N * p.T * p.c.heads;
-    if (p.new_lengths && i < p.N) {
-        const int cnt = p.counts ? min(max(p.counts[i], 0), p.T) : p.T;
-        p.new_lengths[i] = p.lengths[i] + cnt;
-    }
+    const int64_t n = blockIdx.x / p.blocks;
+    const int i = blockIdx.x % p.blocks * 256 + threadIdx.x, row = i / LPT, part = i % LPT;  // row: (token, head)
+    const int count = p.counts ? min(max(p.counts[n], 0), p.T) : p.T, len = p.lengths[n];
+    if (p.new_lengths && i == 0) p.new_lengths[n] = len + count;
     // lanes past the end go along with the first row and write nothing: the shuffles need whole groups
-    const bool inside = row < rows;
-    const int h = inside ? (int)(row % p.c.heads) : 0;
-    const int64_t nt = inside ? row / p.c.heads : 0;
-    const int t = (int)(nt % p.T);
-    const int64_t n = nt / p.T;
+    const bool inside = row < p.T * p.c.heads;
+    const int t = inside ? row / p.c.heads : 0, h = inside ? row - t * p.c.heads : 0;
     float x[8], y[8];
     load8<T>(static_cast<const T*>(p.k) + n * p.ks[0] + t * p.ks[1] + h * p.ks[2] + part * 8, p.vec, x);
     load8<T>(static_cast<const T*>(p.v) + n * p.vs[0] + t * p.vs[1] + h * p.vs[2] + part * 8, p.vec, y);
-    const int count = p.counts ? min(max(p.counts[n], 0), p.T) : p.T;
     const bool live = inside && t < count;
-    const int pos = p.lengths[n] + t;
+    const int pos = len + t;
     const int page = live && pos >= 0 ? cache_page(p.c, n, pos / kCacheTile) : -1;
     if (live && page < 0) atomicExch(p.err, kCacheErrorPage);
     const int k = pos & (kCacheTile - 1);
@@ -270,18 +262,15 @@ __device__ __forceinline__ void decode8(uint32_t codes, uint32_t word, float (&x
         x[i] = fmaf(s, __uint_as_float((codes >> (4 * i) & 15u) | 0x4B000000u) - 8388608.f, m);
 }
 
+// Single tokens: as the append.
 template <int D, typename T>
 __global__ void __launch_bounds__(256) cache_read_kernel(const ReadParams p) {
     using At = TileAt<D>;
     constexpr int LPT = D / 8;
-    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    const int64_t row = i / LPT;
-    const int part = (int)(i % LPT);
-    if (row >= (int64_t)p.N * p.T * p.c.heads) return;
-    const int h = (int)(row % p.c.heads);
-    const int64_t nt = row / p.c.heads;
-    const int t = (int)(nt % p.T);
-    const int64_t n = nt / p.T;
+    const int64_t n = blockIdx.x / p.blocks;
+    const int i = blockIdx.x % p.blocks * 256 + threadIdx.x, row = i / LPT, part = i % LPT;
+    if (row >= p.T * p.c.heads) return;
+    const int t = row / p.c.heads, h = row - t * p.c.heads;
     const int64_t pos = (p.start ? (int64_t)p.start[n] : 0) + t;
     const bool live = pos >= 0 && pos < p.lengths[n];
     const int page = live ? cache_page(p.c, n, (int)(pos / kCacheTile)) : -1;
@@ -297,11 +286,83 @@ __global__ void __launch_bounds__(256) cache_read_kernel(const ReadParams p) {
         const uint32_t hi = *reinterpret_cast<const uint16_t*>(tile + At::value_half(k, 2 * q + 1, j));
         decode8(lo | hi << 16, *reinterpret_cast<const uint32_t*>(tile + At::value_group(k, j)), xv);
     }
-    store8<T>(static_cast<T*>(p.k) + row * D + part * 8, xk);
-    store8<T>(static_cast<T*>(p.v) + row * D + part * 8, xv);
+    const int64_t at = ((n * p.T + t) * p.c.heads + h) * D + part * 8;
+    store8<T>(static_cast<T*>(p.k) + at, xk);
+    store8<T>(static_cast<T*>(p.v) + at, xv);
 }
 
-unsigned blocks_for(int64_t threads, int block) { return (unsigned)((threads + block - 1) / block); }
+// Runs of tokens: a CTA reads one tile of positions for kTileHeads heads, the tiles in 16-byte words through
+// shared memory, the next one on its way meanwhile.  One thread: 16 channels of one token's key or value.
+template <int D, typename T>
+__global__ void __launch_bounds__(256) cache_read_tiles_kernel(const ReadParams p) {
+    using At = TileAt<D>;
+    constexpr int TB = cache_tile_bytes(D), LPT = D / 16, HP = 128 / D, WORDS = HP * TB / 16;
+    __shared__ __align__(16) uint8_t image[2][HP * TB];
+    const int hg = (p.c.heads + kTileHeads - 1) / kTileHeads;
+    int64_t b = blockIdx.x;
+    const int h0 = (int)(b % hg) * kTileHeads, h1 = min(h0 + kTileHeads, p.c.heads);
+    b /= hg;
+    const int64_t n = b / p.tiles;
+    const int first = p.start ? p.start[n] : 0, len = p.lengths[n];
+    const int tl = (first >= 0 ? first / kCacheTile : -((-first + kCacheTile - 1) / kCacheTile)) + (int)(b % p.tiles);
+    const int t0 = tl * kCacheTile - first;  // token of place 0
+    if (t0 >= p.T) return;
+    const bool any = tl >= 0 && tl * kCacheTile < len;
+    const int page = any ? cache_page(p.c, n, tl) : -1;
+    if (any && page < 0 && threadIdx.x == 0) atomicExch(p.err, kCacheErrorPage);
+    const int i = threadIdx.x, hp = i / (2 * D), which = i / D % 2, k = i / LPT % kCacheTile, part = i % LPT;
+    const int t = t0 + k, j = part / 2, q = part % 2;
+    const bool wanted = t >= 0 && t < p.T, held = page >= 0 && first + t < len;
+    const uint8_t* from = cache_tile<D>(p.c, max(page, 0), h0, max(tl, 0) % p.c.tiles);
+    const int64_t per = (int64_t)p.c.tiles * TB;  // from head to head
+    uint4 raw = make_uint4(0, 0, 0, 0);
+    auto load = [&](int h) {
+        const int hh = i / (TB / 16);
+        if (page >= 0 && i < WORDS && h + hh < h1)
+            raw = __ldg(reinterpret_cast<const uint4*>(from + (h + hh - h0) * per) + i % (TB / 16));
+    };
+    load(h0);
+    int buf = 0;
+    for (int h = h0; h < h1; h += HP, buf ^= 1) {
+        if (i < WORDS) reinterpret_cast<uint4*>(image[buf])[i] = raw;
+        if (h + HP < h1) load(h + HP);
+        __syncthreads();  // two images, one barrier each
+        if (!wanted || h + hp >= h1) continue;
+        const uint8_t* img = image[buf] + hp * TB;
+        float x[2][8] = {};
+        if (held) {
+            uint32_t word;
+            uint32_t codes[2];
+            if (which) {
+                word = *reinterpret_cast<const uint32_t*>(img + At::value_group(k, j));
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+                    codes[e] = *reinterpret_cast<const uint16_t*>(img + At::value_half(k, 4 * q + 2 * e, j)) |
+                               (uint32_t)*reinterpret_cast<const uint16_t*>(img + At::value_half(k, 4 * q + 2 * e + 1, j)) << 16;
+            } else {
+                word = *reinterpret_cast<const uint32_t*>(img + At::key_group(k, j));
+#pragma unroll
+                for (int e = 0; e < 2; ++e) codes[e] = *reinterpret_cast<const uint32_t*>(img + At::key_word(k, 2 * q + e, j));
+            }
+            decode8(codes[0], word, x[0]);
+            decode8(codes[1], word, x[1]);
+        }
+        T* to = static_cast<T*>(which ? p.v : p.k) + ((n * p.T + t) * p.c.heads + h + hp) * D + part * 16;
+        store8<T>(to, x[0]);
+        store8<T>(to + 8, x[1]);
+    }
+}
+
+// Tiles or single tokens, and the grid; false where it is too large.
+bool grid_for(int64_t n_seq, int64_t tokens, int64_t heads, int D, int& tiles, int& blocks, bool& by_tiles, unsigned& grid) {
+    if (tokens > 0x7ffffff0 || tokens * heads > 0x7fffffff / D) return false;
+    tiles = (int)((tokens + 2 * kCacheTile - 2) / kCacheTile);
+    blocks = (int)((tokens * heads * (D / 8) + 255) / 256);
+    by_tiles = tokens >= kTileTokens;
+    const int64_t ctas = n_seq * (by_tiles ? tiles * ((heads + kTileHeads - 1) / kTileHeads) : (int64_t)blocks);
+    grid = (unsigned)ctas;
+    return ctas <= 0x7fffffff;
+}
 
 int check_table(const int32_t* table, int64_t n_seq, int64_t width, int64_t stride, const char* what) {
     if (n_seq <= 0) return fail(DBL_ERR_INVALID_ARGUMENT, "%s: n_seq must be positive", what);
@@ -356,9 +417,6 @@ extern "C" int dbl_relay_cache_append(const dbl_relay_cache_append_args* a, dbl_
     resolve_strides(a->v_stride, dims, 4, vs);
     if (ks[3] != 1 || vs[3] != 1)
         return fail(DBL_ERR_INVALID_ARGUMENT, "relay cache append: the innermost stride of k and v must be 1");
-    const int64_t threads = a->n_seq * a->tokens * a->cache.kv_heads * (D / 8);
-    if (a->tokens > 0x7fffffff || threads / 256 > 0x7ffffff0)
-        return fail(DBL_ERR_UNSUPPORTED, "relay cache append: grid too large");
     AppendParams p{};
     p.c = cache_view(&a->cache, a->page_table, a->table_width, a->table_stride);
     p.k = a->k;
@@ -367,19 +425,17 @@ extern "C" int dbl_relay_cache_append(const dbl_relay_cache_append_args* a, dbl_
     p.lengths = a->lengths;
     p.counts = a->counts;
     p.new_lengths = a->new_lengths;
-    p.N = (int)a->n_seq;
     p.T = (int)a->tokens;
-    rc = device_error_record(&p.err);
-    if (rc != DBL_OK) return rc;
     // 16-byte loads where every row of k and v starts on 16 bytes
     const int64_t per = 16 / (int64_t)dtype_size(a->dtype);
     p.vec = aligned(a->k, 16) && aligned(a->v, 16);
     for (int i = 0; i < 3; ++i) p.vec = p.vec && ks[i] % per == 0 && vs[i] % per == 0;
-    p.tiles = (int)((a->tokens + 2 * kCacheTile - 2) / kCacheTile);
-    const int64_t ctas = a->n_seq * p.tiles * ((a->cache.kv_heads + kTileHeads - 1) / kTileHeads);
-    const bool tiles = a->tokens >= kTileTokens;
-    if (tiles && ctas > 0x7fffffff) return fail(DBL_ERR_UNSUPPORTED, "relay cache append: grid too large");
-    const unsigned grid = tiles ? (unsigned)ctas : blocks_for(threads, 256);
+    bool tiles;
+    unsigned grid;
+    if (!grid_for(a->n_seq, a->tokens, a->cache.kv_heads, D, p.tiles, p.blocks, tiles, grid))
+        return fail(DBL_ERR_UNSUPPORTED, "relay cache append: grid too large");
+    rc = device_error_record(&p.err);
+    if (rc != DBL_OK) return rc;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
     const auto launch = [&](auto kernel) { kernel<<<grid, 256, 0, st>>>(p); };
     if (a->dtype == DBL_BF16) {
@@ -406,27 +462,27 @@ extern "C" int dbl_relay_cache_read(const dbl_relay_cache_read_args* a, dbl_stre
     if (!aligned(a->k, 16) || !aligned(a->v, 16))
         return fail(DBL_ERR_INVALID_ARGUMENT, "relay cache read: k and v must be 16-byte aligned");
     const int D = (int)a->cache.head_dim;
-    const int64_t threads = a->n_seq * a->tokens * a->cache.kv_heads * (D / 8);
-    if (a->tokens > 0x7fffffff || threads / 256 > 0x7ffffff0)
-        return fail(DBL_ERR_UNSUPPORTED, "relay cache read: grid too large");
     ReadParams p{};
     p.c = cache_view(&a->cache, a->page_table, a->table_width, a->table_stride);
     p.k = a->k;
     p.v = a->v;
     p.lengths = a->lengths;
     p.start = a->start;
-    p.N = (int)a->n_seq;
     p.T = (int)a->tokens;
+    bool tiles;
+    unsigned grid;
+    if (!grid_for(a->n_seq, a->tokens, a->cache.kv_heads, D, p.tiles, p.blocks, tiles, grid))
+        return fail(DBL_ERR_UNSUPPORTED, "relay cache read: grid too large");
     rc = device_error_record(&p.err);
     if (rc != DBL_OK) return rc;
-    const unsigned grid = blocks_for(threads, 256);
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
+    const auto launch = [&](auto kernel) { kernel<<<grid, 256, 0, st>>>(p); };
     if (a->dtype == DBL_BF16) {
-        if (D == 128) cache_read_kernel<128, __nv_bfloat16><<<grid, 256, 0, st>>>(p);
-        else cache_read_kernel<64, __nv_bfloat16><<<grid, 256, 0, st>>>(p);
+        if (D == 128) launch(tiles ? cache_read_tiles_kernel<128, __nv_bfloat16> : cache_read_kernel<128, __nv_bfloat16>);
+        else launch(tiles ? cache_read_tiles_kernel<64, __nv_bfloat16> : cache_read_kernel<64, __nv_bfloat16>);
     } else {
-        if (D == 128) cache_read_kernel<128, float><<<grid, 256, 0, st>>>(p);
-        else cache_read_kernel<64, float><<<grid, 256, 0, st>>>(p);
+        if (D == 128) launch(tiles ? cache_read_tiles_kernel<128, float> : cache_read_kernel<128, float>);
+        else launch(tiles ? cache_read_tiles_kernel<64, float> : cache_read_kernel<64, float>);
     }
     return launch_status("cache_read_kernel");
 }
