@@ -35,6 +35,12 @@ struct ReadParams {
     int* err;
 };
 
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN where one of them is
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
 // Codes of NC channels of a group, of which 32 / NC neighbouring lanes hold NC each: 8 to a word, the
 // first in the lowest four bits.  Returns the group's (scale, minimum) word.
 //
@@ -44,19 +50,16 @@ struct ReadParams {
 // 2^24 of them) and says which.
 template <int NC>
 __device__ __forceinline__ uint32_t encode(const float (&x)[NC], uint32_t (&codes)[NC / 8]) {
-    // fminf and fmaxf pass over a NaN, the sum does not
-    float lo = x[0], hi = x[0], sum = x[0];
+    float lo = x[0], hi = x[0];
 #pragma unroll
     for (int i = 1; i < NC; ++i) {
         lo = fminf(lo, x[i]);
-        hi = fmaxf(hi, x[i]);
-        sum += x[i];
+        hi = max_nan(hi, x[i]);
     }
 #pragma unroll
     for (int o = 1; o < 32 / NC; o <<= 1) {
         lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-        hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-        sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        hi = max_nan(hi, __shfl_xor_sync(0xffffffffu, hi, o));
     }
     uint32_t lb = __float_as_uint(lo);
     lb = (lb & 0x80000000u) ? (lb + 0xFFFFu) & 0xFFFF0000u : lb & 0xFFFF0000u;
@@ -64,7 +67,7 @@ __device__ __forceinline__ uint32_t encode(const float (&x)[NC], uint32_t (&code
     const float span = hi - base;
     uint32_t sb = (__float_as_uint(__fdiv_rn(span, 15.f)) + 0xFFFFu) & 0xFFFF0000u;
     if (span < 7.888609052e-31f) sb = 0;  // 2^-100
-    const bool bad = sum != sum || !(span <= 3.402823466e38f);
+    const bool bad = !(span <= 3.402823466e38f);  // NaN too
     const float s = __uint_as_float(sb), half = 0.5f * s;
     float inv;
     asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
@@ -76,10 +79,10 @@ __device__ __forceinline__ uint32_t encode(const float (&x)[NC], uint32_t (&code
 #pragma unroll
         for (int i = 7; i >= 0; --i) {
             const float d = x[8 * w + i] - base, t = fmaf(d, inv, kRound);
-            const uint32_t more = fmaf(kRound - t, s, d) > half ? 1u : 0u;
-            word = word * 16u + (__float_as_uint(t) + more - __float_as_uint(kRound));
+            word = word * 16u + __float_as_uint(t);
+            if (fmaf(kRound - t, s, d) > half) ++word;
         }
-        codes[w] = bad || sb == 0 ? 0u : word;
+        codes[w] = bad || sb == 0 ? 0u : word - __float_as_uint(kRound) * 0x11111111u;  // kRound's bits of all eight
     }
     return bad ? 0x7FFF0000u /* scale 0, minimum NaN */ : (sb >> 16) | lb;
 }
@@ -157,14 +160,13 @@ __global__ void __launch_bounds__(256) cache_append_tiles_kernel(const AppendPar
     constexpr int TB = cache_tile_bytes(D), LPT = D / 16, HP = 128 / D;  // lanes of a token, heads of a pass
     constexpr int NW = 16 / (16 / (int)sizeof(T));                       // 16-byte words of 16 channels
     __shared__ __align__(16) uint8_t image[2][HP * TB];
-    const int hg = (p.c.heads + kTileHeads - 1) / kTileHeads;
-    int64_t b = blockIdx.x;
-    const int h0 = (int)(b % hg) * kTileHeads, h1 = min(h0 + kTileHeads, p.c.heads);
-    b /= hg;
-    const int64_t n = b / p.tiles;
+    const unsigned hg = (p.c.heads + kTileHeads - 1) / kTileHeads;
+    const unsigned b = blockIdx.x / hg, tn = b / p.tiles;
+    const int h0 = (int)(blockIdx.x - b * hg) * kTileHeads, h1 = min(h0 + kTileHeads, p.c.heads), ti = (int)(b - tn * p.tiles);
+    const int64_t n = tn;
     const int count = p.counts ? min(max(p.counts[n], 0), p.T) : p.T, len = p.lengths[n];
-    if (p.new_lengths && b % p.tiles == 0 && h0 == 0 && threadIdx.x == 0) p.new_lengths[n] = len + count;
-    const int tl = max(len, 0) / kCacheTile + (int)(b % p.tiles), t0 = tl * kCacheTile - len;  // token of place 0
+    if (p.new_lengths && ti == 0 && h0 == 0 && threadIdx.x == 0) p.new_lengths[n] = len + count;
+    const int tl = max(len, 0) / kCacheTile + ti, t0 = tl * kCacheTile - len;  // token of place 0
     if (t0 >= count || len < 0) return;
     const int page = cache_page(p.c, n, tl);
     if (page < 0) {
@@ -298,13 +300,12 @@ __global__ void __launch_bounds__(256) cache_read_tiles_kernel(const ReadParams 
     using At = TileAt<D>;
     constexpr int TB = cache_tile_bytes(D), LPT = D / 16, HP = 128 / D, WORDS = HP * TB / 16;
     __shared__ __align__(16) uint8_t image[2][HP * TB];
-    const int hg = (p.c.heads + kTileHeads - 1) / kTileHeads;
-    int64_t b = blockIdx.x;
-    const int h0 = (int)(b % hg) * kTileHeads, h1 = min(h0 + kTileHeads, p.c.heads);
-    b /= hg;
-    const int64_t n = b / p.tiles;
+    const unsigned hg = (p.c.heads + kTileHeads - 1) / kTileHeads;
+    const unsigned b = blockIdx.x / hg, tn = b / p.tiles;
+    const int h0 = (int)(blockIdx.x - b * hg) * kTileHeads, h1 = min(h0 + kTileHeads, p.c.heads), ti = (int)(b - tn * p.tiles);
+    const int64_t n = tn;
     const int first = p.start ? p.start[n] : 0, len = p.lengths[n];
-    const int tl = (first >= 0 ? first / kCacheTile : -((-first + kCacheTile - 1) / kCacheTile)) + (int)(b % p.tiles);
+    const int tl = (first >= 0 ? first / kCacheTile : -((-first + kCacheTile - 1) / kCacheTile)) + ti;
     const int t0 = tl * kCacheTile - first;  // token of place 0
     if (t0 >= p.T) return;
     const bool any = tl >= 0 && tl * kCacheTile < len;
@@ -329,24 +330,22 @@ __global__ void __launch_bounds__(256) cache_read_tiles_kernel(const ReadParams 
         __syncthreads();  // two images, one barrier each
         if (!wanted || h + hp >= h1) continue;
         const uint8_t* img = image[buf] + hp * TB;
-        float x[2][8] = {};
-        if (held) {
-            uint32_t word;
-            uint32_t codes[2];
-            if (which) {
-                word = *reinterpret_cast<const uint32_t*>(img + At::value_group(k, j));
+        float x[2][8];
+        uint32_t word, codes[2];
+        if (which) {
+            word = *reinterpret_cast<const uint32_t*>(img + At::value_group(k, j));
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
-                    codes[e] = *reinterpret_cast<const uint16_t*>(img + At::value_half(k, 4 * q + 2 * e, j)) |
-                               (uint32_t)*reinterpret_cast<const uint16_t*>(img + At::value_half(k, 4 * q + 2 * e + 1, j)) << 16;
-            } else {
-                word = *reinterpret_cast<const uint32_t*>(img + At::key_group(k, j));
+            for (int e = 0; e < 2; ++e)
+                codes[e] = *reinterpret_cast<const uint16_t*>(img + At::value_half(k, 4 * q + 2 * e, j)) |
+                           (uint32_t)*reinterpret_cast<const uint16_t*>(img + At::value_half(k, 4 * q + 2 * e + 1, j)) << 16;
+        } else {
+            word = *reinterpret_cast<const uint32_t*>(img + At::key_group(k, j));
 #pragma unroll
-                for (int e = 0; e < 2; ++e) codes[e] = *reinterpret_cast<const uint32_t*>(img + At::key_word(k, 2 * q + e, j));
-            }
-            decode8(codes[0], word, x[0]);
-            decode8(codes[1], word, x[1]);
+            for (int e = 0; e < 2; ++e) codes[e] = *reinterpret_cast<const uint32_t*>(img + At::key_word(k, 2 * q + e, j));
         }
+        if (!held) word = 0;  // zero, whatever the codes
+        decode8(codes[0], word, x[0]);
+        decode8(codes[1], word, x[1]);
         T* to = static_cast<T*>(which ? p.v : p.k) + ((n * p.T + t) * p.c.heads + h + hp) * D + part * 16;
         store8<T>(to, x[0]);
         store8<T>(to + 8, x[1]);
