@@ -293,13 +293,13 @@ __global__ void __launch_bounds__(256) cache_read_kernel(const ReadParams p) {
     store8<T>(static_cast<T*>(p.v) + at, xv);
 }
 
-// Runs of tokens: a CTA reads one tile of positions for kTileHeads heads, the tiles in 16-byte words through
-// shared memory, the next one on its way meanwhile.  One thread: 16 channels of one token's key or value.
+// Runs of tokens: a CTA reads one tile of positions for kTileHeads heads, all of them at once in 16-byte
+// words to shared memory.  One thread: 16 channels of one token's key or value.
 template <int D, typename T>
 __global__ void __launch_bounds__(256) cache_read_tiles_kernel(const ReadParams p) {
     using At = TileAt<D>;
-    constexpr int TB = cache_tile_bytes(D), LPT = D / 16, HP = 128 / D, WORDS = HP * TB / 16;
-    __shared__ __align__(16) uint8_t image[2][HP * TB];
+    constexpr int TB = cache_tile_bytes(D), LPT = D / 16, HP = 128 / D, WORDS = TB / 16;
+    __shared__ __align__(16) uint8_t image[kTileHeads * TB];
     const unsigned hg = (p.c.heads + kTileHeads - 1) / kTileHeads;
     const unsigned b = blockIdx.x / hg, tn = b / p.tiles;
     const int h0 = (int)(blockIdx.x - b * hg) * kTileHeads, h1 = min(h0 + kTileHeads, p.c.heads), ti = (int)(b - tn * p.tiles);
@@ -316,20 +316,22 @@ __global__ void __launch_bounds__(256) cache_read_tiles_kernel(const ReadParams 
     const bool wanted = t >= 0 && t < p.T, held = page >= 0 && first + t < len;
     const uint8_t* from = cache_tile<D>(p.c, max(page, 0), h0, max(tl, 0) % p.c.tiles);
     const int64_t per = (int64_t)p.c.tiles * TB;  // from head to head
-    uint4 raw = make_uint4(0, 0, 0, 0);
-    auto load = [&](int h) {
-        const int hh = i / (TB / 16);
-        if (page >= 0 && i < WORDS && h + hh < h1)
-            raw = __ldg(reinterpret_cast<const uint4*>(from + (h + hh - h0) * per) + i % (TB / 16));
-    };
-    load(h0);
-    int buf = 0;
-    for (int h = h0; h < h1; h += HP, buf ^= 1) {
-        if (i < WORDS) reinterpret_cast<uint4*>(image[buf])[i] = raw;
-        if (h + HP < h1) load(h + HP);
-        __syncthreads();  // two images, one barrier each
-        if (!wanted || h + hp >= h1) continue;
-        const uint8_t* img = image[buf] + hp * TB;
+    if (page >= 0) {
+        const int words = (h1 - h0) * WORDS;
+        uint4 raw[(kTileHeads * WORDS + 255) / 256];
+#pragma unroll
+        for (int w = 0; w < (kTileHeads * WORDS + 255) / 256; ++w) {
+            const int at = i + 256 * w, hh = at / WORDS;
+            if (at < words) raw[w] = __ldg(reinterpret_cast<const uint4*>(from + hh * per) + (at - hh * WORDS));
+        }
+#pragma unroll
+        for (int w = 0; w < (kTileHeads * WORDS + 255) / 256; ++w)
+            if (i + 256 * w < words) reinterpret_cast<uint4*>(image)[i + 256 * w] = raw[w];
+    }
+    __syncthreads();
+    if (!wanted) return;
+    for (int h = h0 + hp; h < h1; h += HP) {
+        const uint8_t* img = image + (h - h0) * TB;
         float x[2][8];
         uint32_t word, codes[2];
         if (which) {
@@ -346,7 +348,7 @@ __global__ void __launch_bounds__(256) cache_read_tiles_kernel(const ReadParams 
         if (!held) word = 0;  // zero, whatever the codes
         decode8(codes[0], word, x[0]);
         decode8(codes[1], word, x[1]);
-        T* to = static_cast<T*>(which ? p.v : p.k) + ((n * p.T + t) * p.c.heads + h + hp) * D + part * 16;
+        T* to = static_cast<T*>(which ? p.v : p.k) + ((n * p.T + t) * p.c.heads + h) * D + part * 16;
         store8<T>(to, x[0]);
         store8<T>(to + 8, x[1]);
     }
