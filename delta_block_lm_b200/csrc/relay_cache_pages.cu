@@ -7,8 +7,8 @@
 // and integer atomics only count and take maxima, so the results do not depend on the order in which
 // threads run.
 //
-// The integer work is one thread-block cluster (8 CTAs of 1024 threads): its phases are separated by
-// the cluster's barrier, which orders global memory among its threads, so each call is one launch
+// The integer work is one CTA of 1024 threads, or for large states a cluster of 8: its phases are
+// separated by the barrier, which orders global memory among its threads, so each call is one launch
 // (two with the copies of page data, which use the whole GPU).
 #include "relay_cache.cuh"
 #include "tc_ptx.cuh"
@@ -19,8 +19,12 @@ int cache_check_table(const int32_t* table, int64_t n_seq, int64_t width, int64_
 
 namespace {
 
-constexpr int CL = 8, CT = 1024;       // CTAs of the cluster, threads of a CTA
-constexpr int NT = CL * CT, NWARP = NT / 32;
+constexpr int CT = 1024;             // threads of a CTA
+constexpr int MOST_WARPS = 8 * CT / 32;
+// Table entries and pages that one CTA deals with.  Measured, release + fork + reserve: 8 sequences (100
+// entries and pages) 15 us by one CTA, 23 us by eight; 32 sequences (2 K) 21 and 26 us; 256 sequences (14 K)
+// 73 and 36 us.
+constexpr int64_t kSmallState = 4096;
 
 struct PageParams {
     const int32_t *table, *lengths, *refs;      // before
@@ -35,8 +39,10 @@ struct PageParams {
     int* err;
 };
 
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+template <int CL>  // CTAs of the launch
+__device__ __forceinline__ void sync_all() {
+    if constexpr (CL == 1) __syncthreads();
+    else asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
 }
 __device__ __forceinline__ int gtid() { return blockIdx.x * CT + threadIdx.x; }
 __device__ __forceinline__ int gwarp() { return gtid() >> 5; }
@@ -56,7 +62,10 @@ __device__ __forceinline__ int warp_total(const int32_t* v, int count) {
 }
 __device__ __forceinline__ int64_t entry(const PageParams& p, int s, int w) { return (int64_t)s * p.stride + w; }
 
+template <int CL>
 __device__ void copy_state(const PageParams& p, bool lengths) {
+    constexpr int NT = CL * CT;
+    // in place there is nothing to copy
     if (p.table_out != p.table)
         for (int64_t i = gtid(); i < (int64_t)p.S * p.W; i += NT) {
             const int s = (int)(i / p.W), w = (int)(i % p.W);
@@ -69,9 +78,11 @@ __device__ void copy_state(const PageParams& p, bool lengths) {
 }
 
 // a = the sequences to release.  An entry that two list items name is released once.
+template <int CL>
 __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(CT, 1) cache_release_kernel(const PageParams p) {
-    copy_state(p, true);
-    cluster_sync();
+    constexpr int NT = CL * CT;
+    copy_state<CL>(p, true);
+    sync_all<CL>();
     for (int64_t i = gtid(); i < (int64_t)p.n * p.W; i += NT) {
         const int s = p.a[i / p.W];
         if (s < 0 || s >= p.S) {
@@ -85,9 +96,11 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(CT, 1) cache_releas
 }
 
 // a = parents, b = children (empty sequences, each named once, none of them a parent).
+template <int CL>
 __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(CT, 1) cache_fork_kernel(const PageParams p) {
-    copy_state(p, true);
-    cluster_sync();
+    constexpr int NT = CL * CT;
+    copy_state<CL>(p, true);
+    sync_all<CL>();
     for (int64_t i = gtid(); i < (int64_t)p.n * p.W; i += NT) {
         const int from = p.a[i / p.W], to = p.b[i / p.W], w = (int)(i % p.W);
         if (from < 0 || from >= p.S || to < 0 || to >= p.S || from == to) {
@@ -104,10 +117,13 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(CT, 1) cache_fork_k
 
 // b = tokens of each sequence, or null: p.tokens of each.
 //   scratch: asked [P], last [P], list [P], src [S], dst [S], tiles [S], free [NWARP], want [NWARP]
+template <int CL>
 __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(CT, 1) cache_reserve_kernel(const PageParams p) {
+    constexpr int NT = CL * CT, NWARP = NT / 32;
     int32_t *asked = p.scratch, *last = asked + p.P, *list = last + p.P;
     int32_t *src = list + p.P, *dst = src + p.S, *tiles = dst + p.S, *nfree = tiles + p.S, *nwant = nfree + NWARP;
     const int warp = gwarp(), lane = lane_id();
+    copy_state<CL>(p, false);
     // the page in which the next token of sequence s falls, where it holds tokens already
     auto partial = [&](int s, int& len, int& add) -> int {
         len = max(p.lengths[s], 0);
@@ -121,7 +137,7 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(CT, 1) cache_reserv
         const int page = partial(s, len, add);
         if (page >= 0) asked[page] = 0, last[page] = -1;
     }
-    cluster_sync();
+    sync_all<CL>();
     for (int s = gtid(); s < p.S; s += NT) {
         const int page = partial(s, len, add);
         if (page >= 0) {
@@ -129,7 +145,7 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(CT, 1) cache_reserv
             atomicMax(last + page, s);
         }
     }
-    cluster_sync();
+    sync_all<CL>();
     // A holder copies the page it is about to write where others hold it too; if all of its holders
     // are about to write, the last of them keeps it.
     auto copies = [&](int s, int page) {
@@ -163,7 +179,7 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(CT, 1) cache_reserv
         nwant[warp] = want;
         if (beyond) atomicExch(p.err, kCacheErrorPage);
     }
-    cluster_sync();
+    sync_all<CL>();
     const int total_want = warp_total(nwant, NWARP), total_free = warp_total(nfree, NWARP);
     const bool ok = total_want <= total_free;
     if (gtid() == 0) p.result[0] = ok ? 0 : total_want - total_free;
@@ -175,9 +191,7 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(CT, 1) cache_reserv
         if (f && r < total_want) list[r] = i + lane;
         at += __popc(m);
     }
-    cluster_sync();
-    copy_state(p, false);
-    cluster_sync();
+    sync_all<CL>();
     at = warp_total(nwant, warp);
     for (int s = s0; s < s1; ++s) {
         partial(s, len, add);
@@ -207,7 +221,9 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(CT, 1) cache_reserv
 
 // Pages in use move to the front: the i-th page in use at or past `used` goes to the i-th free page
 // below it.   scratch: count [2], src [P], dst [P], to [P], inuse [NWARP]
+template <int CL>
 __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(CT, 1) cache_compact_kernel(const PageParams p) {
+    constexpr int NT = CL * CT, NWARP = NT / 32;
     int32_t *count = p.scratch, *src = count + 2, *dst = src + p.P, *to = dst + p.P, *inuse = to + p.P;
     const int warp = gwarp(), lane = lane_id();
     const int pages = (p.P + NWARP - 1) / NWARP, p0 = min(p.P, warp * pages), p1 = min(p.P, p0 + pages);
@@ -215,7 +231,7 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(CT, 1) cache_compac
     for (int i = p0 + lane; i < p1; i += 32) nu += p.refs[i] > 0;
     nu = wsum_i(nu);
     if (lane == 0) inuse[warp] = nu;
-    cluster_sync();
+    sync_all<CL>();
     const int used = warp_total(inuse, NWARP), before = warp_total(inuse, warp);
     if (gtid() == 0) p.result[0] = used;
     if (p0 <= used && used < p1) {  // pages in use below `used`
@@ -225,7 +241,7 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(CT, 1) cache_compac
         if (lane == 0) count[1] = before + c;
     }
     if (used == p.P && gtid() == 0) count[1] = used;
-    cluster_sync();
+    sync_all<CL>();
     const int below = ld(count + 1);
     if (gtid() == 0) count[0] = used - below;
     int at = before;
@@ -238,11 +254,11 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(CT, 1) cache_compac
         if (in && !u && page >= used) to[page] = page;  // no entry names it
         at += __popc(m);
     }
-    cluster_sync();
+    sync_all<CL>();
     for (int i = gtid(); i < used - below; i += NT) to[ld(src + i)] = ld(dst + i);
     if (p.refs_out != p.refs)
         for (int i = gtid(); i < p.P; i += NT) p.refs_out[i] = p.refs[i];
-    cluster_sync();
+    sync_all<CL>();
     for (int i = gtid(); i < used - below; i += NT) {
         const int a = ld(src + i);
         p.refs_out[ld(dst + i)] = ld(p.refs + a);
@@ -280,7 +296,16 @@ __global__ void __launch_bounds__(128) cache_copy_kernel(const CopyParams p) {
         const int64_t per = (int64_t)p.page_tiles * p.tile_words;
         const uint4* from = p.pool + ((int64_t)a * p.heads + h) * per;
         uint4* to = p.pool + ((int64_t)b * p.heads + h) * per;
-        for (int w = threadIdx.x; w < words; w += 128) to[w] = from[w];
+        constexpr int U = 5;  // words of a thread on their way at once: 10 KB of a page of 64 tokens
+        for (int w0 = threadIdx.x; w0 < words; w0 += 128 * U) {
+            uint4 x[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (w0 + 128 * u < words) x[u] = __ldcs(from + w0 + 128 * u);
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+                if (w0 + 128 * u < words) __stcs(to + w0 + 128 * u, x[u]);
+        }
     }
 }
 
@@ -325,7 +350,10 @@ int page_params(const dbl_relay_cache_pages_args* a, PageParams& p, const char* 
     return DBL_OK;
 }
 
-size_t page_scratch(int64_t P, int64_t S) { return (size_t)(4 * P + 3 * S + 2 * NWARP + 16) * sizeof(int32_t); }
+// One CTA, or a cluster.
+bool small_state(const PageParams& p) { return (int64_t)p.S * p.W + p.P <= kSmallState; }
+
+size_t page_scratch(int64_t P, int64_t S) { return (size_t)(4 * P + 3 * S + 2 * MOST_WARPS + 16) * sizeof(int32_t); }
 
 int check_scratch(const dbl_relay_cache_pages_args* a, PageParams& p, void* ws, size_t bytes, const char* what) {
     const size_t need = page_scratch(a->cache.pages, a->n_seq);
@@ -355,7 +383,9 @@ extern "C" int dbl_relay_cache_release(const dbl_relay_cache_pages_args* a, cons
     p.a = sequences;
     p.n = (int)count;
     if ((rc = device_error_record(&p.err)) != DBL_OK) return rc;
-    cache_release_kernel<<<CL, CT, 0, reinterpret_cast<cudaStream_t>(stream)>>>(p);
+    const auto st = reinterpret_cast<cudaStream_t>(stream);
+    if (small_state(p)) cache_release_kernel<1><<<1, CT, 0, st>>>(p);
+    else cache_release_kernel<8><<<8, CT, 0, st>>>(p);
     return launch_status("cache_release_kernel");
 }
 
@@ -372,7 +402,9 @@ extern "C" int dbl_relay_cache_fork(const dbl_relay_cache_pages_args* a, const i
     p.b = children;
     p.n = (int)count;
     if ((rc = device_error_record(&p.err)) != DBL_OK) return rc;
-    cache_fork_kernel<<<CL, CT, 0, reinterpret_cast<cudaStream_t>(stream)>>>(p);
+    const auto st = reinterpret_cast<cudaStream_t>(stream);
+    if (small_state(p)) cache_fork_kernel<1><<<1, CT, 0, st>>>(p);
+    else cache_fork_kernel<8><<<8, CT, 0, st>>>(p);
     return launch_status("cache_fork_kernel");
 }
 
@@ -391,7 +423,8 @@ extern "C" int dbl_relay_cache_reserve(const dbl_relay_cache_pages_args* a, cons
     p.result = missing;
     if ((rc = device_error_record(&p.err)) != DBL_OK) return rc;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    cache_reserve_kernel<<<CL, CT, 0, st>>>(p);
+    if (small_state(p)) cache_reserve_kernel<1><<<1, CT, 0, st>>>(p);
+    else cache_reserve_kernel<8><<<8, CT, 0, st>>>(p);
     if ((rc = launch_status("cache_reserve_kernel")) != DBL_OK) return rc;
     const int32_t* src = p.scratch + 3 * (int64_t)p.P;
     return launch_copy(a->cache, src, src + p.S, src + 2 * (int64_t)p.S, nullptr, p.S, p.err, st);
@@ -408,7 +441,8 @@ extern "C" int dbl_relay_cache_compact(const dbl_relay_cache_pages_args* a, int3
     p.result = used;
     if ((rc = device_error_record(&p.err)) != DBL_OK) return rc;
     cudaStream_t st = reinterpret_cast<cudaStream_t>(stream);
-    cache_compact_kernel<<<CL, CT, 0, st>>>(p);
+    if (small_state(p)) cache_compact_kernel<1><<<1, CT, 0, st>>>(p);
+    else cache_compact_kernel<8><<<8, CT, 0, st>>>(p);
     if ((rc = launch_status("cache_compact_kernel")) != DBL_OK) return rc;
     const int32_t* src = p.scratch + 2;
     return launch_copy(a->cache, src, src + p.P, nullptr, p.scratch, p.P, p.err, st);
