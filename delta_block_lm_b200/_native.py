@@ -210,18 +210,18 @@ EXPORTS = [
     ("dbl_gdn2_prefill_time_sharded", ctypes.c_int,
      [ctypes.POINTER(PrefillArgs), ctypes.c_int, ctypes.POINTER(ctypes.c_int), ctypes.POINTER(_vp), _i64,
       ctypes.POINTER(_vp), ctypes.POINTER(ctypes.c_size_t)]),
-    ("dbl_relay_cache_append", ctypes.c_int, [ctypes.POINTER(RelayCacheAppendArgs), _vp]),
-    ("dbl_relay_cache_read", ctypes.c_int, [ctypes.POINTER(RelayCacheReadArgs), _vp]),
-    ("dbl_relay_cache_attention_workspace_bytes", ctypes.c_size_t, [ctypes.POINTER(RelayCacheAttentionArgs)]),
+    ("dbl_relay_cache_append", ctypes.c_int, [_vp, _vp]),
+    ("dbl_relay_cache_read", ctypes.c_int, [_vp, _vp]),
+    ("dbl_relay_cache_attention_workspace_bytes", ctypes.c_size_t, [_vp]),
     ("dbl_relay_cache_attention", ctypes.c_int,
-     [ctypes.POINTER(RelayCacheAttentionArgs), _vp, ctypes.c_size_t, _vp]),
+     [_vp, _vp, ctypes.c_size_t, _vp]),
     ("dbl_relay_cache_pages_workspace_bytes", ctypes.c_size_t, [_i64, _i64]),
-    ("dbl_relay_cache_release", ctypes.c_int, [ctypes.POINTER(RelayCachePagesArgs), _vp, _i64, _vp]),
-    ("dbl_relay_cache_fork", ctypes.c_int, [ctypes.POINTER(RelayCachePagesArgs), _vp, _vp, _i64, _vp]),
+    ("dbl_relay_cache_release", ctypes.c_int, [_vp, _vp, _i64, _vp]),
+    ("dbl_relay_cache_fork", ctypes.c_int, [_vp, _vp, _vp, _i64, _vp]),
     ("dbl_relay_cache_reserve", ctypes.c_int,
-     [ctypes.POINTER(RelayCachePagesArgs), _vp, _i64, _vp, _vp, ctypes.c_size_t, _vp]),
+     [_vp, _vp, _i64, _vp, _vp, ctypes.c_size_t, _vp]),
     ("dbl_relay_cache_compact", ctypes.c_int,
-     [ctypes.POINTER(RelayCachePagesArgs), _vp, _vp, ctypes.c_size_t, _vp]),
+     [_vp, _vp, _vp, ctypes.c_size_t, _vp]),
     ("dbl_relay_cache_copy_pages", ctypes.c_int, [ctypes.POINTER(RelayCache), _vp, _vp, _i64, _vp]),
 ]
 

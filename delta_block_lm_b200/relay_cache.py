@@ -26,6 +26,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import struct
 from typing import Optional
 
 import torch
@@ -34,6 +35,25 @@ from . import _native as N
 from .kernels import _dtype_code, _ptr, _require_cuda
 
 TILE = 16  # tokens of one tile: page sizes are multiples of it
+
+
+def _packer(args):
+    """Packs the fields of an argument structure, one after another, into its bytes: a fifth of the time that
+    building the ctypes structure takes."""
+    codes = {ctypes.c_int64: "q", ctypes.c_int32: "i", ctypes.c_float: "f", ctypes.c_void_p: "P"}
+
+    def of(t):
+        if issubclass(t, ctypes.Structure):
+            return "".join(of(f) for _, f in t._fields_)
+        return f"{t._length_}{codes[t._type_]}" if issubclass(t, ctypes.Array) else codes[t]
+
+    packed = struct.Struct("@" + of(args) + "0q")
+    assert packed.size == ctypes.sizeof(args), args
+    return packed.pack
+
+
+_APPEND, _READ = _packer(N.RelayCacheAppendArgs), _packer(N.RelayCacheReadArgs)
+_ATTENTION, _PAGES = _packer(N.RelayCacheAttentionArgs), _packer(N.RelayCachePagesArgs)
 
 
 class _Here:
@@ -66,12 +86,14 @@ def relay_cache_pool(pages: int, kv_heads: int, head_dim: int, page_size: int = 
     return torch.zeros((pages, kv_heads, page_size // TILE, 20 * head_dim), device=device, dtype=torch.uint8)
 
 
-def _cache(pool: torch.Tensor) -> N.RelayCache:
-    if pool.dtype != torch.uint8 or pool.dim() != 4 or not pool.is_contiguous() or pool.shape[3] not in (1280, 2560):
+def _cache(pool: torch.Tensor) -> tuple:
+    """The fields of dbl_relay_cache: pages, kv heads, head width, page size, address."""
+    shape = pool.shape
+    if pool.dtype != torch.uint8 or len(shape) != 4 or not pool.is_contiguous() or shape[3] not in (1280, 2560):
         raise ValueError("relay cache: pool must be a contiguous uint8 [pages, kv_heads, page_size / 16, 20 head_dim]"
-                         f" with head_dim 64 or 128, got {pool.dtype} {list(pool.shape)}")
-    p, h, t, b = pool.shape
-    return N.RelayCache(p, h, b // 20, t * TILE, pool.data_ptr())
+                         f" with head_dim 64 or 128, got {pool.dtype} {list(shape)}")
+    p, h, t, b = shape
+    return p, h, b // 20, t * TILE, pool.data_ptr()
 
 
 def _ints(name: str, t: Optional[torch.Tensor], shape: tuple) -> Optional[torch.Tensor]:
@@ -82,6 +104,10 @@ def _ints(name: str, t: Optional[torch.Tensor], shape: tuple) -> Optional[torch.
     if t.dtype != torch.int32 or not t.is_contiguous():
         t = t.to(torch.int32).contiguous()
     return t
+
+
+def _at(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def _list(name: str, t: torch.Tensor) -> torch.Tensor:
@@ -96,15 +122,16 @@ def relay_cache_append(pool, page_table, lengths, k, v, *, counts=None, out=None
     how many of the T tokens are real (ragged prompts).  The pages must have been reserved."""
     dev = _require_cuda(pool, page_table, lengths, k, v, counts, out)
     c = _cache(pool)
-    n, t = k.shape[:2] if k.dim() == 4 else (0, 0)
-    if k.dim() != 4 or tuple(k.shape[2:]) != (c.kv_heads, c.head_dim) or k.shape != v.shape:
-        raise ValueError(f"relay cache append: k and v must be [N,T,{c.kv_heads},{c.head_dim}], got {list(k.shape)} and "
+    shape = k.shape
+    if len(shape) != 4 or shape[2:] != c[1:3] or shape != v.shape:
+        raise ValueError(f"relay cache append: k and v must be [N,T,{c[1]},{c[2]}], got {list(k.shape)} and "
                          f"{list(v.shape)}")
+    n, t = shape[:2]
     if v.dtype != k.dtype:
         raise ValueError("relay cache append: v must have the dtype of k")
     if page_table.dim() != 2 or page_table.shape[0] != n:
         raise ValueError(f"relay cache append: page_table must be [{n},width], got {list(page_table.shape)}")
-    page_table = _ints("page_table", page_table, tuple(page_table.shape))
+    page_table = _ints("page_table", page_table, page_table.shape)
     lengths, counts = _ints("lengths", lengths, (n,)), _ints("counts", counts, (n,))
     if t == 0 or n == 0:
         return lengths.clone() if out is None else out.copy_(lengths)
@@ -114,9 +141,9 @@ def relay_cache_append(pool, page_table, lengths, k, v, *, counts=None, out=None
         v = v.contiguous()
     with _on(dev):
         new = torch.empty_like(lengths)
-        a = N.RelayCacheAppendArgs(c, n, t, page_table.shape[1], 0, _dtype_code(k), _ptr(k), _ptr(v), k.stride(),
-                                   v.stride(), _ptr(page_table), _ptr(lengths), _ptr(counts), _ptr(new))
-        N.check(N.lib().dbl_relay_cache_append(ctypes.byref(a), _stream(dev)))
+        a = _APPEND(*c, n, t, page_table.shape[1], 0, _dtype_code(k), k.data_ptr(), v.data_ptr(), *k.stride(), *v.stride(),
+                    page_table.data_ptr(), lengths.data_ptr(), _at(counts), new.data_ptr())
+        N.check(N.lib().dbl_relay_cache_append(a, _stream(dev)))
         return new if out is None else out.copy_(new)
 
 
@@ -128,15 +155,15 @@ def relay_cache_read(pool, page_table, lengths, *, start=None, tokens: int, dtyp
     if page_table.dim() != 2:
         raise ValueError(f"relay cache read: page_table must be [N,width], got {list(page_table.shape)}")
     n = page_table.shape[0]
-    page_table = _ints("page_table", page_table, tuple(page_table.shape))
+    page_table = _ints("page_table", page_table, page_table.shape)
     lengths, start = _ints("lengths", lengths, (n,)), _ints("start", start, (n,))
     with _on(dev):
-        k = torch.empty((n, tokens, c.kv_heads, c.head_dim), device=dev, dtype=dtype)
+        k = torch.empty((n, tokens, c[1], c[2]), device=dev, dtype=dtype)
         v = torch.empty_like(k)
-        a = N.RelayCacheReadArgs(c, n, tokens, page_table.shape[1], 0, _dtype_code(k), _ptr(page_table), _ptr(lengths),
-                                 _ptr(start), _ptr(k), _ptr(v))
+        a = _READ(*c, n, tokens, page_table.shape[1], 0, _dtype_code(k), page_table.data_ptr(), lengths.data_ptr(),
+                  _at(start), k.data_ptr(), v.data_ptr())
         if k.numel():
-            N.check(N.lib().dbl_relay_cache_read(ctypes.byref(a), _stream(dev)))
+            N.check(N.lib().dbl_relay_cache_read(a, _stream(dev)))
     return k, v
 
 
@@ -169,8 +196,8 @@ def relay_cache_attention(q, pool, page_table, lengths, *, prefix_pages=None, pr
     without keys gives o = 0 and (0, 1)."""
     dev = _require_cuda(q, pool, page_table, lengths, prefix_pages, out, workspace)
     c = _cache(pool)
-    if q.dim() not in (3, 4) or q.shape[-1] != c.head_dim:
-        raise ValueError(f"relay cache attention: q must be [N,heads,{c.head_dim}] or [N,Tq,heads,{c.head_dim}], got "
+    if q.dim() not in (3, 4) or q.shape[-1] != c[2]:
+        raise ValueError(f"relay cache attention: q must be [N,heads,{c[2]}] or [N,Tq,heads,{c[2]}], got "
                          f"{list(q.shape)}")
     n, heads = q.shape[0], q.shape[-2]
     tq = q.shape[1] if q.dim() == 4 else 1
@@ -178,14 +205,14 @@ def relay_cache_attention(q, pool, page_table, lengths, *, prefix_pages=None, pr
         raise ValueError(f"relay cache attention: page_table must be [{n},width], got {list(page_table.shape)}")
     if prefix_len and (prefix_pages is None or prefix_pages.dim() != 1):
         raise ValueError("relay cache attention: prefix_pages must be a list of pages")
-    page_table = _ints("page_table", page_table, tuple(page_table.shape))
+    page_table = _ints("page_table", page_table, page_table.shape)
     lengths = _ints("lengths", lengths, (n,))
     if prefix_len:
         prefix_pages = _list("prefix_pages", prefix_pages)
     if q.stride(-1) != 1:
         q = q.contiguous()
     if scale is None:
-        scale = 1.0 / math.sqrt(c.head_dim)
+        scale = 1.0 / math.sqrt(c[2])
     with _on(dev):
         if out is None:
             out = torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, device=dev, dtype=q.dtype)
@@ -195,15 +222,15 @@ def relay_cache_attention(q, pool, page_table, lengths, *, prefix_pages=None, pr
         row_max = torch.empty_strided(rows, steps, device=dev, dtype=torch.float32)
         row_sum = torch.empty_strided(rows, steps, device=dev, dtype=torch.float32)
         qs = q.stride() if q.dim() == 4 else (q.stride(0), 0, q.stride(1), 1)
-        a = N.RelayCacheAttentionArgs(c, n, tq, heads, page_table.shape[1], 0, prefix_len,
-                                      prefix_pages.shape[0] if prefix_len else 0, _dtype_code(q), scale, _ptr(q), qs,
-                                      _ptr(page_table), _ptr(lengths), _ptr(prefix_pages) if prefix_len else None,
-                                      _ptr(out), _ptr(row_max), _ptr(row_sum))
+        a = _ATTENTION(*c, n, tq, heads, page_table.shape[1], 0, prefix_len, prefix_pages.shape[0] if prefix_len else 0,
+                       _dtype_code(q), scale, q.data_ptr(), *qs, page_table.data_ptr(), lengths.data_ptr(),
+                       prefix_pages.data_ptr() if prefix_len else 0, out.data_ptr(), row_max.data_ptr(),
+                       row_sum.data_ptr())
         if q.numel():
             stream = _stream(dev)
             if workspace is None:
-                workspace = _workspace("attention", N.lib().dbl_relay_cache_attention_workspace_bytes(ctypes.byref(a)), dev, stream)
-            N.check(N.lib().dbl_relay_cache_attention(ctypes.byref(a), _ptr(workspace), workspace.numel(), stream))
+                workspace = _workspace("attention", N.lib().dbl_relay_cache_attention_workspace_bytes(a), dev, stream)
+            N.check(N.lib().dbl_relay_cache_attention(a, workspace.data_ptr(), workspace.numel(), stream))
     return out, row_max, row_sum
 
 
@@ -214,7 +241,7 @@ def _pages(pool, page_table, lengths, refs, out, lists, new_lengths=True):
     if page_table.dim() != 2:
         raise ValueError(f"relay cache: page_table must be [sequences,width], got {list(page_table.shape)}")
     s, w = page_table.shape
-    page_table, refs = _ints("page_table", page_table, (s, w)), _ints("refs", refs, (c.pages,))
+    page_table, refs = _ints("page_table", page_table, (s, w)), _ints("refs", refs, c[:1])
     lengths = _ints("lengths", lengths, (s,))
     new_lengths = new_lengths and lengths is not None
     given = (page_table, lengths, refs) if new_lengths else (page_table, refs)
@@ -227,13 +254,13 @@ def _pages(pool, page_table, lengths, refs, out, lists, new_lengths=True):
         for t, o in zip(given, after):
             if o.shape != t.shape or o.dtype != torch.int32 or not o.is_contiguous():
                 raise ValueError("relay cache: out must be contiguous int32 tensors shaped like the state")
-    a = N.RelayCachePagesArgs(c, s, w, 0, page_table.data_ptr(), _ptr(lengths), refs.data_ptr(), after[0].data_ptr(),
-                              after[1].data_ptr() if new_lengths else None, after[-1].data_ptr())
+    a = _PAGES(*c, s, w, 0, page_table.data_ptr(), _at(lengths), refs.data_ptr(), after[0].data_ptr(),
+               after[1].data_ptr() if new_lengths else 0, after[-1].data_ptr())
     return dev, a, after, (page_table, lengths, refs)
 
 
-def _scratch(a, dev, stream):
-    return _workspace("pages", N.lib().dbl_relay_cache_pages_workspace_bytes(a.cache.pages, a.n_seq), dev, stream)
+def _scratch(pages, sequences, dev, stream):
+    return _workspace("pages", N.lib().dbl_relay_cache_pages_workspace_bytes(pages, sequences), dev, stream)
 
 
 def relay_cache_release(pool, page_table, lengths, refs, sequences, *, out=None):
@@ -241,7 +268,7 @@ def relay_cache_release(pool, page_table, lengths, refs, sequences, *, out=None)
     sequences = _list("sequences", sequences)
     dev, a, after, _keep = _pages(pool, page_table, lengths, refs, out, (sequences,))
     with _on(dev):
-        N.check(N.lib().dbl_relay_cache_release(ctypes.byref(a), _ptr(sequences), sequences.numel(), _stream(dev)))
+        N.check(N.lib().dbl_relay_cache_release(a, sequences.data_ptr(), sequences.numel(), _stream(dev)))
     return after
 
 
@@ -253,7 +280,7 @@ def relay_cache_fork(pool, page_table, lengths, refs, parents, children, *, out=
         raise ValueError("relay cache fork: parents and children must have the same length")
     dev, a, after, _keep = _pages(pool, page_table, lengths, refs, out, (parents, children))
     with _on(dev):
-        N.check(N.lib().dbl_relay_cache_fork(ctypes.byref(a), _ptr(parents), _ptr(children), parents.numel(),
+        N.check(N.lib().dbl_relay_cache_fork(a, parents.data_ptr(), children.data_ptr(), parents.numel(),
                                              _stream(dev)))
     return after
 
@@ -269,8 +296,8 @@ def relay_cache_reserve(pool, page_table, lengths, refs, tokens, *, out=None):
     dev, a, after, _keep = _pages(pool, page_table, lengths, refs, out, () if counts is None else (counts,), False)
     with _on(dev):
         missing, stream = refs.new_empty(1), _stream(dev)
-        ws = _scratch(a, dev, stream)
-        N.check(N.lib().dbl_relay_cache_reserve(ctypes.byref(a), _ptr(counts), tokens, _ptr(missing), _ptr(ws),
+        ws = _scratch(pool.shape[0], page_table.shape[0], dev, stream)
+        N.check(N.lib().dbl_relay_cache_reserve(a, _ptr(counts), tokens, missing.data_ptr(), ws.data_ptr(),
                                                 ws.numel(), stream))
     return after[0], after[1], missing
 
@@ -282,8 +309,8 @@ def relay_cache_compact(pool, page_table, refs, *, out=None):
     dev, a, after, _keep = _pages(pool, page_table, None, refs, out, ())
     with _on(dev):
         used, stream = refs.new_empty(1, dtype=torch.int32), _stream(dev)
-        ws = _scratch(a, dev, stream)
-        N.check(N.lib().dbl_relay_cache_compact(ctypes.byref(a), _ptr(used), _ptr(ws), ws.numel(), stream))
+        ws = _scratch(pool.shape[0], page_table.shape[0], dev, stream)
+        N.check(N.lib().dbl_relay_cache_compact(a, used.data_ptr(), ws.data_ptr(), ws.numel(), stream))
     return after[0], after[1], used
 
 
@@ -293,6 +320,6 @@ def relay_cache_copy_pages(pool, src, dst) -> None:
     dev = _require_cuda(pool, src, dst)
     if src.shape != dst.shape:
         raise ValueError("relay cache copy: src and dst must have the same length")
-    c = _cache(pool)
+    c = N.RelayCache(*_cache(pool))
     with _on(dev):
         N.check(N.lib().dbl_relay_cache_copy_pages(ctypes.byref(c), _ptr(src), _ptr(dst), src.numel(), _stream(dev)))
