@@ -174,10 +174,11 @@ __device__ __forceinline__ float over_g_sum(float x) {
     return x;
 }
 
-// The power of two that takes w to 2^13 .. 2^14, and the inverse of a power of two.
+// The power of two that takes w to 2^7 .. 2^8 (p may grow by kSlack before it is raised again, and f16 holds
+// what is 2^-22 of it to 11 bits), and the inverse of a power of two.
 __device__ __forceinline__ float mult_for(float w) {
     const int e = min(max((int)(__float_as_uint(w) >> 23), 40), 250);
-    return __uint_as_float((uint32_t)(267 - e) << 23);
+    return __uint_as_float((uint32_t)(261 - e) << 23);
 }
 __device__ __forceinline__ float pow2_inverse(float x) { return __uint_as_float((254u << 23) - __float_as_uint(x)); }
 
@@ -731,6 +732,7 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E)) cache_attn_kernel(cons
                         for (int j = 0; j < G; ++j) omin[nr][e][j] *= c[e];
                     }
                     pacc[nr][e] *= c[e];
+                    if (done == 0) continue;  // the sums are zero
 #pragma unroll
                     for (int j = 0; j < G; ++j)
 #pragma unroll
@@ -763,6 +765,7 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E)) cache_attn_kernel(cons
                     const float m = fminf(mult[nr][e], mult_for(over_g_max(wtop[nr][e])));
                     const float c = pow2_inverse(mult[nr][e]) * m;
                     mult[nr][e] = m;
+                    if (done == 0) continue;
 #pragma unroll
                     for (int j = 0; j < G; ++j)
 #pragma unroll
