@@ -32,13 +32,23 @@
 // usually costs one vote instead of the shuffles of a maximum and the rescaling of the sums.
 //
 // Work: an item is (sequence, kv head, up to 8 NR rows), or (kv head, up to 8 NR rows of all
-// sequences) of the prefix, which is thus read once per head for 8 NR rows.  Items are cut into units
-// of 128 tokens, and the units of all items, one after another, are dealt to the CTAs that the GPU
-// holds in equal runs, whatever the lengths are: a CTA finds its run in the lengths, so the host does
-// not need them.  A CTA's four warps take turns at steps of 32 tokens, each with a ring of its own that
-// bulk copies fill.  An item that one CTA holds whole is finished there; the others' sums go to the
-// workspace, and the CTA that arrives last at an item joins them.  The prefix is a launch of its own
-// before the sequences' launch, which starts beside it and joins its sums to every item's.
+// sequences) of a prefix that is worth a launch of its own, which is thus read once per head for 8 NR
+// rows; other prefixes are read with every sequence's own tokens.  Items are cut into units of 128
+// tokens, and the units of all items, one after another, are dealt to the CTAs that the GPU holds in
+// equal runs, whatever the lengths are: a CTA finds its run in the lengths, so the host does not need
+// them.  A CTA's four warps take turns at steps of 32 tokens, each with a ring of its own that bulk
+// copies fill (tcgen05 would need 64 or 128 query rows to a tile, and a kernel with it holds an SM
+// alone).  An item that one CTA holds whole is finished there; the others' sums go to the workspace,
+// and the CTA that arrives last at an item joins them.  The prefix's launch comes before the
+// sequences', which starts beside it and joins its sums to every item's.
+//
+// Bound: the codes' way from memory to operand.  131072 tokens of one sequence, 16 heads of 128 (336
+// MB): 77 us = 4340 GB/s, 66% of the measured copy rate; 343 instructions a warp and tile of 16 tokens,
+// issue slots 60% and ALU 52% busy (LOP3, shifts and byte permutes; a tile needs 64 + 16 + 8 of them).
+// The slope is 83% of the copy rate (131072 to 262144 tokens); the rest is some 20 us of starts, joins
+// and an uneven end.  Tried and slower: 3 and 5 CTAs an SM, steps of 16 and 64 tokens, rings of 1, 3
+// and 4 stages, CTAs of 2 and 8 warps, the next item's copies before this one's sums are joined
+// (registers), shifts as high products.
 #include <float.h>
 
 #include "relay_cache.cuh"
@@ -55,9 +65,8 @@ constexpr int TS = 2;             // tiles of a step
 constexpr int STEP = TS * kCacheTile;
 constexpr int NS = 2;             // stages of a warp's ring
 constexpr int UNIT = W * STEP;    // tokens of a unit
-constexpr int kApartTokens = 512, kApartSequences = 8;  // of a prefix with a launch of its own
+constexpr int64_t kApart = 1 << 19;  // sequences x kv heads x tokens of a prefix with a launch of its own
 constexpr int kStart = 3;         // units that the start and end of an item cost (about 6 us, a unit 2 us)
-constexpr int kLeast = 4;         // units of a CTA's run at least
 constexpr int kCounterBytes = DBL_RELAY_CACHE_COUNTER_BYTES;
 constexpr int WIN = 32 / TS;      // steps whose page numbers the lanes of a warp hold
 constexpr int kCacheWaitFull = 40;  // wait-site code (dbl_device_error)
@@ -394,7 +403,7 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E)) cache_attn_kernel(cons
             total += sint[8 + w];
         }
         total *= HT;
-        run = max((total + (int)gridDim.x - 1) / (int)gridDim.x, kLeast);
+        run = max((total + (int)gridDim.x - 1) / (int)gridDim.x, start + 1);
         pos = blockIdx.x * run;
         end = min(pos + run, total);
         upto *= HT;
@@ -986,11 +995,13 @@ struct Segment {  // the prefix, or the sequences' own tokens
 Segment segment_of(int64_t rows, int64_t items, int64_t tokens, int start, bool bf16) {
     Segment s{};
     s.e = rows <= 4 ? 1 : 2;
+    // two groups of columns share the codes' operands: 16 rows of 48 sequences 64 us, in two tiles of 8 70 us (f32 rows
+    // take the registers twice)
     s.nr = bf16 && rows > 8 ? 2 : 1;
     s.rows = 4 * s.e * s.nr;
     s.tiles = (int)ceil_div(rows, s.rows);
     s.units = items * s.tiles * (start + (tokens > UNIT ? ceil_div(tokens, UNIT) : 1));
-    const int64_t held = 148 * held_at(s.nr, s.e), runs = ceil_div(s.units, kLeast);
+    const int64_t held = 148 * held_at(s.nr, s.e), runs = ceil_div(s.units, start + 1);
     s.grid = runs < held ? runs : held;
     return s;
 }
@@ -1006,8 +1017,11 @@ Plan plan_of(const dbl_relay_cache_attention_args* a) {
     const int64_t TG = a->queries * (a->heads / a->cache.kv_heads), H = a->cache.kv_heads, N = a->n_seq;
     const bool bf16 = a->dtype == DBL_BF16;
     const size_t row = (size_t)(a->cache.head_dim + kPartPad) * 4;
-    // A prefix is worth a launch of its own where many sequences share it and it is long.
-    const bool apart = a->prefix_len >= kApartTokens && N >= kApartSequences;
+    // A prefix has a launch of its own (about 12 us) where reading it with every sequence's own tokens costs more.
+    // Measured at 16 heads of 128, 1024 own tokens, apart and with them: 64 sequences, prefix 512: 67 and 66 us, 1024:
+    // 68 and 80, 4096: 82 and 172; 16 sequences, 512: 30 and 26, 1024: 31 and 30, 4096: 34 and 52; 4 sequences, 4096:
+    // 23 and 22.
+    const bool apart = N >= 4 && N * H * a->prefix_len >= kApart;
     L.lead = a->prefix_len > 0 && !apart ? (int)(ceil_div(a->prefix_len, kCacheTile) * kCacheTile) : 0;
     L.own = segment_of(TG, N * H, L.lead + a->table_width * a->cache.page_size, kStart, bf16);
     L.off_part = kCounterBytes;
@@ -1017,7 +1031,6 @@ Plan plan_of(const dbl_relay_cache_attention_args* a) {
         L.pre = segment_of(N * TG, H, a->prefix_len, 0, bf16);
         L.pre_units = (int)ceil_div(a->prefix_len, UNIT);
         L.pre_run = (int)ceil_div(L.pre.units, L.pre.grid);
-        if (L.pre_run < kLeast) L.pre_run = kLeast;
         L.pre.grid = ceil_div(L.pre.units, L.pre_run);
         L.pre_parts = (L.pre_units + L.pre_run - 2) / L.pre_run + 1;
         L.bytes += (size_t)(H * L.pre.tiles * L.pre.rows * L.pre_parts) * row;

@@ -363,6 +363,34 @@ def test_attention_many_sequences_share_a_prefix(cuda, native_lib, dtype):
 
 @gpu
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("n,hkv,group,tq,d,page,prefix", [(64, 2, 1, 1, 128, 64, 4200), (40, 4, 2, 3, 64, 48, 3300),
+                                                          (5, 1, 1, 1, 64, 16, 104900), (33, 2, 9, 1, 128, 32, 8001)])
+def test_attention_long_shared_prefix(cuda, native_lib, dtype, n, hkv, group, tq, d, page, prefix):
+    """Prefixes with a launch of their own: sequences x kv heads x tokens of at least 2^19."""
+    rng = np.random.default_rng(n)
+    assert n * hkv * prefix >= 1 << 19
+    lens = [int(x) for x in rng.integers(0, 200, n)]
+    lens[0], lens[-1] = 0, tq
+    pool, tab, held, kk, vv = _fill(cuda, rng, [prefix] + lens, hkv, d, page)
+    q = torch.as_tensor(rng.standard_normal((n, tq, hkv * group, d))).to(cuda, dtype)
+    want = M.attention(q.double().cpu().numpy(), kk[1:], vv[1:], lens, kk[0], vv[0])
+    call = lambda: dbl.relay_cache_attention(q, pool, tab[1:], held[1:], prefix_pages=tab[0], prefix_len=prefix)  # noqa: E731
+    got = call()
+    _check_attention(got, want, dtype, d, prefix + 200)
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(got, call()))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        again = call()
+    for _ in range(2):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, again))
+    _ok()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
 def test_attention_scales_of_all_sizes(cuda, native_lib, dtype):
     """Queries and values far from 1 in size, rows of q that differ by many powers of two, tokens whose value
     scales differ, one all-zero query, constant value groups."""
