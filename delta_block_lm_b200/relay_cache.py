@@ -68,13 +68,40 @@ class _Here:
 
 _here = _Here()
 
+# A decode step makes several of these calls, and the host path is most of a small one's time: the short ways
+# to the current device and stream, and the library's functions looked up once.
 
-def _on(dev: torch.device):
-    return _here if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+def _device(first: torch.Tensor, *others: Optional[torch.Tensor]) -> int:
+    """The index of the CUDA device that the tensors share."""
+    d = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != d:
+            d = -1
+    if d < 0:
+        _require_cuda(first, *others)  # says what is wrong
+    return d
 
 
-def _stream(dev: torch.device) -> int:  # a decode step makes several of these calls: the short way
-    return torch._C._cuda_getCurrentRawStream(dev.index)
+def _on(d: int):
+    return _here if d == torch._C._cuda_getDevice() else torch.cuda.device(d)
+
+
+_stream = torch._C._cuda_getCurrentRawStream
+_functions: dict = {}
+
+
+def _library(name: str):
+    f = _functions.get(name)
+    if f is None:
+        f = _functions[name] = getattr(N.lib(), "dbl_relay_cache_" + name)
+    return f
+
+
+def _call(name: str, *args) -> None:
+    status = _library(name)(*args)
+    if status:
+        N.check(status)
 
 
 def relay_cache_pool(pages: int, kv_heads: int, head_dim: int, page_size: int = 64, *, device="cuda") -> torch.Tensor:
@@ -120,7 +147,7 @@ def relay_cache_append(pool, page_table, lengths, k, v, *, counts=None, out=None
     """Writes the tokens k, v [N, T, kv_heads, D] (f32 or bf16; any strides with unit innermost) after
     the ``lengths`` [N] tokens that each sequence holds, and returns the new lengths.  ``counts`` [N]:
     how many of the T tokens are real (ragged prompts).  The pages must have been reserved."""
-    dev = _require_cuda(pool, page_table, lengths, k, v, counts, out)
+    dev = _device(pool, page_table, lengths, k, v, counts, out)
     c = _cache(pool)
     shape = k.shape
     if len(shape) != 4 or shape[2:] != c[1:3] or shape != v.shape:
@@ -143,14 +170,14 @@ def relay_cache_append(pool, page_table, lengths, k, v, *, counts=None, out=None
         new = torch.empty_like(lengths)
         a = _APPEND(*c, n, t, page_table.shape[1], 0, _dtype_code(k), k.data_ptr(), v.data_ptr(), *k.stride(), *v.stride(),
                     page_table.data_ptr(), lengths.data_ptr(), _at(counts), new.data_ptr())
-        N.check(N.lib().dbl_relay_cache_append(a, _stream(dev)))
+        _call("append", a, _stream(dev))
         return new if out is None else out.copy_(new)
 
 
 def relay_cache_read(pool, page_table, lengths, *, start=None, tokens: int, dtype=torch.bfloat16):
     """Tokens start[n] .. start[n] + tokens - 1 of every sequence as the values that the cache holds:
     (k, v) [N, tokens, kv_heads, D] in ``dtype`` (f32 or bf16); zeros at and past ``lengths``."""
-    dev = _require_cuda(pool, page_table, lengths, start)
+    dev = _device(pool, page_table, lengths, start)
     c = _cache(pool)
     if page_table.dim() != 2:
         raise ValueError(f"relay cache read: page_table must be [N,width], got {list(page_table.shape)}")
@@ -158,29 +185,29 @@ def relay_cache_read(pool, page_table, lengths, *, start=None, tokens: int, dtyp
     page_table = _ints("page_table", page_table, page_table.shape)
     lengths, start = _ints("lengths", lengths, (n,)), _ints("start", start, (n,))
     with _on(dev):
-        k = torch.empty((n, tokens, c[1], c[2]), device=dev, dtype=dtype)
+        k = pool.new_empty((n, tokens, c[1], c[2]), dtype=dtype)
         v = torch.empty_like(k)
         a = _READ(*c, n, tokens, page_table.shape[1], 0, _dtype_code(k), page_table.data_ptr(), lengths.data_ptr(),
                   _at(start), k.data_ptr(), v.data_ptr())
         if k.numel():
-            N.check(N.lib().dbl_relay_cache_read(a, _stream(dev)))
+            _call("read", a, _stream(dev))
     return k, v
 
 
 _workspaces: dict = {}  # (what for, device, stream): a workspace kept from call to call
 
 
-def _workspace(what: str, need: int, dev: torch.device, stream: int) -> torch.Tensor:
+def _workspace(what: str, need: int, dev: int, stream: int) -> torch.Tensor:
     """A workspace whose counters (the attention's) are zero.  Calls on one stream follow one another, so
     each stream keeps one; a graph that is being captured gets its own (it may be replayed beside other
     calls)."""
-    capturing = torch.cuda.is_current_stream_capturing()
-    ws = None if capturing else _workspaces.get((what, dev.index, stream))
+    capturing = torch._C._cuda_isCurrentStreamCapturing()
+    ws = None if capturing else _workspaces.get((what, dev, stream))
     if ws is None or ws.numel() < need:
-        ws = torch.empty(need, device=dev, dtype=torch.uint8)
+        ws = torch.empty(need, device=torch.device("cuda", dev), dtype=torch.uint8)
         ws[:N.RELAY_CACHE_COUNTER_BYTES].zero_()
         if not capturing:
-            _workspaces[what, dev.index, stream] = ws
+            _workspaces[what, dev, stream] = ws
     return ws
 
 
@@ -192,51 +219,63 @@ def relay_cache_attention(q, pool, page_table, lengths, *, prefix_pages=None, pr
     themselves; f32 or bf16, heads a multiple of the pool's kv heads.  ``lengths`` counts the queries'
     own tokens (append first).  ``prefix_pages`` [width] names the pages of ``prefix_len`` tokens that
     every sequence sees before its own.  ``workspace``: a uint8 tensor whose first
-    ``RELAY_CACHE_COUNTER_BYTES`` bytes are zero before its first use (by default each stream keeps one).  Returns (o, row_max, row_sum) as ``relay_merge_decode``; a row
-    without keys gives o = 0 and (0, 1)."""
-    dev = _require_cuda(q, pool, page_table, lengths, prefix_pages, out, workspace)
+    ``RELAY_CACHE_COUNTER_BYTES`` bytes are zero before its first use (by default each stream keeps one, until the
+    process ends).  Returns (o, row_max, row_sum) as ``relay_merge_decode``; a row without keys gives o = 0
+    and (0, 1)."""
+    dev = _device(q, pool, page_table, lengths, prefix_pages, out, workspace)
     c = _cache(pool)
-    if q.dim() not in (3, 4) or q.shape[-1] != c[2]:
-        raise ValueError(f"relay cache attention: q must be [N,heads,{c[2]}] or [N,Tq,heads,{c[2]}], got "
-                         f"{list(q.shape)}")
-    n, heads = q.shape[0], q.shape[-2]
-    tq = q.shape[1] if q.dim() == 4 else 1
-    if page_table.dim() != 2 or page_table.shape[0] != n:
-        raise ValueError(f"relay cache attention: page_table must be [{n},width], got {list(page_table.shape)}")
-    if prefix_len and (prefix_pages is None or prefix_pages.dim() != 1):
-        raise ValueError("relay cache attention: prefix_pages must be a list of pages")
-    page_table = _ints("page_table", page_table, page_table.shape)
+    shape = q.shape
+    if len(shape) == 3:
+        n, heads, d = shape
+        tq, rows, steps = 1, (n, heads), (heads, 1)
+    elif len(shape) == 4:
+        n, tq, heads, d = shape
+        rows, steps = (n, tq, heads), (tq * heads, heads, 1)
+    else:
+        d = 0
+    if d != c[2]:
+        raise ValueError(f"relay cache attention: q must be [N,heads,{c[2]}] or [N,Tq,heads,{c[2]}], got {list(shape)}")
+    table_shape = page_table.shape
+    if len(table_shape) != 2 or table_shape[0] != n:
+        raise ValueError(f"relay cache attention: page_table must be [{n},width], got {list(table_shape)}")
+    page_table = _ints("page_table", page_table, table_shape)
     lengths = _ints("lengths", lengths, (n,))
+    prefix_at = prefix_width = 0
     if prefix_len:
+        if prefix_pages is None or prefix_pages.dim() != 1:
+            raise ValueError("relay cache attention: prefix_pages must be a list of pages")
         prefix_pages = _list("prefix_pages", prefix_pages)
-    if q.stride(-1) != 1:
+        prefix_at, prefix_width = prefix_pages.data_ptr(), prefix_pages.shape[0]
+    strides = q.stride()
+    if strides[-1] != 1:
         q = q.contiguous()
+        strides = q.stride()
+    if len(shape) == 3:
+        strides = (strides[0], 0, strides[1], 1)
     if scale is None:
-        scale = 1.0 / math.sqrt(c[2])
+        scale = 1.0 / math.sqrt(d)
     with _on(dev):
         if out is None:
-            out = torch.empty_like(q) if q.is_contiguous() else torch.empty(q.shape, device=dev, dtype=q.dtype)
-        elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+            out = torch.empty_like(q) if q.is_contiguous() else q.new_empty(shape)
+        elif out.shape != shape or out.dtype != q.dtype or not out.is_contiguous():
             raise ValueError("relay cache attention: out must be contiguous with the shape and dtype of q")
-        rows, steps = q.shape[:-1], (heads, 1) if q.dim() == 3 else (tq * heads, heads, 1)
-        row_max = torch.empty_strided(rows, steps, device=dev, dtype=torch.float32)
-        row_sum = torch.empty_strided(rows, steps, device=dev, dtype=torch.float32)
-        qs = q.stride() if q.dim() == 4 else (q.stride(0), 0, q.stride(1), 1)
-        a = _ATTENTION(*c, n, tq, heads, page_table.shape[1], 0, prefix_len, prefix_pages.shape[0] if prefix_len else 0,
-                       _dtype_code(q), scale, q.data_ptr(), *qs, page_table.data_ptr(), lengths.data_ptr(),
-                       prefix_pages.data_ptr() if prefix_len else 0, out.data_ptr(), row_max.data_ptr(),
+        device = q.device
+        row_max = torch.empty_strided(rows, steps, device=device, dtype=torch.float32)
+        row_sum = torch.empty_strided(rows, steps, device=device, dtype=torch.float32)
+        a = _ATTENTION(*c, n, tq, heads, table_shape[1], 0, prefix_len, prefix_width, _dtype_code(q), scale, q.data_ptr(),
+                       *strides, page_table.data_ptr(), lengths.data_ptr(), prefix_at, out.data_ptr(), row_max.data_ptr(),
                        row_sum.data_ptr())
         if q.numel():
             stream = _stream(dev)
             if workspace is None:
-                workspace = _workspace("attention", N.lib().dbl_relay_cache_attention_workspace_bytes(a), dev, stream)
-            N.check(N.lib().dbl_relay_cache_attention(a, workspace.data_ptr(), workspace.numel(), stream))
+                workspace = _workspace("attention", _library("attention_workspace_bytes")(a), dev, stream)
+            _call("attention", a, workspace.data_ptr(), workspace.numel(), stream)
     return out, row_max, row_sum
 
 
 def _pages(pool, page_table, lengths, refs, out, lists, new_lengths=True):
     """(device, arguments, outputs, tensors to keep) of a page operation; lengths None: it has none."""
-    dev = _require_cuda(pool, page_table, lengths, refs, *lists, *(out or ()))
+    dev = _device(pool, page_table, lengths, refs, *lists, *(out or ()))
     c = _cache(pool)
     if page_table.dim() != 2:
         raise ValueError(f"relay cache: page_table must be [sequences,width], got {list(page_table.shape)}")
@@ -260,7 +299,7 @@ def _pages(pool, page_table, lengths, refs, out, lists, new_lengths=True):
 
 
 def _scratch(pages, sequences, dev, stream):
-    return _workspace("pages", N.lib().dbl_relay_cache_pages_workspace_bytes(pages, sequences), dev, stream)
+    return _workspace("pages", _library("pages_workspace_bytes")(pages, sequences), dev, stream)
 
 
 def relay_cache_release(pool, page_table, lengths, refs, sequences, *, out=None):
@@ -268,7 +307,7 @@ def relay_cache_release(pool, page_table, lengths, refs, sequences, *, out=None)
     sequences = _list("sequences", sequences)
     dev, a, after, _keep = _pages(pool, page_table, lengths, refs, out, (sequences,))
     with _on(dev):
-        N.check(N.lib().dbl_relay_cache_release(a, sequences.data_ptr(), sequences.numel(), _stream(dev)))
+        _call("release", a, sequences.data_ptr(), sequences.numel(), _stream(dev))
     return after
 
 
@@ -280,8 +319,7 @@ def relay_cache_fork(pool, page_table, lengths, refs, parents, children, *, out=
         raise ValueError("relay cache fork: parents and children must have the same length")
     dev, a, after, _keep = _pages(pool, page_table, lengths, refs, out, (parents, children))
     with _on(dev):
-        N.check(N.lib().dbl_relay_cache_fork(a, parents.data_ptr(), children.data_ptr(), parents.numel(),
-                                             _stream(dev)))
+        _call("fork", a, parents.data_ptr(), children.data_ptr(), parents.numel(), _stream(dev))
     return after
 
 
@@ -295,10 +333,9 @@ def relay_cache_reserve(pool, page_table, lengths, refs, tokens, *, out=None):
         counts, tokens = _ints("tokens", tokens, tuple(lengths.shape)), 0
     dev, a, after, _keep = _pages(pool, page_table, lengths, refs, out, () if counts is None else (counts,), False)
     with _on(dev):
-        missing, stream = refs.new_empty(1), _stream(dev)
+        missing, stream = refs.new_empty(1, dtype=torch.int32), _stream(dev)
         ws = _scratch(pool.shape[0], page_table.shape[0], dev, stream)
-        N.check(N.lib().dbl_relay_cache_reserve(a, _ptr(counts), tokens, missing.data_ptr(), ws.data_ptr(),
-                                                ws.numel(), stream))
+        _call("reserve", a, _ptr(counts), tokens, missing.data_ptr(), ws.data_ptr(), ws.numel(), stream)
     return after[0], after[1], missing
 
 
@@ -310,16 +347,16 @@ def relay_cache_compact(pool, page_table, refs, *, out=None):
     with _on(dev):
         used, stream = refs.new_empty(1, dtype=torch.int32), _stream(dev)
         ws = _scratch(pool.shape[0], page_table.shape[0], dev, stream)
-        N.check(N.lib().dbl_relay_cache_compact(a, used.data_ptr(), ws.data_ptr(), ws.numel(), stream))
+        _call("compact", a, used.data_ptr(), ws.data_ptr(), ws.numel(), stream)
     return after[0], after[1], used
 
 
 def relay_cache_copy_pages(pool, src, dst) -> None:
     """Copies page src[i] to page dst[i] (no page is both, none is written twice)."""
     src, dst = _list("src", src), _list("dst", dst)
-    dev = _require_cuda(pool, src, dst)
+    dev = _device(pool, src, dst)
     if src.shape != dst.shape:
         raise ValueError("relay cache copy: src and dst must have the same length")
     c = N.RelayCache(*_cache(pool))
     with _on(dev):
-        N.check(N.lib().dbl_relay_cache_copy_pages(ctypes.byref(c), _ptr(src), _ptr(dst), src.numel(), _stream(dev)))
+        _call("copy_pages", ctypes.byref(c), _ptr(src), _ptr(dst), src.numel(), _stream(dev))
