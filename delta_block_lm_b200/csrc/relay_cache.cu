@@ -178,7 +178,7 @@ __global__ void __launch_bounds__(256) cache_append_tiles_kernel(const AppendPar
     const bool live = t >= 0 && t < count;
     const bool whole = t0 >= 0 && t0 + kCacheTile <= count;
     const T* src = static_cast<const T*>(which ? p.v : p.k) + n * (which ? p.vs[0] : p.ks[0]) +
-                   (live ? t : max(0, -t0)) * (which ? p.vs[1] : p.ks[1]) + part * 16;
+                   (live ? t : 0) * (which ? p.vs[1] : p.ks[1]) + part * 16;
     const int64_t hs = which ? p.vs[2] : p.ks[2];
     uint4 raw[NW];
     auto load = [&](int h) {

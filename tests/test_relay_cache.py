@@ -270,6 +270,36 @@ def test_append_strided_views_and_alignment(cuda, native_lib, dtype):
 
 
 @gpu
+@pytest.mark.parametrize("dtype,d", [(BF16, 128), (F32, 64)])
+def test_append_few_tokens_inside_a_tile(cuda, native_lib, dtype, d):
+    """Calls of 1 to 40 tokens that begin inside a tile, with k and v at the very end of their memory: no lane may
+    read past the call's own tokens, and what is written is what one token at a time writes."""
+    rng = np.random.default_rng(6)
+    h, page = 5, 16
+    for t in (1, 2, 7, 8, 9, 15, 16, 17, 31, 32, 33, 40):
+        start = [0, 5, 15]
+        table, pages, _ = _tables(rng, [s + t for s in start], page)
+        tab = _i32(table, cuda)
+        store = torch.empty((2, 3, t, h, d), device=cuda, dtype=dtype)  # v ends where the memory does
+        store.copy_(torch.as_tensor(rng.standard_normal(store.shape)))
+        pools = [dbl.relay_cache_pool(pages, h, d, page, device=cuda) for _ in "ab"]
+        new = dbl.relay_cache_append(pools[0], tab, _i32(start, cuda), store[0], store[1])
+        assert new.tolist() == [s + t for s in start]
+        for i in range(t):
+            dbl.relay_cache_append(pools[1], tab, _i32([s + i for s in start], cuda), store[0, :, i:i + 1], store[1, :, i:i + 1])
+        assert torch.equal(*pools), t
+    _ok()
+
+
+def test_lanes_without_a_token_read_the_first_one():
+    """The source's own rule for which token a lane without one loads (it must load some: the shuffles need whole
+    groups).  It once was the place of the tile's first token, which can lie past a short call's tokens."""
+    src = open(os.path.join(ROOT, "delta_block_lm_b200", "csrc", "relay_cache.cu")).read()
+    body = src[src.index("cache_append_tiles_kernel(const AppendParams p)"):]
+    assert "(live ? t : 0) * (which ? p.vs[1] : p.ks[1])" in body
+
+
+@gpu
 def test_append_special_values(cuda, native_lib):
     """Constants, a range below 2^-100, the largest values, and groups that hold an infinity or NaN: those
     become NaN, the other groups of the token are untouched."""
