@@ -150,9 +150,14 @@ __global__ void __launch_bounds__(256) cache_append_kernel(const AppendParams p)
 // Prompts.  A CTA writes one tile of positions for p.per heads, one after another: the tile is put together in shared
 // memory and leaves in 16-byte words (in the pieces of single tokens where it is not written whole).  One
 // thread: 16 channels of one token's key or value, two neighbouring lanes a group; its next head's
-// values are on their way while it encodes.
+// values are on their way while it encodes.  8 x 4096 tokens, 16 heads of 128, bf16 (268 MB in, 84 MB out): 88 us
+// = 4000 GB/s, 61% of the measured copy rate; bound by instructions (19 an element, issue slots 81% busy).  A
+// correction on the FMA pipe alone (saturating products instead of compares) took the same time.
 constexpr int kTileHeads = 4, kManyHeads = 16;
-constexpr int kTileTokens = 8;  // calls of at least so many tokens a sequence go by tiles
+// Calls of at least so many tokens a sequence go by tiles.  256 sequences at all places in a tile, 16 heads of 128,
+// by tiles and by single tokens: 8 tokens, append 26 and 12 us, read 13 and 10 us; 16 tokens 31 and 21, 16 and 17
+// us; 64 tokens 66 and 78, 41 and 57 us.
+constexpr int kTileTokens = 32;
 
 template <int D, typename T>
 __global__ void __launch_bounds__(256) cache_append_tiles_kernel(const AppendParams p) {
@@ -294,7 +299,8 @@ __global__ void __launch_bounds__(256) cache_read_kernel(const ReadParams p) {
 }
 
 // Runs of tokens: a CTA reads one tile of positions for kTileHeads heads, all of them at once in 16-byte
-// words to shared memory.  One thread: 16 channels of one token's key or value.
+// words to shared memory.  One thread: 16 channels of one token's key or value.  The prompts above (84 MB in,
+// 268 MB out): 66.5 us = 5300 GB/s, 81% of the measured copy rate; one tile at a time took 79 us.
 template <int D, typename T>
 __global__ void __launch_bounds__(256) cache_read_tiles_kernel(const ReadParams p) {
     using At = TileAt<D>;

@@ -291,14 +291,6 @@ def test_append_few_tokens_inside_a_tile(cuda, native_lib, dtype, d):
     _ok()
 
 
-def test_lanes_without_a_token_read_the_first_one():
-    """The source's own rule for which token a lane without one loads (it must load some: the shuffles need whole
-    groups).  It once was the place of the tile's first token, which can lie past a short call's tokens."""
-    src = open(os.path.join(ROOT, "delta_block_lm_b200", "csrc", "relay_cache.cu")).read()
-    body = src[src.index("cache_append_tiles_kernel(const AppendParams p)"):]
-    assert "(live ? t : 0) * (which ? p.vs[1] : p.ks[1])" in body
-
-
 @gpu
 def test_append_special_values(cuda, native_lib):
     """Constants, a range below 2^-100, the largest values, and groups that hold an infinity or NaN: those
@@ -742,4 +734,40 @@ def test_a_serving_loop(cuda, native_lib):
             assert used.tolist() == [int((refs > 0).sum())] and not refs[used.item():].any()
             attend()
     assert refs.sum() == (table >= 0).sum()
+    _ok()
+
+
+@gpu
+def test_the_example(cuda, native_lib, capsys):
+    """The serving example, small: its last step against relay_merge_decode on the cache's values, which it reads back
+    rounded to bf16 (2^-9 of a value; rounding of both outputs to bf16, 2^-9 each, norm-wise below 1e-2)."""
+    import importlib.util
+    spec = importlib.util.spec_from_file_location("serving", os.path.join(ROOT, "examples", "relay_cache_serving.py"))
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    assert m.main(["--sequences", "5", "--prefix", "77", "--prompt", "30", "--steps", "40"]) < 1e-2
+    assert "pages in use" in capsys.readouterr().out
+    _ok()
+
+
+@gpu
+def test_states_and_lists_of_other_types(cuda, native_lib):
+    """int64 tables, lengths and lists, and strided ones, are converted; the arguments stay as they were."""
+    pool = dbl.relay_cache_pool(8, 1, 64, 16, device=cuda)
+    big = torch.full((4, 6), -1, device=cuda, dtype=torch.int64)
+    table, lengths, refs = big[::2, ::2], torch.tensor([0, 0], device=cuda), torch.zeros(8, device=cuda, dtype=torch.int64)
+    table, refs2, missing = dbl.relay_cache_reserve(pool, table, lengths, refs, torch.tensor([20, 3], device=cuda))
+    assert missing.dtype == torch.int32 and missing.tolist() == [0]
+    assert table.tolist() == [[0, 1, -1], [2, -1, -1]] and refs2.tolist() == [1, 1, 1, 0, 0, 0, 0, 0]
+    assert (big == -1).all() and not refs.any()
+    kv = torch.randn(2, 20, 1, 64, device=cuda)
+    lengths = dbl.relay_cache_append(pool, table.long(), lengths, kv, kv, counts=torch.tensor([20, 3], device=cuda))
+    assert lengths.tolist() == [20, 3]
+    o, _, _ = dbl.relay_cache_attention(kv[:, 0], pool, table.long(), lengths.long())
+    assert torch.equal(o, dbl.relay_cache_attention(kv[:, 0], pool, table, lengths)[0])
+    table, refs2, used = dbl.relay_cache_compact(pool, table.long(), refs2.long())
+    assert used.tolist() == [3] and table.tolist() == [[0, 1, -1], [2, -1, -1]]
+    table, lengths, refs2 = dbl.relay_cache_release(pool, table, lengths, refs2, torch.tensor([1], device=cuda))
+    assert lengths.tolist() == [20, 0] and refs2.tolist() == [1, 1, 0, 0, 0, 0, 0, 0]
+    dbl.relay_cache_release(pool, table, lengths, refs2, torch.zeros(0, device=cuda, dtype=torch.int32))  # an empty list
     _ok()
