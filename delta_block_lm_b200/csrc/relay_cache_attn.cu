@@ -599,7 +599,6 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E)) cache_attn_kernel(cons
     float l[NR][E], top[NR][E];      // sums; largest inner score of the lane
     float ref[NR][E], bar_[NR][E];   // p = 2^(f inner - ref); the inner score at which ref is raised
     float wtop[NR][E], mult[NR][E];  // largest p scale of the lane; r = p scale mult, a power of two
-    int lim[NR][E];
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr) {
 #pragma unroll
@@ -613,7 +612,6 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E)) cache_attn_kernel(cons
             l[nr][e] = wtop[nr][e] = ref[nr][e] = 0.f;
             mult[nr][e] = kMostMult;
             top[nr][e] = bar_[nr][e] = -INFINITY;
-            lim[nr][e] = limit_of(row_at(nr, e));
 #pragma unroll
             for (int j = 0; j < G; ++j) omin[nr][e][j] = 0.f;
         }
@@ -688,14 +686,18 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E)) cache_attn_kernel(cons
         // tokens that a row does not see, or that are not there
         if (masked) {
 #pragma unroll
-            for (int i = 0; i < TS; ++i)
+            for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-                for (int nr = 0; nr < NR; ++nr)
+                for (int e = 0; e < E; ++e) {
+                    const int lim = min(limit_of(row_at(nr, e)), c1);
 #pragma unroll
-                    for (int e = 0; e < 2 * E; ++e) {
-                        const int tok = tok0 + i * kCacheTile + g + 8 * (e / E);
-                        if (!(have >> i & 1) || tok >= min(lim[nr][e % E], c1) || (tok >= lead_end && tok < lead)) s[i][nr][e] = -INFINITY;
-                    }
+                    for (int i = 0; i < TS; ++i)
+#pragma unroll
+                        for (int b = 0; b < 2; ++b) {
+                            const int tok = tok0 + i * kCacheTile + g + 8 * b;
+                            if (!(have >> i & 1) || tok >= lim || (tok >= lead_end && tok < lead)) s[i][nr][b * E + e] = -INFINITY;
+                        }
+                }
         }
         // a bound of each token's value scales: their sum
         float sa_top[TS], sb_top[TS];
@@ -931,17 +933,17 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E)) cache_attn_kernel(cons
     }
     bool finish = !pre && whole;
     if (!pre && !whole) {  // the CTA that arrives last at the item joins its parts, and leaves the counter at zero
-        __threadfence();
         __syncthreads();
-        if (threadIdx.x == 0) {
+        if (threadIdx.x == 0) {  // the barriers make its fences the whole CTA's
+            __threadfence();
             const bool last = atomicAdd(p.counter + cta_first, 1u) == (unsigned)(cta_last - cta_first);
             if (last) p.counter[cta_first] = 0;
             sint[1] = last;
+            __threadfence();
         }
         __syncthreads();
         finish = sint[1];
         if (finish) {
-            __threadfence();
             for (int i = lane; i < rows * D; i += 32) sacc[i] = 0.f;
             if (lane < rows) sml[warp * R + lane] = make_float2(-INFINITY, 0.f);
             __syncwarp();
