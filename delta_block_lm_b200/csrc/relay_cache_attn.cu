@@ -12,12 +12,12 @@
 //     o_c   = sum_k (p_k scale_kj) code_kc + sum_k p_k min_kj
 // and the products with the codes run on mma.sync m16n8k16 with f16 operands and f32 sums, tokens
 // (K) or channels (V) in the 16 rows and up to 8 query rows in the 8 columns:
-//   * a code needs no conversion: the 16-bit word with the code in its lowest 4 bits is the f16
-//     subnormal code * 2^-24, with the code in the next 4 bits 16 times that, so one AND makes the
-//     operand register of two codes.  The powers of two go into q (keys) or the output (values).
-//     The products' sums drop what lies 24 bits below the largest operand exponent, and a
-//     subnormal's counts as 2^-14, which leaves about 17 bits: for f32 rows the keys' codes are
-//     shifted to the top of the mantissa (code * 2^-18, 22 bits).  The values' codes become normal
+//   * a code needs no conversion: the 16-bit word with the code in four of its lowest 10 bits is an f16
+//     subnormal, code * 2^-20 in bits 4 .. 7, so a shift and an AND make the operand register of two
+//     keys' codes.  The powers of two go into q.  The products' sums drop what lies 24 bits below the
+//     largest operand exponent, and a subnormal's counts as 2^-14, which leaves 18 to 22 bits (in the
+//     lowest four bits it would be 14 to 18: an error of 1e-6 in the sums of small calls); for f32 rows the
+//     codes go to the top of the mantissa (code * 2^-18, 20 to 24 bits).  The values' codes become normal
 //     numbers around zero (code - 8), so that long sums neither drop bits nor cancel:
 //     o = sum r (code - 8) + sum p (min + 8 scale), r the rounded p scale.
 //   * q is held in f16 relative to a power of two of its own row (bf16 q: exact; f32 q: two f16
@@ -192,8 +192,8 @@ __device__ __forceinline__ float mult_for(float w) {
 __device__ __forceinline__ float pow2_inverse(float x) { return __uint_as_float((254u << 23) - __float_as_uint(x)); }
 
 // The operand registers of the 8 codes of w, codes (0, 4), (1, 5), (2, 6), (3, 7), and what they are
-// multiplied by to be the codes (kUnit of register i).
-enum class Codes { kLow, kHigh, kCentred };
+// multiplied by to be the codes (code_unit).
+enum class Codes { kMid, kHigh, kCentred };
 // (x & mask) | bits in one instruction, which takes one constant: the other one stays in a register.
 __device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {
     uint32_t r;
@@ -205,23 +205,21 @@ __device__ __forceinline__ void code_operands(uint32_t w, uint32_t (&r)[4]) {
     if constexpr (C == Codes::kHigh) {
         r[0] = (w << 6) & 0x03C003C0u, r[1] = (w << 2) & 0x03C003C0u;
         r[2] = (w >> 2) & 0x03C003C0u, r[3] = (w >> 6) & 0x03C003C0u;
-    } else {
+    } else if constexpr (C == Codes::kMid) {
+        r[0] = (w << 4) & 0x00F000F0u, r[1] = w & 0x00F000F0u;
+        r[2] = (w >> 4) & 0x00F000F0u, r[3] = (w >> 8) & 0x00F000F0u;
+    } else {  // 1024 + x is the f16 with mantissa x; 1032 = 1024 + 8, 1152 = 1024 + 16 * 8
         const uint32_t v = w >> 8;
-        if constexpr (C == Codes::kLow) {
-            r[0] = w & 0x000F000Fu, r[1] = w & 0x00F000F0u;
-            r[2] = v & 0x000F000Fu, r[3] = v & 0x00F000F0u;
-        } else {  // 1024 + x is the f16 with mantissa x; 1032 = 1024 + 8, 1152 = 1024 + 16 * 8
-            r[0] = and_or(w, 0x000F000Fu, 0x64006400u), r[1] = and_or(w, 0x00F000F0u, 0x64006400u);
-            r[2] = and_or(v, 0x000F000Fu, 0x64006400u), r[3] = and_or(v, 0x00F000F0u, 0x64006400u);
+        r[0] = and_or(w, 0x000F000Fu, 0x64006400u), r[1] = and_or(w, 0x00F000F0u, 0x64006400u);
+        r[2] = and_or(v, 0x000F000Fu, 0x64006400u), r[3] = and_or(v, 0x00F000F0u, 0x64006400u);
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                asm("add.rn.f16x2 %0, %0, %1;" : "+r"(r[i]) : "r"(i & 1 ? 0xE480E480u : 0xE408E408u));
-        }
+        for (int i = 0; i < 4; ++i)
+            asm("add.rn.f16x2 %0, %0, %1;" : "+r"(r[i]) : "r"(i & 1 ? 0xE480E480u : 0xE408E408u));
     }
 }
 template <Codes C>
 constexpr float code_unit(int i) {
-    return C == Codes::kHigh ? 262144.f : (i & 1 ? 0.0625f : 1.f) * (C == Codes::kLow ? 16777216.f : 1.f);
+    return C == Codes::kHigh ? 262144.f : C == Codes::kMid ? 1048576.f : i & 1 ? 0.0625f : 1.f;
 }
 
 // The operand whose rows are the 2 G scales and minima of a tile's tokens (scale 0, minimum 0, scale 1,
@@ -351,7 +349,7 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E)) cache_attn_kernel(cons
     constexpr bool SPLIT = sizeof(T) == 4;
     constexpr int NP = SPLIT ? 2 : 1;  // f16 parts of q and of p
     constexpr int PER = 16 / sizeof(T);
-    constexpr Codes KX = SPLIT ? Codes::kHigh : Codes::kLow, VX = Codes::kCentred;
+    constexpr Codes KX = SPLIT ? Codes::kHigh : Codes::kMid, VX = Codes::kCentred;
     extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     uint64_t* bar = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR) + warp * NS;
@@ -564,7 +562,7 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E)) cache_attn_kernel(cons
         int e = (int)(__float_as_uint(top) >> 23) - 126;
         e = top == 0.f ? 0 : min(max(e, -90), 110);
         const float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
-        constexpr int unit = KX == Codes::kHigh ? 18 : 24;  // log2 of code_unit<KX>(0)
+        constexpr int unit = KX == Codes::kHigh ? 18 : 20;  // log2 of code_unit<KX>(0)
         const float fr = __uint_as_float((uint32_t)(127 - 14 + unit + e) << 23) * fscale;
         const float inv = __uint_as_float((uint32_t)(127 + 14 - unit - e) << 23);
         float mine_sum = 0.f;
