@@ -43,8 +43,8 @@
 // sequences', which starts beside it and joins its sums to every item's.
 //
 // Bound: the codes' way from memory to operand.  131072 tokens of one sequence, 16 heads of 128 (336
-// MB): 77 us = 4340 GB/s, 66% of the measured copy rate; 343 instructions a warp and tile of 16 tokens,
-// issue slots 60% and ALU 52% busy (LOP3, shifts and byte permutes; a tile needs 64 + 16 + 8 of them).
+// MB): 79 us = 4240 GB/s, 65% of the measured copy rate; 358 instructions a warp and tile of 16 tokens,
+// issue slots 61% and ALU 54% busy (LOP3, shifts and byte permutes; a tile needs 64 + 32 + 8 of them).
 // The slope is 83% of the copy rate (131072 to 262144 tokens); the rest is some 20 us of starts, joins
 // and an uneven end.  Tried and slower: 3 and 5 CTAs an SM, steps of 16 and 64 tokens, rings of 1, 3
 // and 4 stages, CTAs of 2 and 8 warps, the next item's copies before this one's sums are joined
