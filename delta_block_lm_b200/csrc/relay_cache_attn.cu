@@ -625,6 +625,31 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E)) cache_attn_kernel(cons
         const bool gap = tok0 < lead && tok0 + STEP > lead_end;  // holds the end of the prefix's last tile
         const bool masked = tok0 + STEP > min(all_see, c1) || have != (1u << TS) - 1 || gap;
         if (masked) {  // what the groups of tokens that are not there hold is not a number that may be used
+            // Drafted tokens that the tile's first rows do not see: a NaN group of their values would reach those rows as
+            // 0 * NaN.  It is put into the sums of the rows that see the token instead.
+            if (tok0 + STEP > all_see && all_see < c1) {
+                static_assert(STEP == 32, "a lane for each token of a step");
+                const int at = tok0 + lane;
+                const bool asked = at >= all_see && at < c1 && (have >> (lane / kCacheTile) & 1);
+#pragma unroll
+                for (int j = 0; j < G; ++j) {
+                    uint32_t* word = reinterpret_cast<uint32_t*>(const_cast<uint8_t*>(st) + lane / kCacheTile * L::TB +
+                                                                 At::value_group(lane % kCacheTile, j));
+                    const float low = group_min(*word);
+                    const bool nan = asked && low != low;
+                    const unsigned who = __ballot_sync(0xffffffffu, nan);
+                    if (who == 0) continue;
+                    if (nan) *word = 0u;
+                    const int first = tok0 + __ffs(who) - 1;
+#pragma unroll
+                    for (int nr = 0; nr < NR; ++nr)
+#pragma unroll
+                        for (int e = 0; e < E; ++e)
+                            if (limit_of(row_at(nr, e)) > first)
+#pragma unroll
+                                for (int i = e; i < 8; i += 2) acc[nr][j][i / 4][i % 4] = NAN;
+                }
+            }
 #pragma unroll
             for (int i = 0; i < TS; ++i)
                 for (int w = lane; w < 2 * kCacheTile * G; w += 32) {

@@ -470,6 +470,39 @@ def test_attention_nan_stays_where_it_is_read(cuda, native_lib):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("tq,g,d,t,prefix", [(3, 1, 64, 2, 0), (4, 2, 128, 33, 0), (5, 1, 128, 130, 21), (3, 8, 64, 300, 0),
+                                             (17, 1, 128, 16, 0)])
+def test_attention_nan_of_later_tokens(cuda, native_lib, dtype, tq, g, d, t, prefix):
+    """What a query does not see yet does not reach it: NaN keys and values of the last two drafted tokens leave the
+    rows before them right, and the rows that see such a token get its NaN where they read it."""
+    rng = np.random.default_rng(tq * t)
+    lens, hkv = [t, t], 2
+    pool, tab, held, kk, vv = _fill(cuda, rng, [prefix] + lens, hkv, d, 16)
+    q = torch.as_tensor(rng.standard_normal((2, tq, hkv * g, d))).to(cuda, dtype)
+    pre = (kk[0], vv[0]) if prefix else (None, None)
+    want = M.attention(q.double().cpu().numpy(), kk[1:], vv[1:], lens, *pre)
+    # the last two tokens once more: the last value of (0, head 1), the one before it, the last key of (1, head 0)
+    k, v = (torch.as_tensor(rng.standard_normal((2, 2, hkv, d)), dtype=F32) for _ in "kv")
+    v[0, 1, 1, 40] = float("inf")
+    v[0, 0, 1, 3] = float("nan")
+    k[1, 1, 0, 5] = float("nan")
+    dbl.relay_cache_append(pool, tab[1:], held[1:] - 2, k.to(cuda), v.to(cuda))
+    kw = dict(prefix_pages=tab[0], prefix_len=prefix) if prefix else {}
+    got = dbl.relay_cache_attention(q, pool, tab[1:], held[1:], **kw)
+    nan = torch.zeros_like(got[0], dtype=torch.bool)
+    nan[0, -1, g:, 32:64] = True
+    nan[0, -2:, g:, :32] = True
+    nan[1, -1, :g] = True
+    assert torch.equal(torch.isnan(got[0]), nan)
+    none = torch.zeros_like(got[2], dtype=torch.bool)
+    none[1, -1, :g] = True
+    assert torch.equal(torch.isnan(got[2]), none)
+    _check_attention([x[:, :-2] for x in got], [x[:, :-2] for x in want], dtype, d, t + prefix)
+    _ok()
+
+
+@gpu
 def test_attention_repeats_streams_strides_and_graphs(cuda, native_lib):
     """The same bits from call to call, with one workspace, on a side stream, from a strided q, in a graph."""
     rng = np.random.default_rng(21)
