@@ -115,6 +115,22 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(CT, 1) cache_fork_k
     }
 }
 
+// Gives every slot [first, end) of every sequence s to visit(s, w): a thread takes a sequence and its first slot; where
+// there are more (prompts), its warp takes them together.  range(s, first, end) says which slots.
+template <int CL, typename Range, typename Visit>
+__device__ __forceinline__ void each_slot(int S, Range range, Visit visit) {
+    for (int s0 = gwarp() * 32; s0 < S; s0 += CL * CT) {
+        const int s = s0 + lane_id();
+        int first = 0, end = 0;
+        if (s < S) range(s, first, end);
+        if (first < end) visit(s, first);
+        for (unsigned more = __ballot_sync(0xffffffffu, end - first > 1); more; more &= more - 1) {
+            const int l = __ffs(more) - 1, w1 = __shfl_sync(0xffffffffu, end, l);
+            for (int w = __shfl_sync(0xffffffffu, first, l) + 1 + lane_id(); w < w1; w += 32) visit(s0 + l, w);
+        }
+    }
+}
+
 // b = tokens of each sequence, or null: p.tokens of each.
 //   scratch: asked [P], last [P], list [P], src [S], dst [S], tiles [S], free [NWARP], want [NWARP]
 template <int CL>
@@ -125,52 +141,60 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(CT, 1) cache_reserv
     int32_t *src = list + p.P, *dst = src + p.S, *tiles = dst + p.S, *nfree = tiles + p.S, *nwant = nfree + NWARP;
     const int warp = gwarp(), lane = lane_id();
     copy_state<CL>(p, false);
-    // the page in which the next token of sequence s falls, where it holds tokens already
-    auto partial = [&](int s, int& len, int& add) -> int {
+    // the slots that the next tokens of sequence s are written to: [len / page, end), cut to the table
+    int len, add;
+    auto range = [&](int s, int& first, int& end) -> bool {  // false: the table has no slots for some of the tokens
         len = max(p.lengths[s], 0);
         add = max(p.b ? p.b[s] : p.tokens, 0);
-        if (add == 0 || len % p.page == 0 || len / p.page >= p.W) return -1;
-        const int page = ld(p.table + entry(p, s, len / p.page));
+        first = len / p.page;
+        const int64_t past = add ? ((int64_t)len + add + p.page - 1) / p.page : 0;
+        end = (int)min(past, (int64_t)p.W);
+        return past <= p.W;
+    };
+    auto held = [&](int s, int w) {  // the page that slot w holds, or -1
+        const int page = ld(p.table + entry(p, s, w));
         return page >= 0 && page < p.P ? page : -1;
     };
-    int len, add;
-    for (int s = gtid(); s < p.S; s += NT) {
-        const int page = partial(s, len, add);
+    // Who is about to write to a page: how many, and the last of them.  Lengths are the caller's and may have been
+    // lowered, so any page of a range may be one that others hold too, not only the one that the range begins in.
+    each_slot<CL>(p.S, range, [&](int s, int w) {
+        const int page = held(s, w);
         if (page >= 0) asked[page] = 0, last[page] = -1;
-    }
+    });
     sync_all<CL>();
-    for (int s = gtid(); s < p.S; s += NT) {
-        const int page = partial(s, len, add);
+    each_slot<CL>(p.S, range, [&](int s, int w) {
+        const int page = held(s, w);
         if (page >= 0) {
             atomicAdd(asked + page, 1);
             atomicMax(last + page, s);
         }
-    }
+    });
     sync_all<CL>();
-    // A holder copies the page it is about to write where others hold it too; if all of its holders
-    // are about to write, the last of them keeps it.
-    auto copies = [&](int s, int page) {
-        const int r = page >= 0 ? ld(p.refs + page) : 0;
-        return r > 1 && !(ld(asked + page) == r && ld(last + page) == s);
+    // A holder replaces the page it is about to write where others hold it too; if all of its holders are about to
+    // write, the last of them keeps it.  Only that last one asks for the page's references, which it alone changes below.
+    auto replaces = [&](int s, int page) {
+        if (ld(last + page) != s) return true;
+        const int r = ld(p.refs + page);
+        return r > 1 && ld(asked + page) < r;
     };
     // does slot w of sequence s need a page?
-    auto wants = [&](int s, int w, bool cow) {
-        const int64_t full = ((int64_t)len + p.page - 1) / p.page, end = ((int64_t)len + add + p.page - 1) / p.page;
-        if (add == 0 || w >= p.W) return false;
-        return (w >= full && w < end && ld(p.table + entry(p, s, w)) < 0) || (cow && w == len / p.page);
+    auto wants = [&](int s, int w, int& page) {
+        page = held(s, w);
+        if (page >= 0) return replaces(s, page);
+        return (int64_t)w * p.page >= len && ld(p.table + entry(p, s, w)) < 0;
     };
     const int rows = (p.S + NWARP - 1) / NWARP, s0 = min(p.S, warp * rows), s1 = min(p.S, s0 + rows);
     const int pages = (p.P + NWARP - 1) / NWARP, p0 = min(p.P, warp * pages), p1 = min(p.P, p0 + pages);
-    int want = 0;
-    bool beyond = false;  // the table has no slots for some of the tokens
+    int want = 0, first, end, page;
+    bool beyond = false;
     for (int s = s0; s < s1; ++s) {
-        const int old = partial(s, len, add);
-        const bool cow = copies(s, old);
-        if (lane == 0) src[s] = cow ? old : -1;
-        const int64_t end = ((int64_t)len + add + p.page - 1) / p.page;
-        beyond = beyond || (add > 0 && end > p.W);
-        for (int64_t w = len / p.page; w < min((int64_t)p.W, end); w += 32)
-            want += __popc(__ballot_sync(0xffffffffu, w + lane < end && wants(s, (int)w + lane, cow)));
+        if (!range(s, first, end)) beyond = true;
+        if (lane == 0) src[s] = -1;
+        for (int w = first; w < end; w += 32) {
+            const bool need = w + lane < end && wants(s, w + lane, page);
+            if (need && page >= 0 && lane == 0 && w == first && len % p.page) src[s] = page;  // it holds tokens: a copy
+            want += __popc(__ballot_sync(0xffffffffu, need));
+        }
     }
     int nf = 0;
     for (int i = p0 + lane; i < p1; i += 32) nf += p.refs[i] == 0;
@@ -195,28 +219,27 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(CT, 1) cache_reserv
     sync_all<CL>();
     at = warp_total(nwant, warp);
     for (int s = s0; s < s1; ++s) {
-        partial(s, len, add);
-        const int old = ld(src + s);  // decided above: the reference counts change now
-        const bool cow = old >= 0;
-        __syncwarp();
+        range(s, first, end);
         if (lane == 0) {
             if (!ok) src[s] = -1;
             tiles[s] = (len % p.page + kCacheTile - 1) / kCacheTile;
         }
         if (!ok) continue;
-        const int64_t end = min((int64_t)p.W, ((int64_t)len + add + p.page - 1) / p.page);
-        for (int64_t w = len / p.page; w < end; w += 32) {
-            const bool need = w + lane < end && wants(s, (int)w + lane, cow);
+        for (int w = first; w < end; w += 32) {
+            const bool in = w + lane < end, need = in && wants(s, w + lane, page);
             const unsigned m = __ballot_sync(0xffffffffu, need);
+            if (in && page >= 0 && ld(last + page) == s) {  // what the page's holders that are about to write leave
+                const int r = ld(p.refs + page), a = ld(asked + page);
+                if (r > 1) p.refs_out[page] = a < r ? r - a : 1;
+            }
             if (need) {
-                const int page = ld(list + at + __popc(m & ((1u << lane) - 1)));
-                p.table_out[entry(p, s, (int)w + lane)] = page;
-                p.refs_out[page] = 1;
-                if (cow && w + lane == len / p.page) dst[s] = page;
+                const int fresh = ld(list + at + __popc(m & ((1u << lane) - 1)));
+                p.table_out[entry(p, s, w + lane)] = fresh;
+                p.refs_out[fresh] = 1;
+                if (w + lane == first) dst[s] = fresh;
             }
             at += __popc(m);
         }
-        if (cow && lane == 0) atomicSub(p.refs_out + old, 1);
     }
 }
 

@@ -325,9 +325,10 @@ def relay_cache_fork(pool, page_table, lengths, refs, parents, children, *, out=
 
 def relay_cache_reserve(pool, page_table, lengths, refs, tokens, *, out=None):
     """Pages for the next ``tokens`` (a number, or a list of one for each sequence) tokens of every
-    sequence.  A page that others hold too is copied before it is written to.  Returns (page_table,
-    refs, missing): ``missing`` [1] is 0, or how many pages the pool lacks, and then nothing changes.
-    ``out``: (page_table, refs)."""
+    sequence.  Every page that they are written to and that others hold too is replaced before (with the
+    tokens that it holds below ``lengths``), so lowering a length drops a sequence's last tokens and no one
+    else's.  Returns (page_table, refs, missing): ``missing`` [1] is 0, or how many pages the pool lacks, and
+    then nothing changes.  ``out``: (page_table, refs)."""
     counts = None
     if isinstance(tokens, torch.Tensor):
         counts, tokens = _ints("tokens", tokens, tuple(lengths.shape)), 0

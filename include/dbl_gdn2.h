@@ -505,10 +505,12 @@ int dbl_relay_cache_release(const dbl_relay_cache_pages_args *args, const int32_
 int dbl_relay_cache_fork(const dbl_relay_cache_pages_args *args, const int32_t *parents,
                          const int32_t *children, int64_t count, dbl_stream_t stream);
 /* Gives every sequence the pages for its next counts[n] tokens (counts NULL: `tokens` each) and
- * makes the page in which they begin its own: where others hold it too, its tiles that hold tokens
- * are copied to a new page (if all holders of a page are about to write, the last of them keeps
- * it).  lengths_out is not used.  *missing: 0, or, where the pool has too few free pages, how many
- * are missing; then nothing is changed. */
+ * makes every page that they are written to its own: one that others hold too is replaced by a new
+ * page, to which the tiles that hold tokens below lengths[n] are copied (if all holders of a page are
+ * about to write, the last of them keeps it).  lengths may have been lowered since the pages were
+ * shared: that drops a sequence's last tokens and leaves the other holders theirs.  lengths_out is
+ * not used.  *missing: 0, or, where the pool has too few free pages, how many are missing; then
+ * nothing is changed. */
 int dbl_relay_cache_reserve(const dbl_relay_cache_pages_args *args, const int32_t *counts,
                             int64_t tokens, int32_t *missing, void *workspace,
                             size_t workspace_bytes, dbl_stream_t stream);
