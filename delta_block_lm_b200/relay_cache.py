@@ -27,6 +27,7 @@ from __future__ import annotations
 import ctypes
 import math
 import struct
+import threading
 from typing import Optional
 
 import torch
@@ -194,20 +195,25 @@ def relay_cache_read(pool, page_table, lengths, *, start=None, tokens: int, dtyp
     return k, v
 
 
-_workspaces: dict = {}  # (what for, device, stream): a workspace kept from call to call
+_workspaces = threading.local()  # .kept: (what for, device, stream) -> a workspace kept from call to call
 
 
 def _workspace(what: str, need: int, dev: int, stream: int) -> torch.Tensor:
-    """A workspace whose counters (the attention's) are zero.  Calls on one stream follow one another, so
-    each stream keeps one; a graph that is being captured gets its own (it may be replayed beside other
+    """A workspace whose counters (the attention's) are zero.  The calls of one thread on one stream follow
+    one another, so each thread keeps one a stream; launches of two threads may interleave between the
+    two launches of a call.  A graph that is being captured gets its own (it may be replayed beside other
     calls)."""
     capturing = torch._C._cuda_isCurrentStreamCapturing()
-    ws = None if capturing else _workspaces.get((what, dev, stream))
+    try:
+        kept = _workspaces.kept
+    except AttributeError:
+        kept = _workspaces.kept = {}
+    ws = None if capturing else kept.get((what, dev, stream))
     if ws is None or ws.numel() < need:
         ws = torch.empty(need, device=torch.device("cuda", dev), dtype=torch.uint8)
         ws[:N.RELAY_CACHE_COUNTER_BYTES].zero_()
         if not capturing:
-            _workspaces[what, dev, stream] = ws
+            kept[what, dev, stream] = ws
     return ws
 
 
@@ -219,9 +225,9 @@ def relay_cache_attention(q, pool, page_table, lengths, *, prefix_pages=None, pr
     themselves; f32 or bf16, heads a multiple of the pool's kv heads.  ``lengths`` counts the queries'
     own tokens (append first).  ``prefix_pages`` [width] names the pages of ``prefix_len`` tokens that
     every sequence sees before its own.  ``workspace``: a uint8 tensor whose first
-    ``RELAY_CACHE_COUNTER_BYTES`` bytes are zero before its first use (by default each stream keeps one, until the
-    process ends).  Returns (o, row_max, row_sum) as ``relay_merge_decode``; a row without keys gives o = 0
-    and (0, 1)."""
+    ``RELAY_CACHE_COUNTER_BYTES`` bytes are zero before its first use, and that no other thread uses
+    meanwhile (by default each thread keeps one a stream, until it ends).  Returns (o, row_max, row_sum) as
+    ``relay_merge_decode``; a row without keys gives o = 0 and (0, 1)."""
     dev = _device(q, pool, page_table, lengths, prefix_pages, out, workspace)
     c = _cache(pool)
     shape = q.shape

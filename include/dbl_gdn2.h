@@ -464,7 +464,9 @@ int dbl_relay_cache_read(const dbl_relay_cache_read_args *args, dbl_stream_t str
  * dbl_relay_merge_decode (o = 0, max = 0, sum = 1).
  * The workspace (dbl_relay_cache_attention_workspace_bytes, 16-byte aligned) holds counters in its
  * first DBL_RELAY_CACHE_COUNTER_BYTES bytes, which must be zero before its first use; every call leaves them
- * zero again.  Calls that overlap on the GPU must use distinct workspaces. */
+ * zero again.  Calls that overlap on the GPU must use distinct workspaces, and so must host threads
+ * that make calls at the same time, even on one stream: a call can be two launches, the second of
+ * which reads what the first left in the workspace. */
 #define DBL_RELAY_CACHE_COUNTER_BYTES 8192
 typedef struct {
     dbl_relay_cache cache;
@@ -493,7 +495,8 @@ typedef struct {
     int32_t *page_table_out, *lengths_out, *refs_out;
 } dbl_relay_cache_pages_args;
 
-/* Scratch bytes of reserve and compact (16-byte aligned; need not be cleared). */
+/* Scratch bytes of reserve and compact (16-byte aligned; need not be cleared; two launches a call, so
+ * not shared as the attention's workspace is not). */
 size_t dbl_relay_cache_pages_workspace_bytes(int64_t pages, int64_t n_seq);
 
 /* Releases sequences: their rows become -1, their lengths 0, and a page is free (refs 0) once no

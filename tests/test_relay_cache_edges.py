@@ -123,3 +123,85 @@ def test_a_cut_fork_leaves_the_other_sequence_alone(cuda, native_lib, cut, more)
     _ok()
 
 
+# ------------------------------------------------------------------------------------------ threads, streams, graphs
+def test_threads_do_not_share_a_workspace(monkeypatch):
+    """A call can be two launches that hand results over in its workspace, and the interpreter lock is let go in between:
+    host threads on one stream need workspaces of their own, and one thread keeps its own from call to call."""
+    real = torch.empty
+    monkeypatch.setattr(torch, "empty", lambda *a, device=None, **kw: real(*a, **kw))
+    monkeypatch.setattr(torch._C, "_cuda_isCurrentStreamCapturing", lambda: False)
+    ready, got = threading.Barrier(2, timeout=30), [None, None]
+
+    def work(i):
+        mine = R._workspace("attention", 9000, 0, 7)
+        ready.wait()
+        got[i] = mine.data_ptr(), R._workspace("attention", 8500, 0, 7).data_ptr(), mine
+        ready.wait()
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert got[0][0] != got[1][0]
+    assert all(first == again for first, again, _ in got)
+
+
+@gpu
+def test_two_threads_on_one_stream(cuda, native_lib):
+    """Attention with a launch of the prefix's own, reserve with copies and compact, from two host threads on the default
+    stream, each with its own state: every result is the one that the thread gets alone."""
+    rng = np.random.default_rng(3)
+
+    def job(i):
+        n, hkv, d, page, prefix = 8, 16, 64, 64, 4096 + 64 * i
+        pool = dbl.relay_cache_pool(100 + n, hkv, d, page, device=cuda)
+        tab = torch.arange(100 + n, device=cuda, dtype=torch.int32)
+        k, v = (torch.as_tensor(rng.standard_normal((1, prefix + 40 * n, hkv, d))).to(cuda, BF16) for _ in "kv")
+        dbl.relay_cache_append(pool, tab[None], _i32([0], cuda), k, v)
+        q = torch.as_tensor(rng.standard_normal((n, hkv, d))).to(cuda, BF16)
+        own, lens = tab[60:60 + n, None].contiguous(), _i32(range(5, 5 + n), cuda)
+        # pages 0 .. 9 of two sequences, the second a fork of the first, holes between them
+        table = torch.full((4, 12), -1, device=cuda, dtype=torch.int32)
+        table[0, :10] = torch.arange(0, 30, 3, device=cuda) + i
+        table[1:3] = table[0]
+        refs = torch.zeros(len(pool), device=cuda, dtype=torch.int32)
+        refs[table[0, :10].long()] = 3
+        small = pool.clone()
+
+        def attend():
+            return dbl.relay_cache_attention(q, pool, own, lens, prefix_pages=tab[:66], prefix_len=prefix)
+
+        def pages():
+            p = small.clone()
+            t, r, missing = dbl.relay_cache_reserve(p, table, _i32([600, 600, 600, 0], cuda), refs, 30)
+            t, r, used = dbl.relay_cache_compact(p, t, r)
+            return p, t, r, missing, used
+
+        return attend, pages
+
+    jobs = [job(i) for i in range(2)]
+    want = [[f() for f in j] for j in jobs]
+    torch.cuda.synchronize()
+    wrong, failures = [torch.zeros(1, device=cuda, dtype=torch.int64) for _ in jobs], []
+    ready = threading.Barrier(2, timeout=60)
+
+    def work(i):
+        try:
+            ready.wait()
+            for _ in range(150):
+                for f, w in zip(jobs[i], want[i]):
+                    for a, b in zip(f(), w):
+                        wrong[i] += (a != b).any()
+        except Exception as e:  # noqa: BLE001
+            failures.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures and [int(x) for x in wrong] == [0, 0]
+    _ok()
+
+
