@@ -373,11 +373,12 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E)) cache_attn_kernel(cons
     // An item's tokens: the prefix's where it has no launch of its own, to the end of their last tile, then
     // the sequence's.
     const int lead = p.lead, lead_end = lead ? p.prefix_len : 0;
-    auto length_of = [&](int n) {
-        return pre ? p.prefix_len : lead + min(max(p.lengths[n], 0), p.c.width * p.c.tiles * kCacheTile);
-    };
+    const int most = p.c.width * p.c.tiles * kCacheTile;  // own tokens that the table has entries for
     const int start = pre ? 0 : kStart;
-    auto units_of = [&](int n) { return start + max(1, (length_of(n) + UNIT - 1) / UNIT); };
+    auto units_of = [&](int n) {
+        const int len = pre ? p.prefix_len : lead + min(max(p.lengths[n], 0), most);
+        return start + max(1, (len + UNIT - 1) / UNIT);
+    };
     int run, pos, end, seq = 0, base = 0;  // base: units before sequence seq
     if (pre) {
         run = p.pre_run;
@@ -441,12 +442,14 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E)) cache_attn_kernel(cons
         q = x / p.group;
         hq = h * p.group + x % p.group;
     };
-    const int len = length_of(seq);
+    const int len = pre ? p.prefix_len : max(p.lengths[seq], 0);
     auto row_at = [&](int nr, int e) { return E == 2 ? 8 * nr + 2 * t + e : 4 * nr + t; };  // of the lane's column e
     auto limit_of = [&](int r) {
         if (r >= rows) return 0;
-        return pre ? len : max(lead, len - p.Tq + (rt * R + r) / p.group + 1);
+        return pre ? len : lead + min(max(len - p.Tq + (rt * R + r) / p.group + 1, 0), most);
     };
+    // Tokens that the table has no entries for are left out; the queries still count from the length.
+    if (!pre && len > most && threadIdx.x == 0) atomicExch(p.err, kCacheErrorPage);
     const int c0 = u0 * UNIT, c1 = min(u1 * UNIT, limit_of(rows - 1));  // later rows see more
     const int all_see = limit_of(0);                                         // tokens below it need no mask
     const int steps = c1 > c0 ? (c1 - c0 + STEP - 1) / STEP : 0;

@@ -457,7 +457,8 @@ int dbl_relay_cache_read(const dbl_relay_cache_read_args *args, dbl_stream_t str
 
 /* Attention of the last `queries` tokens of each sequence over a prefix that all sequences share
  * (prefix_len tokens in the pages prefix_pages names) and the sequence's own lengths[n] tokens,
- * which include the queries' own: query t sees own keys below lengths[n] - queries + t + 1.
+ * which include the queries' own: query t sees own keys below lengths[n] - queries + t + 1, of which
+ * those without a page are left out and recorded (code 102).
  * q [n_seq, queries, heads, head_dim] (strides in elements, innermost 1); head h reads kv head
  * h / (heads / kv_heads).  out [n_seq, queries, heads, head_dim] in dtype and row_max, row_sum f32
  * [n_seq, queries, heads] are contiguous; the statistics and the empty row are those of

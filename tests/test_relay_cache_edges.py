@@ -123,6 +123,96 @@ def test_a_cut_fork_leaves_the_other_sequence_alone(cuda, native_lib, cut, more)
     _ok()
 
 
+# ------------------------------------------------------------------------------------------ attention
+def _attend(q, kk, vv, lens, pre=(None, None), scale=None):
+    """The model's result and, for each row and channel, sum p (|minimum| + 8 scale) / l and max p scale / l of what the
+    cache holds of its group: the sizes that the rounding of p goes by.  kk, vv: lists of (scale, minimum, code)."""
+    full = lambda x: (x[1][..., None] + x[0][..., None] * x[2]).reshape(*x[0].shape[:-1], -1)  # noqa: E731
+    join = lambda a, b: b if a is None else tuple(np.concatenate([x, y]) for x, y in zip(a, b))  # noqa: E731
+    n, tq, h, d = q.shape
+    scale = d ** -0.5 if scale is None else scale
+    o, mx, sm = np.zeros(q.shape), np.zeros(q.shape[:3]), np.ones(q.shape[:3])
+    size, most, mass = np.zeros(q.shape), np.zeros(q.shape), np.zeros(q.shape[:3])
+    count = np.ones(q.shape[:3])
+    for i in range(n):
+        for t in range(tq):
+            end = max(0, lens[i] - tq + t + 1)
+            keys, vals = (join(p, tuple(y[:end] for y in x[i])) for p, x in zip(pre, (kk, vv)))
+            if len(keys[0]) == 0:
+                continue
+            kf, vf = full(keys), full(vals)
+            for a in range(h):
+                b = a // (h // kf.shape[1])
+                s = kf[:, b] @ q[i, t, a] * scale
+                m = s.max()
+                p = np.exp(s - m)
+                l = p.sum()
+                o[i, t, a], mx[i, t, a], sm[i, t, a] = p @ vf[:, b] / l, m, l
+                per = p[:, None] * (np.abs(vals[1][:, b]) + 8 * vals[0][:, b]) / l
+                size[i, t, a] = np.repeat(per.sum(0), M.GROUP)
+                most[i, t, a] = np.repeat((p[:, None] * vals[0][:, b] / l).max(0), M.GROUP)
+                mass[i, t, a] = (np.abs(kf[:, b]) @ np.abs(q[i, t, a])).max() * abs(scale)
+                count[i, t, a] = len(s)
+    return o, mx, sm, size, most, mass, count
+
+
+def _check(got, want, dtype):
+    """Channel by channel.  A score is off by 2 d + 8 roundings of its terms (f32 sums) and p by 2 more units; p scale
+    is rounded to f16 once (bf16 rows: 2^-12 of it) or twice (f32 rows: 2^-22 at the least), with a floor of 2^-25 where
+    the largest is 2^7, so 2^-32 of the largest for each of at most `count` keys and codes up to 8 from zero; p to two
+    bf16 parts for the minima (2^-17); sums over the keys; the output's own rounding."""
+    o, mx, sm = (x.double().cpu().numpy().reshape(w.shape) for x, w in zip(got, want))
+    eo, em, es, size, most, mass, count = want
+    d = eo.shape[-1]
+    ds = (2 * d + 8) * U32 * mass + 4 * U32 + U32 * np.abs(em)
+    tail = np.sqrt(count) * 4 * U32
+    assert (np.abs(mx - em) <= ds).all()
+    assert (np.abs(sm - es) <= es * (2 * ds + tail) + U32).all()
+    dp = 2.0 ** -12 + 2.0 ** -17 if dtype == BF16 else 2.0 ** -22
+    tol = size * (2 * ds + tail + dp)[..., None] + count[..., None] * 2.0 ** -29 * most
+    tol = tol * (1 + 2.0 ** -7) + np.abs(eo) * (2.0 ** -8 if dtype == BF16 else U32)
+    assert np.isfinite(o).all()
+    assert (np.abs(o - eo) <= tol).all(), float((np.abs(o - eo) / np.maximum(tol, 1e-300)).max())
+
+
+def _cache(dev, k, v, page):
+    """A pool that holds the sequences k[i], v[i] [length, Hkv, D] (tensors on the device), its table and lengths, and
+    what it keeps of them."""
+    lens = [len(x) for x in k]
+    table, pages, _ = _tables(np.random.default_rng(0), lens, page)
+    pool = dbl.relay_cache_pool(pages, k[0].shape[1], k[0].shape[2], page, device=dev)
+    pool.fill_(255)
+    tab, zero = _i32(table, dev), _i32([0], dev)
+    for i, n in enumerate(lens):
+        dbl.relay_cache_append(pool, tab[i:i + 1], zero, k[i][None], v[i][None])
+    kept = [[M.quantise(x.double().cpu().numpy()) for x in y] for y in (k, v)]
+    return pool, tab, _i32(lens, dev), *kept
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("tq,g,prefix,n", [(1, 1, 0, 2), (1, 2, 21, 3), (2, 1, 0, 2), (9, 1, 0, 2), (9, 2, 37, 2), (3, 1, 33000, 4)])
+def test_attention_lengths_past_the_table(cuda, native_lib, dtype, tq, g, prefix, n):
+    """A table of 2 pages of 16 tokens and lengths up to 40: the queries count from the length, the tokens that the table
+    has no pages for are left out and recorded."""
+    rng = np.random.default_rng(tq)
+    hkv, d, page = 4, 64, 16
+    assert prefix == 33000 or n * hkv * prefix < 1 << 19  # with and without a launch of the prefix's own
+    lens = [32] * n
+    k, v = ([torch.as_tensor(rng.standard_normal((x, hkv, d))).to(cuda, BF16) for x in [prefix] + lens] for _ in "kv")
+    pool, tab, held, kk, vv = _cache(cuda, k, v, page)
+    own = tab[1:, :2].contiguous()
+    q = torch.as_tensor(rng.standard_normal((n, tq, hkv * g, d))).to(cuda, dtype)
+    kw = dict(prefix_pages=tab[0], prefix_len=prefix) if prefix else {}
+    pre = (kk[0], vv[0]) if prefix else (None, None)
+    for past in (0, 1, 8, 40, 2 ** 31 - 33):
+        now = [32 + past] + [32] * (n - 1)
+        got = dbl.relay_cache_attention(q, pool, own, _i32(now, cuda), **kw)
+        assert _device_code() == (102 if past else 0)
+        _check(got, _attend(q.double().cpu().numpy(), kk[1:], vv[1:], now, pre), dtype)
+    _ok()
+
+
 # ------------------------------------------------------------------------------------------ threads, streams, graphs
 def test_threads_do_not_share_a_workspace(monkeypatch):
     """A call can be two launches that hand results over in its workspace, and the interpreter lock is let go in between:
