@@ -29,7 +29,8 @@
 //   * the scores arrive with tokens in rows and have to leave with tokens along the product's
 //     inner dimension: movmatrix transposes the 8 x 8 blocks.
 // The running maximum is only raised when a score passes it by 8 (in powers of two), so a step
-// usually costs one vote instead of the shuffles of a maximum and the rescaling of the sums.
+// usually costs one vote instead of the shuffles of a maximum and the rescaling of the sums.  p is relative
+// to that bound, not to the maximum, so it is never above 1 and the sums of large values stay in range.
 //
 // Work: an item is (sequence, kv head, up to 8 NR rows), or (kv head, up to 8 NR rows of all
 // sequences) of a prefix that is worth a launch of its own, which is thus read once per head for 8 NR
@@ -600,7 +601,7 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E)) cache_attn_kernel(cons
     float omin[NR][E][G];    // f32: sum p (min + 8 scale) of this lane's tokens
     float pacc[NR][4];       // bf16: sum p scale, sum p min: lanes g = 2 j, 2 j + 1 hold group j
     float l[NR][E], top[NR][E];      // sums; largest inner score of the lane
-    float ref[NR][E], bar_[NR][E];   // p = 2^(f inner - ref); the inner score at which ref is raised
+    float ref[NR][E], bar_[NR][E];   // p = 2^(f inner - ref) <= 1; the inner score at which ref is raised
     float wtop[NR][E], mult[NR][E];  // largest p scale of the lane; r = p scale mult, a power of two
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr) {
@@ -758,7 +759,7 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E)) cache_attn_kernel(cons
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     const float m = over_g_max(top[nr][e]);
-                    const float to = m == -INFINITY ? 0.f : m * f[nr][e];
+                    const float to = m == -INFINITY ? 0.f : m * f[nr][e] + kSlack;  // so that p stays at most 1
                     c[e] = bar_[nr][e] == -INFINITY ? 0.f : ex2(ref[nr][e] - to);
                     ref[nr][e] = to;
                     bar_[nr][e] = m + kSlack / f[nr][e];

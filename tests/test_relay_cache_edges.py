@@ -213,6 +213,24 @@ def test_attention_lengths_past_the_table(cuda, native_lib, dtype, tq, g, prefix
     _ok()
 
 
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_values_near_the_largest(cuda, native_lib, dtype, d):
+    """Values of 2^120, and scores that rise by 5.4 after the running maximum was set: the sums stay in range where p is
+    at most 1 (264 tokens of 2^120), and so does the result."""
+    rng = np.random.default_rng(d)
+    t = 264
+    k = rng.standard_normal((t, 1, d)) * 1e-3
+    k[260:] += 5.4 / d ** 0.5
+    v = rng.uniform(1.8, 1.99, (t, 1, d)) * 2.0 ** 119
+    k, v = (torch.as_tensor(x).to(cuda, BF16) for x in (k, v))
+    pool, tab, held, kk, vv = _cache(cuda, [k], [v], 16)
+    q = torch.ones((1, 1, 1, d), device=cuda, dtype=dtype)
+    _check(dbl.relay_cache_attention(q, pool, tab, held), _attend(q.double().cpu().numpy(), kk, vv, [t]), dtype)
+    _ok()
+
+
 # ------------------------------------------------------------------------------------------ threads, streams, graphs
 def test_threads_do_not_share_a_workspace(monkeypatch):
     """A call can be two launches that hand results over in its workspace, and the interpreter lock is let go in between:
