@@ -21,8 +21,8 @@
 //     numbers around zero (code - 8), so that long sums neither drop bits nor cancel:
 //     o = sum r (code - 8) + sum p (min + 8 scale), r the rounded p scale.
 //   * q is held in f16 relative to a power of two of its own row (bf16 q: exact; f32 q: two f16
-//     parts, 22 bits), p scale in f16 relative to a power of two near the row's largest (f32: again
-//     two parts).
+//     parts, 22 bits), p scale in f16 relative to a power of two near the largest of its row and group of
+//     channels (f32: again two parts), so that a group of small values is as exact as one of large ones.
 //   * the minima are operands as they lie in memory: a token's (scale, minimum) words are the bf16
 //     pairs of a row, met by zeros in the scales' places (keys), or read by a transposing ldmatrix
 //     (values, which also gives the sums of p scale); sum(q) and p are given in bf16 parts.
@@ -77,7 +77,8 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr int64_t kMostTokens = (int64_t)1 << 27;
 constexpr float kSlack = 8.f;     // how far a score may pass the running maximum (powers of two)
 constexpr float kMostF16 = 60000.f;             // p scale mult stays below it
-constexpr float kMostMult = 1.2676506e30f;      // 2^100
+constexpr float kMostMult = 8.507059173e37f;    // 2^126
+constexpr int kMostMultBits = 127 + 126;        // its exponent's bits
 
 struct AttnParams {
     CacheView c;
@@ -173,6 +174,11 @@ __device__ __forceinline__ void split_f16x2(float a, float b, uint32_t& hi, uint
     hi = pack_f16x2(a, b);
     lo = pack_f16x2(a - f16x2_lo(hi), b - f16x2_hi(hi));
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
 __device__ __forceinline__ float over_g_max(float x) {  // over the lanes of the same column pair
 #pragma unroll
     for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
@@ -184,13 +190,16 @@ __device__ __forceinline__ float over_g_sum(float x) {
     return x;
 }
 
-// The power of two that takes w to 2^7 .. 2^8 (p may grow by kSlack before it is raised again, and f16 holds
-// what is 2^-22 of it to 11 bits), and the inverse of a power of two.
+// The power of two that takes w to 2^7 .. 2^8 (what is added later may be 2^8 times as large before it is lowered,
+// and f16 holds what is 2^-22 of it to 11 bits), and the inverse of a power of two.
 __device__ __forceinline__ float mult_for(float w) {
-    const int e = min(max((int)(__float_as_uint(w) >> 23), 40), 250);
+    const int e = min(max((int)(__float_as_uint(w) >> 23), 261 - kMostMultBits), 250);
     return __uint_as_float((uint32_t)(261 - e) << 23);
 }
 __device__ __forceinline__ float pow2_inverse(float x) { return __uint_as_float((254u << 23) - __float_as_uint(x)); }
+__device__ __forceinline__ float pow2(int e) {  // 0 below 2^-126; e < 128
+    return e < -126 ? 0.f : __uint_as_float((uint32_t)(127 + e) << 23);
+}
 
 // The operand registers of the 8 codes of w, codes (0, 4), (1, 5), (2, 6), (3, 7), and what they are
 // multiplied by to be the codes (code_unit).
@@ -336,15 +345,16 @@ struct AttnLayout {
 
 // NR groups of 8 columns; E = 2: a row in every column, E = 1 (up to 4 rows): in the even columns only,
 // which saves the arithmetic of the others (a lane holds two neighbouring columns of every product).
-// CTAs that an SM holds, by the registers that a tile's sums take.
-constexpr int held_at(int nr, int e) { return nr == 2 ? 2 : e == 2 ? 3 : 4; }
+// CTAs that an SM holds, by the registers that a tile's sums and operands take.  f32 rows, up to 4 of them, at 3 and 4
+// CTAs: one sequence of 100000 tokens, 16 heads of 128, 83.9 and 99.5 us, 16 of 500 to 4000 tokens 49 and 57 us.
+constexpr int held_at(int nr, int e, bool bf16) { return nr == 2 ? 2 : e == 2 || !bf16 ? 3 : 4; }
 template <int NR, int E>
 constexpr int rows_of_tile() { return NR * 4 * E; }
 
 // LATER: a row tile's rows may see different numbers of keys (several queries a sequence).  Without it single tokens save
 // the registers of that case: 131072 tokens 79.6 us, with it 81.5; 64 sequences after a prefix 82.2 and 84 us.
 template <int D, typename T, int NR, int E, bool LATER>
-__global__ void __launch_bounds__(W * 32, held_at(NR, E)) cache_attn_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(W * 32, held_at(NR, E, sizeof(T) == 2)) cache_attn_kernel(const AttnParams p) {
     constexpr int R = rows_of_tile<NR, E>();
     using L = AttnLayout<D, T, R>;
     using At = TileAt<D>;
@@ -352,6 +362,9 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E)) cache_attn_kernel(cons
     constexpr bool SPLIT = sizeof(T) == 4;
     constexpr int NP = SPLIT ? 2 : 1;  // f16 parts of q and of p
     constexpr int PER = 16 / sizeof(T);
+    // Tiles whose p scale is looked over at once: one vote a step costs the operands' registers, which one row a lane
+    // leaves (131072 tokens 80.2 us, with a vote a tile 81.1); 16 rows spill with it (six drafts 40.5 us for 35.3).
+    constexpr int AHEAD = !SPLIT && NR * E == 1 ? TS : 1;
     constexpr Codes KX = SPLIT ? Codes::kHigh : Codes::kMid, VX = Codes::kCentred;
     extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -602,7 +615,7 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E)) cache_attn_kernel(cons
     float pacc[NR][4];       // bf16: sum p scale, sum p min: lanes g = 2 j, 2 j + 1 hold group j
     float l[NR][E], top[NR][E];      // sums; largest inner score of the lane
     float ref[NR][E], bar_[NR][E];   // p = 2^(f inner - ref) <= 1; the inner score at which ref is raised
-    float wtop[NR][E], mult[NR][E];  // largest p scale of the lane; r = p scale mult, a power of two
+    float mult[NR][E][G];            // r = p scale mult, a power of two for each row and group
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr) {
 #pragma unroll
@@ -613,11 +626,10 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E)) cache_attn_kernel(cons
         for (int i = 0; i < 4; ++i) pacc[nr][i] = 0.f;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            l[nr][e] = wtop[nr][e] = ref[nr][e] = 0.f;
-            mult[nr][e] = kMostMult;
+            l[nr][e] = ref[nr][e] = 0.f;
             top[nr][e] = bar_[nr][e] = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < G; ++j) omin[nr][e][j] = 0.f;
+            for (int j = 0; j < G; ++j) omin[nr][e][j] = 0.f, mult[nr][e][j] = kMostMult;
         }
     }
 
@@ -728,19 +740,6 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E)) cache_attn_kernel(cons
                         }
                 }
         }
-        // a bound of each token's value scales: their sum
-        float sa_top[TS], sb_top[TS];
-#pragma unroll
-        for (int i = 0; i < TS; ++i) {
-            const uint8_t* tile = st + i * L::TB;
-            const Words<G> va = lds_words<G>(tile + At::value_group(g, 0)), vb = lds_words<G>(tile + At::value_group(g + 8, 0));
-            uint32_t a = add_bf16x2(va.w[0], va.w[1]), b = add_bf16x2(vb.w[0], vb.w[1]);
-            if constexpr (G == 4) {
-                a = add_bf16x2(a, add_bf16x2(va.w[2], va.w[3]));
-                b = add_bf16x2(b, add_bf16x2(vb.w[2], vb.w[3]));
-            }
-            sa_top[i] = group_scale(a), sb_top[i] = group_scale(b);
-        }
         bool raise = false;
 #pragma unroll
         for (int nr = 0; nr < NR; ++nr)
@@ -755,78 +754,95 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E)) cache_attn_kernel(cons
         if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
             for (int nr = 0; nr < NR; ++nr) {
-                float c[E], back[E], forth[E];
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     const float m = over_g_max(top[nr][e]);
                     const float to = m == -INFINITY ? 0.f : m * f[nr][e] + kSlack;  // so that p stays at most 1
-                    c[e] = bar_[nr][e] == -INFINITY ? 0.f : ex2(ref[nr][e] - to);
+                    // p, and with it what has been summed, shrinks by c; mult grows by the power of two in it
+                    const float by = bar_[nr][e] == -INFINITY ? 0.f : fminf(to - ref[nr][e], 400.f);
+                    const float c = ex2(-by), rest = ex2(floorf(by) - by);
                     ref[nr][e] = to;
                     bar_[nr][e] = m + kSlack / f[nr][e];
-                    l[nr][e] *= c[e];
-                    wtop[nr][e] *= c[e];
-                    back[e] = pow2_inverse(mult[nr][e]);
-                    forth[e] = mult[nr][e] = mult_for(over_g_max(wtop[nr][e]));
-                    if constexpr (SPLIT) {
+                    l[nr][e] *= c;
+                    pacc[nr][e] *= c;
 #pragma unroll
-                        for (int j = 0; j < G; ++j) omin[nr][e][j] *= c[e];
+                    for (int j = 0; j < G; ++j) {
+                        if constexpr (SPLIT) omin[nr][e][j] *= c;
+                        const int bits = (int)(__float_as_uint(mult[nr][e][j]) >> 23) + (int)by, past = max(bits - kMostMultBits, 0);
+                        mult[nr][e][j] = __uint_as_float((uint32_t)(bits - past) << 23);
+                        if (done == 0) continue;  // the sums are zero
+#pragma unroll
+                        for (int i = e; i < 8; i += 2) acc[nr][j][i / 4][i % 4] *= rest * pow2(-past);
                     }
-                    pacc[nr][e] *= c[e];
-                    if (done == 0) continue;  // the sums are zero
-#pragma unroll
-                    for (int j = 0; j < G; ++j)
-#pragma unroll
-                        for (int i = e; i < 8; i += 2) acc[nr][j][i / 4][i % 4] *= back[e] * c[e] * forth[e];
                 }
             }
         }
         // p, relative to ref
-        raise = false;
 #pragma unroll
         for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                float w = 0.f;
+            for (int e = 0; e < E; ++e)
 #pragma unroll
                 for (int i = 0; i < TS; ++i) {
                     s[i][nr][e] = ex2(fmaf(s[i][nr][e], f[nr][e], -ref[nr][e]));
                     s[i][nr][E + e] = ex2(fmaf(s[i][nr][E + e], f[nr][e], -ref[nr][e]));
                     l[nr][e] += s[i][nr][e] + s[i][nr][E + e];
-                    w = fmaxf(w, fmaxf(s[i][nr][e] * sa_top[i], s[i][nr][E + e] * sb_top[i]));
                 }
-                wtop[nr][e] = fmaxf(wtop[nr][e], w);
-                raise = raise || w * mult[nr][e] > kMostF16;
+        // r = p scale mult of AHEAD tiles from i0 on as operands, and the largest of them
+        uint32_t rw[AHEAD][NR][G][2][NP];  // tokens g and g + 8
+        auto weigh = [&](int i0) {
+            float most = 0.f;
+#pragma unroll
+            for (int k = 0; k < AHEAD; ++k) {
+                const uint8_t* tile = st + (i0 + k) * L::TB;
+                const Words<G> va = lds_words<G>(tile + At::value_group(g, 0)), vb = lds_words<G>(tile + At::value_group(g + 8, 0));
+#pragma unroll
+                for (int j = 0; j < G; ++j) {
+                    const float sa = group_scale(va.w[j]), sb = group_scale(vb.w[j]);
+#pragma unroll
+                    for (int nr = 0; nr < NR; ++nr) {
+                        float ra[2] = {0.f, 0.f}, rb[2] = {0.f, 0.f};
+#pragma unroll
+                        for (int e = 0; e < E; ++e) {
+                            ra[e] = s[i0 + k][nr][e] * sa * mult[nr][e][j];
+                            rb[e] = s[i0 + k][nr][E + e] * sb * mult[nr][e][j];
+                            most = max3(most, ra[e], rb[e]);
+                        }
+                        if constexpr (SPLIT) {
+                            split_f16x2(ra[0], ra[1], rw[k][nr][j][0][0], rw[k][nr][j][0][NP - 1]);
+                            split_f16x2(rb[0], rb[1], rw[k][nr][j][1][0], rw[k][nr][j][1][NP - 1]);
+                        } else {
+                            rw[k][nr][j][0][0] = pack_f16x2(ra[0], ra[1]);
+                            rw[k][nr][j][1][0] = pack_f16x2(rb[0], rb[1]);
+                        }
+                    }
+                }
             }
-        if (__any_sync(0xffffffffu, raise)) {
+            return most;
+        };
+        auto lower = [&](int i0) {  // mult of the rows and groups whose r left f16's range
 #pragma unroll
-            for (int nr = 0; nr < NR; ++nr)
+            for (int k = 0; k < AHEAD; ++k) {
+                const uint8_t* tile = st + (i0 + k) * L::TB;
+                const Words<G> va = lds_words<G>(tile + At::value_group(g, 0)), vb = lds_words<G>(tile + At::value_group(g + 8, 0));
 #pragma unroll
-                for (int e = 0; e < E; ++e) {
-                    const float m = fminf(mult[nr][e], mult_for(over_g_max(wtop[nr][e])));
-                    const float c = pow2_inverse(mult[nr][e]) * m;
-                    mult[nr][e] = m;
-                    if (done == 0) continue;
+                for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-                    for (int j = 0; j < G; ++j)
+                    for (int e = 0; e < E; ++e)
 #pragma unroll
-                        for (int i = e; i < 8; i += 2) acc[nr][j][i / 4][i % 4] *= c;
-                }
-        }
+                        for (int j = 0; j < G; ++j) {
+                            const float w = fmaxf(s[i0 + k][nr][e] * group_scale(va.w[j]), s[i0 + k][nr][E + e] * group_scale(vb.w[j]));
+                            const float m = fminf(mult[nr][e][j], mult_for(over_g_max(w)));
+                            const float c = pow2_inverse(mult[nr][e][j]) * m;
+                            mult[nr][e][j] = m;
+#pragma unroll
+                            for (int x = e; x < 8; x += 2) acc[nr][j][x / 4][x % 4] *= c;
+                        }
+            }
+        };
 #pragma unroll
         for (int i = 0; i < TS; ++i) {
             const uint8_t* tile = st + i * L::TB;
-            // codes of channels 4 g .. + 3 of every group, of tokens 2 t, 2 t + 1 (+ 8): 16 bits each
-            uint32_t x[2][G];
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const Words<G> w = lds_words<G>(tile + At::value_half(8 * u + 2 * t, g, 0));
-#pragma unroll
-                for (int j = 0; j < G; j += 2) {
-                    x[u][j] = __byte_perm(w.w[j / 2], w.w[G / 2 + j / 2], 0x5410);
-                    x[u][j + 1] = __byte_perm(w.w[j / 2], w.w[G / 2 + j / 2], 0x7632);
-                }
-            }
-            const Words<G> va = lds_words<G>(tile + At::value_group(g, 0)), vb = lds_words<G>(tile + At::value_group(g + 8, 0));
             if constexpr (!SPLIT) {  // p in two bf16 parts
                 uint32_t w[4];
                 group_operands<G>(tile + At::value_group(0, 0), lane, w);
@@ -840,38 +856,40 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E)) cache_attn_kernel(cons
                     mma_bf16(pacc[nr], w, transpose8x8(pack_bf16x2(a0, a1)), transpose8x8(pack_bf16x2(b0, b1)));
                 }
             }
-            float pm[NR][2 * E];
+            if (i % AHEAD == 0 && __any_sync(0xffffffffu, weigh(i) > kMostF16)) {
+                lower(i);
+                weigh(i);
+            }
+            // codes of channels 4 g .. + 3 of every group, of tokens 2 t, 2 t + 1 (+ 8): 16 bits each
+            uint32_t x[2][G];
 #pragma unroll
-            for (int nr = 0; nr < NR; ++nr)
+            for (int u = 0; u < 2; ++u) {
+                const Words<G> w = lds_words<G>(tile + At::value_half(8 * u + 2 * t, g, 0));
 #pragma unroll
-                for (int e = 0; e < 2 * E; ++e) pm[nr][e] = s[i][nr][e] * mult[nr][e % E];
+                for (int j = 0; j < G; j += 2) {
+                    x[u][j] = __byte_perm(w.w[j / 2], w.w[G / 2 + j / 2], 0x5410);
+                    x[u][j + 1] = __byte_perm(w.w[j / 2], w.w[G / 2 + j / 2], 0x7632);
+                }
+            }
+            const Words<G> va = lds_words<G>(tile + At::value_group(g, 0)), vb = lds_words<G>(tile + At::value_group(g + 8, 0));
 #pragma unroll
             for (int j = 0; j < G; ++j) {
                 uint32_t y[4], z[4];
                 code_operands<VX>(x[0][j], y);
                 code_operands<VX>(x[1][j], z);
-                const float sa = group_scale(va.w[j]), sb = group_scale(vb.w[j]);
 #pragma unroll
                 for (int nr = 0; nr < NR; ++nr) {
                     if constexpr (SPLIT) {
+                        const float sa = group_scale(va.w[j]), sb = group_scale(vb.w[j]);
                         const float ma = fmaf(8.f, sa, group_min(va.w[j])), mb = fmaf(8.f, sb, group_min(vb.w[j]));
 #pragma unroll
                         for (int e = 0; e < E; ++e)
                             omin[nr][e][j] = fmaf(s[i][nr][e], ma, fmaf(s[i][nr][E + e], mb, omin[nr][e][j]));
                     }
-                    const float r0 = pm[nr][0] * sa, r1 = E == 2 ? pm[nr][E - 1] * sa : 0.f;
-                    const float r2 = pm[nr][E] * sb, r3 = E == 2 ? pm[nr][2 * E - 1] * sb : 0.f;
-                    uint32_t b0[NP], b1[NP];
-                    if constexpr (SPLIT) {
-                        split_f16x2(r0, r1, b0[0], b0[NP - 1]);
-                        split_f16x2(r2, r3, b1[0], b1[NP - 1]);
-                    } else {
-                        b0[0] = pack_f16x2(r0, r1);
-                        b1[0] = pack_f16x2(r2, r3);
-                    }
 #pragma unroll
                     for (int np = 0; np < NP; ++np) {
-                        const uint32_t c0_ = transpose8x8(b0[np]), c1_ = transpose8x8(b1[np]);
+                        const uint32_t c0_ = transpose8x8(rw[i % AHEAD][nr][j][0][np]),
+                                       c1_ = transpose8x8(rw[i % AHEAD][nr][j][1][np]);
                         mma_f16(acc[nr][j][0], y[0], y[1], z[0], z[1], c0_, c1_);
                         mma_f16(acc[nr][j][1], y[2], y[3], z[2], z[3], c0_, c1_);
                     }
@@ -899,7 +917,6 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E)) cache_attn_kernel(cons
             const float m = over_g_max(top[nr][e]) * f[nr][e];  // -inf: nothing seen
             const float c = m == -INFINITY ? 0.f : ex2(ref[nr][e] - m);
             const float sum = over_g_sum(l[nr][e]) * c;
-            const float v = pow2_inverse(mult[nr][e]);
             float om[G];
 #pragma unroll
             for (int j = 0; j < G; ++j) {
@@ -911,6 +928,7 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E)) cache_attn_kernel(cons
                 if (g == 0) sml[warp * R + r] = make_float2(m, sum);
 #pragma unroll
                 for (int j = 0; j < G; ++j) {
+                    const float v = pow2_inverse(mult[nr][e][j]);
                     float4 o;
                     o.x = fmaf(acc[nr][j][0][e] * code_unit<VX>(0), v, om[j]) * c;
                     o.y = fmaf(acc[nr][j][0][e + 2] * code_unit<VX>(1), v, om[j]) * c;
@@ -1032,7 +1050,7 @@ Segment segment_of(int64_t rows, int64_t items, int64_t tokens, int start, bool 
     s.rows = 4 * s.e * s.nr;
     s.tiles = (int)ceil_div(rows, s.rows);
     s.units = items * s.tiles * (start + (tokens > UNIT ? ceil_div(tokens, UNIT) : 1));
-    const int64_t held = 148 * held_at(s.nr, s.e), runs = ceil_div(s.units, start + 1);
+    const int64_t held = 148 * held_at(s.nr, s.e, bf16), runs = ceil_div(s.units, start + 1);
     s.grid = runs < held ? runs : held;
     return s;
 }

@@ -175,6 +175,26 @@ def _check(got, want, dtype):
     assert (np.abs(o - eo) <= tol).all(), float((np.abs(o - eo) / np.maximum(tol, 1e-300)).max())
 
 
+def _kept(tiles, length):
+    """((scale, minimum, code) of the keys, of the values) in the bytes of tiles [n, Hkv, 20 D], tokens [length, Hkv, ...].
+    (How append rounds to them is tested to the byte elsewhere.)"""
+    n, h, size = tiles.shape
+    d, g = size // 20, size // 20 // M.GROUP
+    out = []
+    for at, shape in ((0, (16, 4, g, 8)), (10 * d, (2, 8, 8, g, 4))):
+        x = tiles[..., at:at + 8 * d]
+        x = np.stack([x & 15, x >> 4], -1).reshape(n, h, *shape)
+        if at:  # [n, h, half, part, token, group, code] -> [n, half, token, h, group, part, code]
+            x = x.transpose(0, 2, 4, 1, 5, 3, 6)
+        else:  # [n, h, token, part, group, code] -> [n, token, h, group, part, code]
+            x = x.transpose(0, 2, 1, 4, 3, 5)
+        words = np.ascontiguousarray(tiles[..., at + 8 * d:at + 10 * d]).view(np.uint16).reshape(n, h, 16, g, 2)
+        words = (words.astype(np.uint32) << 16).view(np.float32).astype(np.float64).transpose(0, 2, 1, 3, 4)
+        words, x = words.reshape(n * 16, h, g, 2)[:length], x.reshape(n * 16, h, g, M.GROUP)[:length]
+        out.append((words[..., 0], words[..., 1], x.astype(np.int64)))
+    return out
+
+
 def _cache(dev, k, v, page):
     """A pool that holds the sequences k[i], v[i] [length, Hkv, D] (tensors on the device), its table and lengths, and
     what it keeps of them."""
@@ -185,8 +205,9 @@ def _cache(dev, k, v, page):
     tab, zero = _i32(table, dev), _i32([0], dev)
     for i, n in enumerate(lens):
         dbl.relay_cache_append(pool, tab[i:i + 1], zero, k[i][None], v[i][None])
-    kept = [[M.quantise(x.double().cpu().numpy()) for x in y] for y in (k, v)]
-    return pool, tab, _i32(lens, dev), *kept
+    tiles = [pool[tab[i, :-(-n // page)].long()].transpose(1, 2).flatten(0, 1).cpu().numpy() for i, n in enumerate(lens)]
+    kept = [_kept(x, n) for x, n in zip(tiles, lens)]
+    return pool, tab, _i32(lens, dev), [x[0] for x in kept], [x[1] for x in kept]
 
 
 @gpu
@@ -228,6 +249,51 @@ def test_attention_values_near_the_largest(cuda, native_lib, dtype, d):
     pool, tab, held, kk, vv = _cache(cuda, [k], [v], 16)
     q = torch.ones((1, 1, 1, d), device=cuda, dtype=dtype)
     _check(dbl.relay_cache_attention(q, pool, tab, held), _attend(q.double().cpu().numpy(), kk, vv, [t]), dtype)
+    _ok()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("tq,g", [(1, 1), (1, 6), (1, 14), (5, 1)])
+@pytest.mark.parametrize("sizes", [(0, -2, -4, -6), (-1, -3, -5, -7), (0, -8, -10, -12), (3, 3, -20, -25), (-9, 0), (-5, -7)])
+def test_attention_value_groups_of_different_sizes(cuda, native_lib, dtype, tq, g, sizes):
+    """Groups of 32 channels whose values are powers of ten apart: every channel is as exact as its own group allows.
+    Small queries, so that the scores' own error does not hide it."""
+    rng = np.random.default_rng(g + len(sizes))
+    d, hkv, lens = 32 * len(sizes), 2, [300, 33]
+    size = np.repeat(10.0 ** np.array(sizes), 32)
+    k, v = ([torch.as_tensor(rng.standard_normal((n, hkv, d)) * x).to(cuda, F32) for n in lens] for x in (1, size))
+    pool, tab, held, kk, vv = _cache(cuda, k, v, 16)
+    q = torch.as_tensor(rng.standard_normal((2, tq, hkv * g, d)) * 1e-3).to(cuda, dtype)
+    _check(dbl.relay_cache_attention(q, pool, tab, held), _attend(q.double().cpu().numpy(), kk, vv, lens), dtype)
+    _ok()
+
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("g,d", [(1, 128), (3, 64), (7, 128), (16, 64)])
+@pytest.mark.parametrize("prefix,rise", [(0, 0.02), (50, 0.02), (0, -0.02), (50, -0.02), (0, 3.0), (50, 3.0), (0, 400.0),
+                                         (70000, 0.02), (70000, 3.0)])
+def test_attention_scores_that_rise_and_values_that_change(cuda, native_lib, dtype, g, d, prefix, rise):
+    """Scores that rise (or fall) from token to token, up to far past what one power of two of p covers, with value
+    sizes that differ by token and by group, each in its own order."""
+    rng = np.random.default_rng(g + prefix)
+    n, t = 4, 700
+    lens, hkv = [t, 1, 130, 0], 2
+    assert (prefix == 70000) == (n * hkv * prefix >= 1 << 19)  # with a launch of the prefix's own
+    k, v = [], []
+    for x in [prefix] + lens:
+        y = rng.standard_normal((x, hkv, d)) * 1e-2
+        y[..., 0] = (np.arange(x) % t)[:, None] * rise  # channel 0 carries the score
+        z = rng.standard_normal((x, hkv, d // 32, 32)) * 10.0 ** rng.integers(-6, 7, (x, hkv, d // 32, 1))
+        k.append(torch.as_tensor(y).to(cuda, F32)), v.append(torch.as_tensor(z.reshape(x, hkv, d)).to(cuda, F32))
+    pool, tab, held, kk, vv = _cache(cuda, k, v, 64)
+    q = torch.as_tensor(rng.standard_normal((n, 1, hkv * g, d)) * 1e-2)
+    q[..., 0] = d ** 0.5 / torch.arange(1, hkv * g + 1)
+    q = q.to(cuda, dtype)
+    kw = dict(prefix_pages=tab[0], prefix_len=prefix) if prefix else {}
+    want = _attend(q.double().cpu().numpy(), kk[1:], vv[1:], lens, (kk[0], vv[0]) if prefix else (None, None))
+    _check(dbl.relay_cache_attention(q[:, 0], pool, tab[1:], held[1:], **kw), want, dtype)
     _ok()
 
 
