@@ -614,7 +614,9 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E, sizeof(T) == 2)) cache_
     float omin[NR][E][G];    // f32: sum p (min + 8 scale) of this lane's tokens
     float pacc[NR][4];       // bf16: sum p scale, sum p min: lanes g = 2 j, 2 j + 1 hold group j
     float l[NR][E], top[NR][E];      // sums; largest inner score of the lane
-    float ref[NR][E], bar_[NR][E];   // p = 2^(f inner - ref) <= 1; the inner score at which ref is raised
+    // p = 2^(f (inner - ref) - kSlack) <= 1; the inner score at which ref is raised.  The difference comes first: it is
+    // exact near ref, while f ref has a rounding of its own, of any size where the scores are large.
+    float ref[NR][E], bar_[NR][E];
     float mult[NR][E][G];            // r = p scale mult, a power of two for each row and group
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr) {
@@ -757,9 +759,9 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E, sizeof(T) == 2)) cache_
 #pragma unroll
                 for (int e = 0; e < E; ++e) {
                     const float m = over_g_max(top[nr][e]);
-                    const float to = m == -INFINITY ? 0.f : m * f[nr][e] + kSlack;  // so that p stays at most 1
+                    const float to = m == -INFINITY ? 0.f : m;
                     // p, and with it what has been summed, shrinks by c; mult grows by the power of two in it
-                    const float by = bar_[nr][e] == -INFINITY ? 0.f : fminf(to - ref[nr][e], 400.f);
+                    const float by = bar_[nr][e] == -INFINITY ? 0.f : fminf((to - ref[nr][e]) * f[nr][e], 400.f);
                     const float c = ex2(-by), rest = ex2(floorf(by) - by);
                     ref[nr][e] = to;
                     bar_[nr][e] = m + kSlack / f[nr][e];
@@ -784,8 +786,8 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E, sizeof(T) == 2)) cache_
             for (int e = 0; e < E; ++e)
 #pragma unroll
                 for (int i = 0; i < TS; ++i) {
-                    s[i][nr][e] = ex2(fmaf(s[i][nr][e], f[nr][e], -ref[nr][e]));
-                    s[i][nr][E + e] = ex2(fmaf(s[i][nr][E + e], f[nr][e], -ref[nr][e]));
+                    s[i][nr][e] = ex2(fmaf(s[i][nr][e] - ref[nr][e], f[nr][e], -kSlack));
+                    s[i][nr][E + e] = ex2(fmaf(s[i][nr][E + e] - ref[nr][e], f[nr][e], -kSlack));
                     l[nr][e] += s[i][nr][e] + s[i][nr][E + e];
                 }
         // r = p scale mult of AHEAD tiles from i0 on as operands, and the largest of them
@@ -914,8 +916,8 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E, sizeof(T) == 2)) cache_
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const int r = row_at(nr, e);
-            const float m = over_g_max(top[nr][e]) * f[nr][e];  // -inf: nothing seen
-            const float c = m == -INFINITY ? 0.f : ex2(ref[nr][e] - m);
+            const float inner = over_g_max(top[nr][e]), m = inner * f[nr][e];  // -inf: nothing seen
+            const float c = m == -INFINITY ? 0.f : ex2(fmaf(ref[nr][e] - inner, f[nr][e], kSlack));
             const float sum = over_g_sum(l[nr][e]) * c;
             float om[G];
 #pragma unroll

@@ -297,6 +297,41 @@ def test_attention_scores_that_rise_and_values_that_change(cuda, native_lib, dty
     _ok()
 
 
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("exponent", [10, 24, 31, 40, 80, 118])
+@pytest.mark.parametrize("tq,g,prefix", [(1, 1, 0), (1, 7, 40), (3, 4, 0)])
+def test_attention_scores_of_all_sizes(cuda, native_lib, dtype, exponent, tq, g, prefix):
+    """Scores up to 2^118: the largest has the weight 1 (as many times as it occurs), the others what their distance
+    gives, however coarse the scores are."""
+    rng = np.random.default_rng(exponent + g)
+    d, lens = 64, [300, 61]
+    k, v = ([torch.as_tensor(rng.uniform(-1, 1, (n, 2, d))).to(cuda, BF16) for n in [prefix] + lens] for _ in "kv")
+    k[1][200] = k[1][7]  # the same key twice, in the steps of different warps
+    pool, tab, held, kk, vv = _cache(cuda, k, v, 32)
+    q = torch.as_tensor(rng.uniform(-1, 1, (2, tq, 2 * g, d)) * 2.0 ** (exponent // 2)).to(cuda, dtype)
+    q[0, :, 0] = k[1][7, 0].to(dtype) * 2.0 ** (exponent // 2)  # which the query finds
+    scale = 2.0 ** (exponent - exponent // 2)
+    kw = dict(prefix_pages=tab[0], prefix_len=prefix) if prefix else {}
+    got = dbl.relay_cache_attention(q, pool, tab[1:], held[1:], scale=scale, **kw)
+    want = _attend(q.double().cpu().numpy(), kk[1:], vv[1:], lens, (kk[0], vv[0]) if prefix else (None, None), scale)
+    o, mx, sm = (x.double().cpu().numpy().reshape(w.shape) for x, w in zip(got, want))
+    ds = (2 * d + 8) * U32 * want[5]
+    far = ds > 0.1
+    assert (np.abs(mx - want[1]) <= ds + 4 * U32 + U32 * np.abs(want[1])).all()
+    near = torch.as_tensor(~far, device=cuda)
+    _check([x.reshape(w.shape)[near] for x, w in zip(got, want)], [x[~far] for x in want], dtype)
+    # the first rows find one key twice: 2 of its weight, its value rows averaged; with another key as near as the
+    # scores' rounding the weights may differ, so the others are looked at for what every softmax keeps
+    assert np.isfinite(o).all() and (sm >= 1 - 1e-5).all() and (sm <= max(lens) + prefix + 1).all()
+    values = np.concatenate([(x[1][..., None] + x[0][..., None] * x[2]).reshape(-1, 2, d) for x in vv])
+    assert (np.abs(o) <= np.abs(values).max() * (1 + 2.0 ** -7)).all()
+    if exponent >= 31:
+        both = values[prefix + 7] + values[prefix + 200]
+        assert np.allclose(sm[0, :, 0], 2, rtol=1e-6)
+        assert (np.abs(o[0, :, 0] - both[0] / 2) <= 2.0 ** -8 * (np.abs(both[0]) + 15 * max(vv[1][0][7, 0].max(), vv[1][0][200, 0].max()))).all()
+
+
 # ------------------------------------------------------------------------------------------ threads, streams, graphs
 def test_threads_do_not_share_a_workspace(monkeypatch):
     """A call can be two launches that hand results over in its workspace, and the interpreter lock is let go in between:
