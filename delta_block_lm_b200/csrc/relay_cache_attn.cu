@@ -76,6 +76,7 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // Tokens of a segment: tile * tiles_inv has its exact quotient below 2^32 / 256 tiles.
 constexpr int64_t kMostTokens = (int64_t)1 << 27;
 constexpr float kSlack = 8.f;     // how far a score may pass the running maximum (powers of two)
+constexpr int kLift = 32;         // powers of two between the scores of queries from 2^120 on and their f
 constexpr float kMostF16 = 60000.f;             // p scale mult stays below it
 constexpr float kMostMult = 8.507059173e37f;    // 2^126
 constexpr int kMostMultBits = 127 + 126;        // its exponent's bits
@@ -465,7 +466,6 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E, sizeof(T) == 2)) cache_
     // Tokens that the table has no entries for are left out; the queries still count from the length.
     if (!pre && len > most && threadIdx.x == 0) atomicExch(p.err, kCacheErrorPage);
     const int c0 = u0 * UNIT, c1 = min(u1 * UNIT, limit_of(rows - 1));  // later rows see more
-    const int all_see = limit_of(0);                                         // tokens below it need no mask
     const int steps = c1 > c0 ? (c1 - c0 + STEP - 1) / STEP : 0;
     const int mine = steps > warp ? (steps - warp + W - 1) / W : 0;
     const int tile_end = (c1 + kCacheTile - 1) / kCacheTile;
@@ -552,10 +552,13 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E, sizeof(T) == 2)) cache_
     // sums of q over the groups / f as three bf16 parts, in the odd places (the minima's) of the
     // operand for the (scale, minimum) words: group t
     uint32_t qm[NR][3];
-    // the scale goes into f, which stays positive
+    // the scale goes into f, which stays positive.  Where a row's f would leave f32, all rows of the tile take f 2^-kLift
+    // and scores 2^kLift as large, by the path of masked steps.
     const float sign = p.scale > 0.f ? 1.f : p.scale < 0.f ? -1.f : 0.f;
     const float fscale = sign != 0.f ? fabsf(p.scale) * kLog2e : 1.f;
     float f[NR][E];  // of the columns 2 t, 2 t + 1: score = f * inner
+    int fe[NR];      // of column g: f = fscale 2^fe
+    bool lift = false;
 #pragma unroll
     for (int nr = 0; nr < NR; ++nr) {
         float x[G][8];
@@ -579,26 +582,26 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E, sizeof(T) == 2)) cache_
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
         // top < 2^e; q 2^(14 - e) fits f16; score = f inner undoes it and the unit of the codes
         int e = (int)(__float_as_uint(top) >> 23) - 126;
-        e = top == 0.f ? 0 : min(max(e, -90), 110);
+        e = top == 0.f ? 0 : min(max(e, -112), 128);
         const float up = __uint_as_float((uint32_t)(127 + 14 - e) << 23);
         constexpr int unit = KX == Codes::kHigh ? 18 : 20;  // log2 of code_unit<KX>(0)
-        const float fr = __uint_as_float((uint32_t)(127 - 14 + unit + e) << 23) * fscale;
-        const float inv = __uint_as_float((uint32_t)(127 + 14 - unit - e) << 23);
+        fe[nr] = unit - 14 + e;
+        lift = lift || fe[nr] + (int)(__float_as_uint(fscale) >> 23) - 127 >= 126;
         float mine_sum = 0.f;
 #pragma unroll
         for (int j = 0; j < G; ++j) {
             float sum = 0.f;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sum += x[j][i];
+            for (int i = 0; i < 8; ++i) x[j][i] *= up, sum += x[j][i];
             sum += __shfl_xor_sync(0xffffffffu, sum, 1);
             sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            if (t == j) mine_sum = sum * inv;
+            if (t == j) mine_sum = sum / code_unit<KX>(0);
             // the operands of the two products of a group, in the order of code_operands
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float by = up * (code_unit<KX>(i) / code_unit<KX>(0));
-                if constexpr (SPLIT) split_f16x2(x[j][i] * by, x[j][i + 4] * by, qf[nr][0][j][i], qf[nr][NP - 1][j][i]);
-                else qf[nr][0][j][i] = pack_f16x2(x[j][i] * by, x[j][i + 4] * by);
+                static_assert(code_unit<KX>(0) == code_unit<KX>(1), "the keys' codes have one unit");
+                if constexpr (SPLIT) split_f16x2(x[j][i], x[j][i + 4], qf[nr][0][j][i], qf[nr][NP - 1][j][i]);
+                else qf[nr][0][j][i] = pack_f16x2(x[j][i], x[j][i + 4]);
             }
         }
 #pragma unroll
@@ -606,9 +609,15 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E, sizeof(T) == 2)) cache_
             qm[nr][i] = pack_bf16x2(0.f, mine_sum);
             mine_sum -= bf16_hi(qm[nr][i]);
         }
-#pragma unroll
-        for (int e2 = 0; e2 < E; ++e2) f[nr][e2] = __shfl_sync(0xffffffffu, fr, (2 * t + e2) * 4);
     }
+    lift = __any_sync(0xffffffffu, lift);
+#pragma unroll
+    for (int nr = 0; nr < NR; ++nr) {
+        const float fr = ldexpf(fscale, fe[nr] - (lift ? kLift : 0));
+#pragma unroll
+        for (int e = 0; e < E; ++e) f[nr][e] = __shfl_sync(0xffffffffu, fr, (2 * t + e) * 4);
+    }
+    const int clear = lift ? -1 : min(limit_of(0), c1);  // steps that end here need no mask; -1: scores times 2^kLift
 
     float acc[NR][G][2][4];  // [group][channels 4 g + 0, 1 | 2, 3]: (ch 0, row 2t), (0, 2t+1), (1, 2t), (1, 2t+1)
     float omin[NR][E][G];    // f32: sum p (min + 8 scale) of this lane's tokens
@@ -643,10 +652,11 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E, sizeof(T) == 2)) cache_
         const uint32_t have = have_of >> (slot * TS) & ((1u << TS) - 1);
         const int tok0 = c0 + (done * W + warp) * STEP;
         const bool gap = tok0 < lead && tok0 + STEP > lead_end;  // holds the end of the prefix's last tile
-        const bool masked = tok0 + STEP > min(all_see, c1) || have != (1u << TS) - 1 || gap;
+        const bool masked = tok0 + STEP > clear || have != (1u << TS) - 1 || gap;
         if (masked) {  // what the groups of tokens that are not there hold is not a number that may be used
             // Drafted tokens that the tile's first rows do not see: a NaN group of their values would reach those rows as
             // 0 * NaN.  It is put into the sums of the rows that see the token instead.
+            const int all_see = limit_of(0);
             if (LATER && tok0 + STEP > all_see && all_see < c1) {
                 static_assert(STEP == 32, "a lane for each token of a step");
                 const int at = tok0 + lane;
@@ -739,6 +749,7 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E, sizeof(T) == 2)) cache_
                         for (int b = 0; b < 2; ++b) {
                             const int tok = tok0 + i * kCacheTile + g + 8 * b;
                             if (!(have >> i & 1) || tok >= lim || (tok >= lead_end && tok < lead)) s[i][nr][b * E + e] = -INFINITY;
+                            if (clear < 0) s[i][nr][b * E + e] *= (float)(1ll << kLift);
                         }
                 }
         }

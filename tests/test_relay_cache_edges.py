@@ -332,6 +332,36 @@ def test_attention_scores_of_all_sizes(cuda, native_lib, dtype, exponent, tq, g,
         assert (np.abs(o[0, :, 0] - both[0] / 2) <= 2.0 ** -8 * (np.abs(both[0]) + 15 * max(vv[1][0][7, 0].max(), vv[1][0][200, 0].max()))).all()
 
 
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("exponents,k_exponent,scale", [
+    ((90, 111, 112, 118, 121, 123, 125, 126), 0, 2.0 ** -124), ((-112, -118, -122, -125), 112, 0.25),
+    ((127, 120, 112, -3), -60, None), ((126, 126, 124, 3, 126, 122, 117, 111, 126, 125, 126), -8, None)])
+@pytest.mark.parametrize("tq", [1, 3])
+def test_attention_queries_of_all_sizes(cuda, native_lib, dtype, exponents, k_exponent, scale, tq):
+    """Queries of 2^-125 to the largest that the type holds, where the scores are finite."""
+    rng = np.random.default_rng(len(exponents))
+    d, lens, h = 64, [200, 40], len(exponents)
+    k, v = ([torch.as_tensor(rng.uniform(-1, 1, (n, 1, d)) * x).to(cuda, F32) for n in lens] for x in (2.0 ** k_exponent, 1))
+    pool, tab, held, kk, vv = _cache(cuda, k, v, 32)
+    q = rng.uniform(-1, 1, (2, tq, h, d)) * 2.0 ** np.array(exponents)[:, None]
+    q[..., 1, 5] = np.sign(q[..., 1, 5]) * 1.9 * 2.0 ** exponents[1]
+    q = torch.as_tensor(q).to(cuda, dtype)
+    want = _attend(q.double().cpu().numpy(), kk, vv, lens, scale=scale)
+    assert np.abs(want[5]).max() < 2.0 ** 127
+    got = dbl.relay_cache_attention(q, pool, tab, held, scale=scale)
+    # where the scores' rounding is as large as their softmax resolves, one key has all of the weight
+    ds = (2 * d + 8) * U32 * want[5]
+    far, near = ds > 0.1, torch.as_tensor(ds <= 0.1, device=cuda)
+    assert (want[2][far] < 1 + 1e-6).all()
+    _check([x.reshape(w.shape)[near] for x, w in zip(got, want)], [x[~far] for x in want], dtype)
+    o, mx, _ = (x.double().cpu().numpy().reshape(w.shape) for x, w in zip(got, want))
+    assert (np.abs(mx - want[1])[far] <= (ds + U32 * np.abs(want[1]))[far]).all()
+    tol = (2.0 ** -8 if dtype == BF16 else 2.0 ** -20) * (np.abs(want[0]) + want[3])
+    assert (np.abs(o - want[0])[far] <= tol[far]).all()
+    _ok()
+
+
 # ------------------------------------------------------------------------------------------ threads, streams, graphs
 def test_threads_do_not_share_a_workspace(monkeypatch):
     """A call can be two launches that hand results over in its workspace, and the interpreter lock is let go in between:
