@@ -92,7 +92,7 @@ struct AttnParams {
     int N, Tq, H, group, prefix_len, prefix_width;
     float scale;
     uint32_t tiles_inv;  // ceil(2^32 / tiles of a page), 0 for 1: tile / tiles is the high word of a product
-    bool pre;       // this launch: the prefix, or the sequences' own tokens
+    bool pre;       // this launch: the prefix, or the sequences' own tokens (PRE on the device)
     int lead;       // tokens of the prefix's tiles where the sequences' launch reads them itself, 0 where not
     int tiles;      // row tiles: of a kv head over all sequences, or of a kv head and sequence
     int pre_tiles, pre_rows, pre_units, pre_run, pre_parts;  // the prefix: row tiles of a head, rows of a tile, units,
@@ -354,7 +354,8 @@ constexpr int rows_of_tile() { return NR * 4 * E; }
 
 // LATER: a row tile's rows may see different numbers of keys (several queries a sequence).  Without it single tokens save
 // the registers of that case: 131072 tokens 79.6 us, with it 81.5; 64 sequences after a prefix 82.2 and 84 us.
-template <int D, typename T, int NR, int E, bool LATER>
+// PRE: the prefix's launch, likewise (as a parameter of the launch 88.0 us for 85.3).
+template <int D, typename T, int NR, int E, bool LATER, bool PRE>
 __global__ void __launch_bounds__(W * 32, held_at(NR, E, sizeof(T) == 2)) cache_attn_kernel(const AttnParams p) {
     constexpr int R = rows_of_tile<NR, E>();
     using L = AttnLayout<D, T, R>;
@@ -375,7 +376,7 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E, sizeof(T) == 2)) cache_
     int* serr = sint;
     uint8_t* ring = smem + warp * NS * L::STAGE;
     const int TG = p.Tq * p.group, HT = p.c.heads * p.tiles;
-    const bool pre = p.pre;
+    constexpr bool pre = PRE;
     if (lane == 0)
         for (int i = 0; i < NS; ++i) mbar_init(bar + i, 1);
     if (threadIdx.x == 0) *serr = 0;
@@ -1122,13 +1123,13 @@ int attn_validate(const dbl_relay_cache_attention_args* a) {
     return DBL_OK;
 }
 
-template <int D, typename T, int NR, int E, bool LATER>
+template <int D, typename T, int NR, int E, bool LATER, bool PRE>
 int launch_with(const AttnParams& p, int64_t grid, cudaStream_t st) {
     constexpr int smem = AttnLayout<D, T, rows_of_tile<NR, E>()>::BYTES;
     static std::atomic<uint64_t> done{0};
     const int rc = once_per_device(done, [] {
         return cuda_status(
-            cudaFuncSetAttribute(cache_attn_kernel<D, T, NR, E, LATER>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
+            cudaFuncSetAttribute(cache_attn_kernel<D, T, NR, E, LATER, PRE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
             "relay cache attention: cudaFuncSetAttribute");
     });
     if (rc != DBL_OK) return rc;
@@ -1143,12 +1144,13 @@ int launch_with(const AttnParams& p, int64_t grid, cudaStream_t st) {
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = p.pre_units && !p.pre ? 1 : 0;
-    return cuda_status(cudaLaunchKernelEx(&cfg, cache_attn_kernel<D, T, NR, E, LATER>, p), "cache_attn_kernel");
+    return cuda_status(cudaLaunchKernelEx(&cfg, cache_attn_kernel<D, T, NR, E, LATER, PRE>, p), "cache_attn_kernel");
 }
 
 template <int D, typename T, int NR, int E>
 int launch_attn(const AttnParams& p, int64_t grid, cudaStream_t st) {
-    return p.Tq > 1 && !p.pre ? launch_with<D, T, NR, E, true>(p, grid, st) : launch_with<D, T, NR, E, false>(p, grid, st);
+    if (p.pre) return launch_with<D, T, NR, E, false, true>(p, grid, st);
+    return p.Tq > 1 ? launch_with<D, T, NR, E, true, false>(p, grid, st) : launch_with<D, T, NR, E, false, false>(p, grid, st);
 }
 
 template <int D>
