@@ -95,7 +95,7 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(CT, 1) cache_releas
     }
 }
 
-// a = parents, b = children (empty sequences, each named once, none of them a parent).
+// a = parents, b = children (each named once, none of them a parent), which give back the pages that they hold.
 template <int CL>
 __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(CT, 1) cache_fork_kernel(const PageParams p) {
     constexpr int NT = CL * CT;
@@ -109,7 +109,8 @@ __global__ void __cluster_dims__(CL, 1, 1) __launch_bounds__(CT, 1) cache_fork_k
         }
         const int len = ld(p.lengths_out + from);
         const int page = (int64_t)w * p.page < len ? ld(p.table_out + entry(p, from, w)) : -1;
-        p.table_out[entry(p, to, w)] = page;
+        const int old = atomicExch(p.table_out + entry(p, to, w), page);  // reserve may have given it pages
+        if (old >= 0 && old < p.P) atomicSub(p.refs_out + old, 1);
         if (page >= 0 && page < p.P) atomicAdd(p.refs_out + page, 1);
         if (w == 0) p.lengths_out[to] = len;
     }

@@ -318,8 +318,8 @@ def relay_cache_release(pool, page_table, lengths, refs, sequences, *, out=None)
 
 
 def relay_cache_fork(pool, page_table, lengths, refs, parents, children, *, out=None):
-    """children[i] (an empty sequence, named once and no parent itself) continues from parents[i],
-    sharing its pages.  Returns (page_table, lengths, refs)."""
+    """children[i] (named once and no parent itself) continues from parents[i], sharing its pages; the
+    pages that it held are given back.  Returns (page_table, lengths, refs)."""
     parents, children = _list("parents", parents), _list("children", children)
     if parents.shape != children.shape:
         raise ValueError("relay cache fork: parents and children must have the same length")

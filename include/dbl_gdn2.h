@@ -504,8 +504,8 @@ size_t dbl_relay_cache_pages_workspace_bytes(int64_t pages, int64_t n_seq);
  * entry holds it. */
 int dbl_relay_cache_release(const dbl_relay_cache_pages_args *args, const int32_t *sequences,
                             int64_t count, dbl_stream_t stream);
-/* children[i] (an empty sequence, named once, not itself a parent) becomes a copy of parents[i]
- * that shares its pages; pages reserved past the parent's length stay the parent's alone. */
+/* children[i] (named once, not itself a parent) becomes a copy of parents[i] that shares its pages, and
+ * gives back those that it held; pages reserved past the parent's length stay the parent's alone. */
 int dbl_relay_cache_fork(const dbl_relay_cache_pages_args *args, const int32_t *parents,
                          const int32_t *children, int64_t count, dbl_stream_t stream);
 /* Gives every sequence the pages for its next counts[n] tokens (counts NULL: `tokens` each) and

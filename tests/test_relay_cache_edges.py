@@ -123,6 +123,30 @@ def test_a_cut_fork_leaves_the_other_sequence_alone(cuda, native_lib, cut, more)
     _ok()
 
 
+@gpu
+def test_fork_into_a_row_that_holds_pages(cuda, native_lib):
+    """A sequence without tokens that reserve has given pages, or one with tokens: fork gives the pages back."""
+    pool = dbl.relay_cache_pool(8, 1, 64, 16, device=cuda)
+    state = [torch.full((3, 4), -1, device=cuda, dtype=torch.int32), _i32([0, 0, 0], cuda), _i32([0] * 8, cuda)]
+    table, refs, _ = dbl.relay_cache_reserve(pool, *state, _i32([20, 33, 1], cuda))
+    assert refs.tolist() == [1, 1, 1, 1, 1, 1, 0, 0]
+    for out in (False, True):
+        state = [table.clone(), _i32([20, 0, 0], cuda), refs.clone()]
+        got = dbl.relay_cache_fork(pool, *state, _i32([0, 0], cuda), _i32([1, 2], cuda), out=state if out else None)
+        assert got[0].tolist() == [[0, 1, -1, -1]] * 3 and got[1].tolist() == [20, 20, 20]
+        assert got[2].tolist() == [3, 3, 0, 0, 0, 0, 0, 0]
+    # a child that held tokens of its own
+    state = [table.clone(), _i32([20, 33, 1], cuda), refs.clone()]
+    got = dbl.relay_cache_fork(pool, *state, _i32([0], cuda), _i32([1], cuda))
+    assert got[0].tolist() == [[0, 1, -1, -1], [0, 1, -1, -1], [5, -1, -1, -1]] and got[1].tolist() == [20, 20, 1]
+    assert got[2].tolist() == [2, 2, 0, 0, 0, 1, 0, 0]
+    # a child that held the parent's own page already
+    state = [_i32([[0, 1], [1, -1]], cuda), _i32([20, 0], cuda), _i32([1, 2, 0, 0, 0, 0, 0, 0], cuda)]
+    got = dbl.relay_cache_fork(pool, *state, _i32([0], cuda), _i32([1], cuda))
+    assert got[0].tolist() == [[0, 1], [0, 1]] and got[2].tolist() == [2, 2, 0, 0, 0, 0, 0, 0]
+    _ok()
+
+
 # ------------------------------------------------------------------------------------------ attention
 def _attend(q, kk, vv, lens, pre=(None, None), scale=None):
     """The model's result and, for each row and channel, sum p (|minimum| + 8 scale) / l and max p scale / l of what the
