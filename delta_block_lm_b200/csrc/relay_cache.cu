@@ -171,8 +171,12 @@ __global__ void __launch_bounds__(256) cache_append_tiles_kernel(const AppendPar
     const int64_t n = tn;
     const int count = p.counts ? min(max(p.counts[n], 0), p.T) : p.T, len = p.lengths[n];
     if (p.new_lengths && ti == 0 && h0 == 0 && threadIdx.x == 0) p.new_lengths[n] = len + count;
+    if (len < 0) {  // as single tokens: those at positions below zero are left out, and said to be
+        if (count > 0 && threadIdx.x == 0) atomicExch(p.err, kCacheErrorPage);
+        if (len <= -p.T) return;
+    }
     const int tl = max(len, 0) / kCacheTile + ti, t0 = tl * kCacheTile - len;  // token of place 0
-    if (t0 >= count || len < 0) return;
+    if (t0 >= count) return;
     const int page = cache_page(p.c, n, tl);
     if (page < 0) {
         if (threadIdx.x == 0) atomicExch(p.err, kCacheErrorPage);

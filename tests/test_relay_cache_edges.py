@@ -147,6 +147,26 @@ def test_fork_into_a_row_that_holds_pages(cuda, native_lib):
     _ok()
 
 
+# ------------------------------------------------------------------------------------------ append and read
+@gpu
+@pytest.mark.parametrize("length", [-1, -3, -31, -100, -2 ** 31])
+def test_append_at_a_negative_length_is_recorded(cuda, native_lib, length):
+    """A call of many tokens does what single tokens do: those at negative positions are left out and recorded."""
+    rng = np.random.default_rng(4)
+    h, d, page, t = 2, 64, 16, 40
+    k, v = (torch.as_tensor(rng.standard_normal((2, t, h, d))).to(cuda, BF16) for _ in "kv")
+    tab = _i32([[0, 1, 2], [3, 4, 5]], cuda)
+    pools = [dbl.relay_cache_pool(6, h, d, page, device=cuda) for _ in "ab"]
+    dbl.relay_cache_append(pools[0], tab, _i32([length, 3], cuda), k, v)
+    assert _device_code() == 102
+    for i in range(t):
+        dbl.relay_cache_append(pools[1], tab, _i32([length + i, 3 + i], cuda), k[:, i:i + 1], v[:, i:i + 1])
+        assert (_device_code() == 102) == (length + i < 0)
+    assert torch.equal(*pools)
+    dbl.relay_cache_append(pools[0], tab, _i32([length, 3], cuda), k, v, counts=_i32([0, 1], cuda))
+    _ok()
+
+
 # ------------------------------------------------------------------------------------------ attention
 def _attend(q, kk, vv, lens, pre=(None, None), scale=None):
     """The model's result and, for each row and channel, sum p (|minimum| + 8 scale) / l and max p scale / l of what the
