@@ -314,17 +314,19 @@ __global__ void __launch_bounds__(256) cache_read_tiles_kernel(const ReadParams 
     const unsigned b = blockIdx.x / hg, tn = b / p.tiles;
     const int h0 = (int)(blockIdx.x - b * hg) * kTileHeads, h1 = min(h0 + kTileHeads, p.c.heads), ti = (int)(b - tn * p.tiles);
     const int64_t n = tn;
-    const int first = p.start ? p.start[n] : 0, len = p.lengths[n];
-    const int tl = (first >= 0 ? first / kCacheTile : -((-first + kCacheTile - 1) / kCacheTile)) + ti;
-    const int t0 = tl * kCacheTile - first;  // token of place 0
+    const int len = p.lengths[n];
+    static_assert(kCacheTile == 16, "positions shift by 4");
+    const int64_t first = p.start ? p.start[n] : 0;     // positions may pass 32 bits where the start is far out
+    const int64_t tl = (first >> 4) + ti;               // rounded down
+    const int t0 = (int)(tl * kCacheTile - first);      // token of place 0
     if (t0 >= p.T) return;
     const bool any = tl >= 0 && tl * kCacheTile < len;
-    const int page = any ? cache_page(p.c, n, tl) : -1;
+    const int page = any ? cache_page(p.c, n, (int)tl) : -1;
     if (any && page < 0 && threadIdx.x == 0) atomicExch(p.err, kCacheErrorPage);
     const int i = threadIdx.x, hp = i / (2 * D), which = i / D % 2, k = i / LPT % kCacheTile, part = i % LPT;
     const int t = t0 + k, j = part / 2, q = part % 2;
     const bool wanted = t >= 0 && t < p.T, held = page >= 0 && first + t < len;
-    const uint8_t* from = cache_tile<D>(p.c, max(page, 0), h0, max(tl, 0) % p.c.tiles);
+    const uint8_t* from = cache_tile<D>(p.c, max(page, 0), h0, any ? (int)tl % p.c.tiles : 0);
     const int64_t per = (int64_t)p.c.tiles * TB;  // from head to head
     if (page >= 0) {
         const int words = (h1 - h0) * WORDS;

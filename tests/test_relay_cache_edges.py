@@ -167,6 +167,21 @@ def test_append_at_a_negative_length_is_recorded(cuda, native_lib, length):
     _ok()
 
 
+@gpu
+def test_read_that_starts_far_past_the_end(cuda, native_lib):
+    """Zeros and no error, whatever the number of tokens, up to the last position that 32 bits hold."""
+    pool, tab, held, _, _ = _fill(cuda, np.random.default_rng(0), [40, 3], 1, 64, 16)
+    for start in (48, 2 ** 31 - 1, 2 ** 31 - 17, 2 ** 31 - 40):
+        for tokens in (1, 70):
+            k, v = dbl.relay_cache_read(pool, tab, held, start=_i32([start, start], cuda), tokens=tokens, dtype=F32)
+            assert not k.any() and not v.any()
+            _ok()
+    for tokens in (5, 70):  # and far before the beginning
+        k, v = dbl.relay_cache_read(pool, tab, held, start=_i32([-2 ** 31, -2 ** 31 + 9], cuda), tokens=tokens, dtype=F32)
+        assert not k.any() and not v.any()
+        _ok()
+
+
 # ------------------------------------------------------------------------------------------ attention
 def _attend(q, kk, vv, lens, pre=(None, None), scale=None):
     """The model's result and, for each row and channel, sum p (|minimum| + 8 scale) / l and max p scale / l of what the
