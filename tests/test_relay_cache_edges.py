@@ -503,3 +503,101 @@ def test_two_threads_on_one_stream(cuda, native_lib):
     _ok()
 
 
+@gpu
+@pytest.mark.parametrize("prefix", [37, 20000])
+def test_a_serving_loop_in_a_graph(cuda, native_lib, prefix):
+    """Release, fork, reserve, append, attention, read and compact captured as one graph that updates its state in place:
+    every replay gives what the same calls give outside a graph, from the same state."""
+    rng = np.random.default_rng(prefix)
+    n, hkv, d, page = 14, 2, 64, 16
+    assert (prefix == 20000) == (n * hkv * prefix >= 1 << 19)  # with a launch of the prefix's own
+    width = -(-prefix // page)
+    pool = dbl.relay_cache_pool(width + 12 * n, hkv, d, page, device=cuda)
+    pool.fill_(255)
+    table = torch.full((n + 1, width + 8), -1, device=cuda, dtype=torch.int32)  # the last row: the shared prompt
+    state = [table, _i32([0] * (n + 1), cuda), _i32([0] * len(pool), cuda)]
+
+    def write(pool, state, counts, k, v, out=False):
+        table, refs, missing = dbl.relay_cache_reserve(pool, *state, counts, out=(state[0], state[2]) if out else None)
+        lengths = dbl.relay_cache_append(pool, table, state[1], k, v, counts=counts, out=state[1] if out else None)
+        return [table, lengths, refs], missing
+
+    def tokens(t):
+        return [torch.as_tensor(rng.standard_normal((n + 1, t, hkv, d))).to(cuda, BF16) for _ in "kv"]
+
+    state, missing = write(pool, state, _i32([0] * n + [prefix], cuda), *tokens(prefix))
+    state, missing = write(pool, state, _i32([20 + i for i in range(n)] + [0], cuda), *tokens(40))
+    assert missing.tolist() == [0]
+    # the inputs of a step, which the graph reads where they are
+    gone, parents = _i32([0, 0], cuda), _i32([0, 0], cuda)
+    counts, q = _i32([1] * n + [0], cuda), torch.zeros((n, 3 * hkv, d), device=cuda, dtype=BF16)
+    k, v = tokens(1)
+
+    def step(pool, state, out):
+        state = list(dbl.relay_cache_release(pool, *state, gone, out=state if out else None))
+        state = list(dbl.relay_cache_fork(pool, *state, parents, gone, out=state if out else None))
+        state, missing = write(pool, state, counts, k, v, out)
+        got = dbl.relay_cache_attention(q, pool, state[0][:n], state[1][:n], prefix_pages=state[0][n], prefix_len=prefix)
+        back = dbl.relay_cache_read(pool, state[0], state[1], tokens=50, dtype=F32)
+        table, refs, used = dbl.relay_cache_compact(pool, state[0], state[2], out=(state[0], state[2]) if out else None)
+        return [table, state[1], refs], [*got, *back, missing, used]
+
+    gone.copy_(_i32([1, 5], cuda)), parents.copy_(_i32([3, 3], cuda))
+    step(pool.clone(), [x.clone() for x in state], True)  # everything is loaded before the capture
+    torch.cuda.synchronize()
+    graph, kept, kept_pool = torch.cuda.CUDAGraph(), [x.clone() for x in state], pool.clone()
+    with torch.cuda.graph(graph):
+        after, outputs = step(kept_pool, kept, True)
+    for _ in range(12):
+        two = rng.permutation(n)[:4]
+        gone.copy_(_i32(two[:2], cuda)), parents.copy_(_i32(two[2:], cuda))
+        q.copy_(torch.as_tensor(rng.standard_normal(q.shape)))
+        for x, y in zip((k, v), tokens(1)):
+            x.copy_(y)
+        graph.replay()
+        state, want = step(pool, state, False)
+        assert all(torch.equal(a, b) for a, b in zip(outputs, want))
+        assert all(torch.equal(a, b) for a, b in zip(after, state)) and torch.equal(kept_pool, pool)
+        assert outputs[-2].tolist() == [0] and torch.isfinite(outputs[0]).all()
+    _ok()
+
+
+@gpu
+def test_two_streams_at_once(cuda, native_lib):
+    """Reserve with copies, compact and attention on two streams at the same time, each on its own state."""
+    rng = np.random.default_rng(12)
+    jobs = []
+    for i in range(2):
+        n, hkv, d, page, pages = 40, 4, 128, 32, 4600
+        pool = torch.randint(0, 200, (pages, hkv, page // 16, 20 * d), device=cuda, dtype=torch.uint8)
+        pool[..., 8 * d:10 * d] = 1  # scales and minima that are numbers
+        pool[..., 18 * d:] = 1
+        m = Pages(np.full((n, 60), -1), rng.integers(1, 1500, n), np.zeros(pages, int), page)
+        order = list(rng.permutation(pages))
+        for s in range(0, n, 2):
+            for w in range(-(-m.lengths[s] // page)):
+                m.table[s, w] = order.pop()
+                m.refs[m.table[s, w]] = 1
+            m.lengths[s + 1] = 0
+        m.fork(range(0, n, 2), range(1, n, 2))
+        q = torch.as_tensor(rng.standard_normal((n, 8, d))).to(cuda, BF16)
+        jobs.append((pool, _three(m, cuda), q, torch.cuda.Stream()))
+
+    def run(pool, state, q):
+        p = pool.clone()
+        table, refs, missing = dbl.relay_cache_reserve(p, *state, 40)
+        table, refs, used = dbl.relay_cache_compact(p, table, refs)
+        return [p, table, refs, missing, used, *dbl.relay_cache_attention(q, p, table, state[1])]
+
+    want = [run(*job[:3]) for job in jobs]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        got = [None, None]
+        for i, (pool, state, q, stream) in enumerate(jobs):
+            with torch.cuda.stream(stream):
+                got[i] = run(pool, state, q)
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for x, y in zip(got, want) for a, b in zip(x, y))
+    _ok()
+
+
