@@ -378,17 +378,6 @@ bool grid_for(int64_t n_seq, int64_t tokens, int64_t heads, int D, int per, int&
     return ctas <= 0x7fffffff;
 }
 
-int check_table(const int32_t* table, int64_t n_seq, int64_t width, int64_t stride, const char* what) {
-    if (n_seq <= 0) return fail(DBL_ERR_INVALID_ARGUMENT, "%s: n_seq must be positive", what);
-    if (width <= 0 || stride < 0 || (stride && stride < width))
-        return fail(DBL_ERR_INVALID_ARGUMENT, "%s: the page table needs a positive width and a row stride of at least it",
-                    what);
-    if (n_seq > 0x7fffffff || width > 0x7fffffff)
-        return fail(DBL_ERR_UNSUPPORTED, "%s: sizes exceed 32-bit limits", what);
-    if (!table) return fail(DBL_ERR_INVALID_ARGUMENT, "%s: page_table is required", what);
-    return DBL_OK;
-}
-
 }  // namespace
 
 int cache_validate(const dbl_relay_cache* c, const char* what) {
@@ -407,7 +396,14 @@ int cache_validate(const dbl_relay_cache* c, const char* what) {
 }
 
 int cache_check_table(const int32_t* table, int64_t n_seq, int64_t width, int64_t stride, const char* what) {
-    return check_table(table, n_seq, width, stride, what);
+    if (n_seq <= 0) return fail(DBL_ERR_INVALID_ARGUMENT, "%s: n_seq must be positive", what);
+    if (width <= 0 || stride < 0 || (stride && stride < width))
+        return fail(DBL_ERR_INVALID_ARGUMENT, "%s: the page table needs a positive width and a row stride of at least it",
+                    what);
+    if (n_seq > 0x7fffffff || width > 0x7fffffff)
+        return fail(DBL_ERR_UNSUPPORTED, "%s: sizes exceed 32-bit limits", what);
+    if (!table) return fail(DBL_ERR_INVALID_ARGUMENT, "%s: page_table is required", what);
+    return DBL_OK;
 }
 
 }  // namespace dbl
@@ -417,7 +413,7 @@ extern "C" int dbl_relay_cache_append(const dbl_relay_cache_append_args* a, dbl_
     if (!a) return fail(DBL_ERR_INVALID_ARGUMENT, "relay cache append: null args");
     int rc = cache_validate(&a->cache, "relay cache append");
     if (rc == DBL_OK)
-        rc = check_table(a->page_table, a->n_seq, a->table_width, a->table_stride, "relay cache append");
+        rc = cache_check_table(a->page_table, a->n_seq, a->table_width, a->table_stride, "relay cache append");
     if (rc != DBL_OK) return rc;
     if (a->tokens <= 0) return fail(DBL_ERR_INVALID_ARGUMENT, "relay cache append: tokens must be positive");
     if (a->dtype != DBL_F32 && a->dtype != DBL_BF16)
@@ -470,7 +466,7 @@ extern "C" int dbl_relay_cache_read(const dbl_relay_cache_read_args* a, dbl_stre
     using namespace dbl;
     if (!a) return fail(DBL_ERR_INVALID_ARGUMENT, "relay cache read: null args");
     int rc = cache_validate(&a->cache, "relay cache read");
-    if (rc == DBL_OK) rc = check_table(a->page_table, a->n_seq, a->table_width, a->table_stride, "relay cache read");
+    if (rc == DBL_OK) rc = cache_check_table(a->page_table, a->n_seq, a->table_width, a->table_stride, "relay cache read");
     if (rc != DBL_OK) return rc;
     if (a->tokens <= 0) return fail(DBL_ERR_INVALID_ARGUMENT, "relay cache read: tokens must be positive");
     if (a->dtype != DBL_F32 && a->dtype != DBL_BF16)

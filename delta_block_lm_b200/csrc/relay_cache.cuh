@@ -58,8 +58,9 @@ struct TileAt {
 __device__ __forceinline__ float group_scale(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float group_min(uint32_t w) { return __uint_as_float(w & 0xFFFF0000u); }
 
-// Checks what a call says of its pool; `what` names the call.
+// Check what a call says of its pool and of its page table; `what` names the call.
 int cache_validate(const dbl_relay_cache* c, const char* what);
+int cache_check_table(const int32_t* table, int64_t n_seq, int64_t width, int64_t stride, const char* what);
 
 inline CacheView cache_view(const dbl_relay_cache* c, const int32_t* table, int64_t width, int64_t stride) {
     CacheView v;

@@ -15,8 +15,6 @@
 
 namespace dbl {
 
-int cache_check_table(const int32_t* table, int64_t n_seq, int64_t width, int64_t stride, const char* what);
-
 namespace {
 
 constexpr int CT = 1024;             // threads of a CTA
