@@ -350,10 +350,8 @@ constexpr int held_at(int nr, int e, bool bf16) { return nr == 2 ? 2 : e == 2 ||
 template <int NR, int E>
 constexpr int rows_of_tile() { return NR * 4 * E; }
 
-// LATER: a row tile's rows may see different numbers of keys (several queries a sequence).  Without it single tokens save
-// the registers of that case: 131072 tokens 79.6 us, with it 81.5; 64 sequences after a prefix 82.2 and 84 us.
-// PRE: the prefix's launch, likewise (as a parameter of the launch 88.0 us for 85.3).
-template <int D, typename T, int NR, int E, bool LATER, bool PRE>
+// PRE: the prefix's launch.  As a parameter of the launch it cost registers: 64 sequences after a prefix 88.0 us for 85.3.
+template <int D, typename T, int NR, int E, bool PRE>
 __global__ void __launch_bounds__(W * 32, held_at(NR, E, sizeof(T) == 2)) cache_attn_kernel(const AttnParams p) {
     constexpr int R = rows_of_tile<NR, E>();
     using L = AttnLayout<D, T, R>;
@@ -656,7 +654,7 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E, sizeof(T) == 2)) cache_
             // Drafted tokens that the tile's first rows do not see: a NaN group of their values would reach those rows as
             // 0 * NaN.  It is put into the sums of the rows that see the token instead.
             const int all_see = limit_of(0);
-            if (LATER && tok0 + STEP > all_see && all_see < c1) {
+            if (tok0 + STEP > all_see && all_see < c1) {
                 static_assert(STEP == 32, "a lane for each token of a step");
                 const int at = tok0 + lane;
                 const bool asked = at >= all_see && at < c1 && (have >> (lane / kCacheTile) & 1);
@@ -1121,13 +1119,13 @@ int attn_validate(const dbl_relay_cache_attention_args* a) {
     return DBL_OK;
 }
 
-template <int D, typename T, int NR, int E, bool LATER, bool PRE>
+template <int D, typename T, int NR, int E, bool PRE>
 int launch_with(const AttnParams& p, int64_t grid, cudaStream_t st) {
     constexpr int smem = AttnLayout<D, T, rows_of_tile<NR, E>()>::BYTES;
     static std::atomic<uint64_t> done{0};
     const int rc = once_per_device(done, [] {
         return cuda_status(
-            cudaFuncSetAttribute(cache_attn_kernel<D, T, NR, E, LATER, PRE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
+            cudaFuncSetAttribute(cache_attn_kernel<D, T, NR, E, PRE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
             "relay cache attention: cudaFuncSetAttribute");
     });
     if (rc != DBL_OK) return rc;
@@ -1142,13 +1140,12 @@ int launch_with(const AttnParams& p, int64_t grid, cudaStream_t st) {
     attr.val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = &attr;
     cfg.numAttrs = p.pre_units && !p.pre ? 1 : 0;
-    return cuda_status(cudaLaunchKernelEx(&cfg, cache_attn_kernel<D, T, NR, E, LATER, PRE>, p), "cache_attn_kernel");
+    return cuda_status(cudaLaunchKernelEx(&cfg, cache_attn_kernel<D, T, NR, E, PRE>, p), "cache_attn_kernel");
 }
 
 template <int D, typename T, int NR, int E>
 int launch_attn(const AttnParams& p, int64_t grid, cudaStream_t st) {
-    if (p.pre) return launch_with<D, T, NR, E, false, true>(p, grid, st);
-    return p.Tq > 1 ? launch_with<D, T, NR, E, true, false>(p, grid, st) : launch_with<D, T, NR, E, false, false>(p, grid, st);
+    return p.pre ? launch_with<D, T, NR, E, true>(p, grid, st) : launch_with<D, T, NR, E, false>(p, grid, st);
 }
 
 template <int D>
