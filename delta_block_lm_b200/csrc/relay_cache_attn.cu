@@ -360,9 +360,6 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E, sizeof(T) == 2)) cache_
     constexpr bool SPLIT = sizeof(T) == 4;
     constexpr int NP = SPLIT ? 2 : 1;  // f16 parts of q and of p
     constexpr int PER = 16 / sizeof(T);
-    // Tiles whose p scale is looked over at once: one vote a step costs the operands' registers, which one row a lane
-    // leaves (131072 tokens 80.2 us, with a vote a tile 81.1); 16 rows spill with it (six drafts 40.5 us for 35.3).
-    constexpr int AHEAD = !SPLIT && NR * E == 1 ? TS : 1;
     constexpr Codes KX = SPLIT ? Codes::kHigh : Codes::kMid, VX = Codes::kCentred;
     extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -798,57 +795,51 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E, sizeof(T) == 2)) cache_
                     s[i][nr][E + e] = ex2(fmaf(s[i][nr][E + e] - ref[nr][e], f[nr][e], -kSlack));
                     l[nr][e] += s[i][nr][e] + s[i][nr][E + e];
                 }
-        // r = p scale mult of AHEAD tiles from i0 on as operands, and the largest of them
-        uint32_t rw[AHEAD][NR][G][2][NP];  // tokens g and g + 8
-        auto weigh = [&](int i0) {
+        // r = p scale mult of tile i as operands, and the largest of them
+        uint32_t rw[NR][G][2][NP];  // tokens g and g + 8
+        auto weigh = [&](int i) {
+            const uint8_t* tile = st + i * L::TB;
+            const Words<G> va = lds_words<G>(tile + At::value_group(g, 0)), vb = lds_words<G>(tile + At::value_group(g + 8, 0));
             float most = 0.f;
 #pragma unroll
-            for (int k = 0; k < AHEAD; ++k) {
-                const uint8_t* tile = st + (i0 + k) * L::TB;
-                const Words<G> va = lds_words<G>(tile + At::value_group(g, 0)), vb = lds_words<G>(tile + At::value_group(g + 8, 0));
+            for (int j = 0; j < G; ++j) {
+                const float sa = group_scale(va.w[j]), sb = group_scale(vb.w[j]);
 #pragma unroll
-                for (int j = 0; j < G; ++j) {
-                    const float sa = group_scale(va.w[j]), sb = group_scale(vb.w[j]);
+                for (int nr = 0; nr < NR; ++nr) {
+                    float ra[2] = {0.f, 0.f}, rb[2] = {0.f, 0.f};
 #pragma unroll
-                    for (int nr = 0; nr < NR; ++nr) {
-                        float ra[2] = {0.f, 0.f}, rb[2] = {0.f, 0.f};
-#pragma unroll
-                        for (int e = 0; e < E; ++e) {
-                            ra[e] = s[i0 + k][nr][e] * sa * mult[nr][e][j];
-                            rb[e] = s[i0 + k][nr][E + e] * sb * mult[nr][e][j];
-                            most = max3(most, ra[e], rb[e]);
-                        }
-                        if constexpr (SPLIT) {
-                            split_f16x2(ra[0], ra[1], rw[k][nr][j][0][0], rw[k][nr][j][0][NP - 1]);
-                            split_f16x2(rb[0], rb[1], rw[k][nr][j][1][0], rw[k][nr][j][1][NP - 1]);
-                        } else {
-                            rw[k][nr][j][0][0] = pack_f16x2(ra[0], ra[1]);
-                            rw[k][nr][j][1][0] = pack_f16x2(rb[0], rb[1]);
-                        }
+                    for (int e = 0; e < E; ++e) {
+                        ra[e] = s[i][nr][e] * sa * mult[nr][e][j];
+                        rb[e] = s[i][nr][E + e] * sb * mult[nr][e][j];
+                        most = max3(most, ra[e], rb[e]);
+                    }
+                    if constexpr (SPLIT) {
+                        split_f16x2(ra[0], ra[1], rw[nr][j][0][0], rw[nr][j][0][NP - 1]);
+                        split_f16x2(rb[0], rb[1], rw[nr][j][1][0], rw[nr][j][1][NP - 1]);
+                    } else {
+                        rw[nr][j][0][0] = pack_f16x2(ra[0], ra[1]);
+                        rw[nr][j][1][0] = pack_f16x2(rb[0], rb[1]);
                     }
                 }
             }
             return most;
         };
-        auto lower = [&](int i0) {  // mult of the rows and groups whose r left f16's range
+        auto lower = [&](int i) {  // mult of the rows and groups whose r left f16's range
+            const uint8_t* tile = st + i * L::TB;
+            const Words<G> va = lds_words<G>(tile + At::value_group(g, 0)), vb = lds_words<G>(tile + At::value_group(g + 8, 0));
 #pragma unroll
-            for (int k = 0; k < AHEAD; ++k) {
-                const uint8_t* tile = st + (i0 + k) * L::TB;
-                const Words<G> va = lds_words<G>(tile + At::value_group(g, 0)), vb = lds_words<G>(tile + At::value_group(g + 8, 0));
+            for (int nr = 0; nr < NR; ++nr)
 #pragma unroll
-                for (int nr = 0; nr < NR; ++nr)
+                for (int e = 0; e < E; ++e)
 #pragma unroll
-                    for (int e = 0; e < E; ++e)
+                    for (int j = 0; j < G; ++j) {
+                        const float w = fmaxf(s[i][nr][e] * group_scale(va.w[j]), s[i][nr][E + e] * group_scale(vb.w[j]));
+                        const float m = fminf(mult[nr][e][j], mult_for(over_g_max(w)));
+                        const float c = pow2_inverse(mult[nr][e][j]) * m;
+                        mult[nr][e][j] = m;
 #pragma unroll
-                        for (int j = 0; j < G; ++j) {
-                            const float w = fmaxf(s[i0 + k][nr][e] * group_scale(va.w[j]), s[i0 + k][nr][E + e] * group_scale(vb.w[j]));
-                            const float m = fminf(mult[nr][e][j], mult_for(over_g_max(w)));
-                            const float c = pow2_inverse(mult[nr][e][j]) * m;
-                            mult[nr][e][j] = m;
-#pragma unroll
-                            for (int x = e; x < 8; x += 2) acc[nr][j][x / 4][x % 4] *= c;
-                        }
-            }
+                        for (int x = e; x < 8; x += 2) acc[nr][j][x / 4][x % 4] *= c;
+                    }
         };
 #pragma unroll
         for (int i = 0; i < TS; ++i) {
@@ -866,7 +857,7 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E, sizeof(T) == 2)) cache_
                     mma_bf16(pacc[nr], w, transpose8x8(pack_bf16x2(a0, a1)), transpose8x8(pack_bf16x2(b0, b1)));
                 }
             }
-            if (i % AHEAD == 0 && __any_sync(0xffffffffu, weigh(i) > kMostF16)) {
+            if (__any_sync(0xffffffffu, weigh(i) > kMostF16)) {
                 lower(i);
                 weigh(i);
             }
@@ -898,8 +889,7 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E, sizeof(T) == 2)) cache_
                     }
 #pragma unroll
                     for (int np = 0; np < NP; ++np) {
-                        const uint32_t c0_ = transpose8x8(rw[i % AHEAD][nr][j][0][np]),
-                                       c1_ = transpose8x8(rw[i % AHEAD][nr][j][1][np]);
+                        const uint32_t c0_ = transpose8x8(rw[nr][j][0][np]), c1_ = transpose8x8(rw[nr][j][1][np]);
                         mma_f16(acc[nr][j][0], y[0], y[1], z[0], z[1], c0_, c1_);
                         mma_f16(acc[nr][j][1], y[2], y[3], z[2], z[3], c0_, c1_);
                     }
