@@ -304,7 +304,7 @@ __global__ void __launch_bounds__(256) cache_read_kernel(const ReadParams p) {
 
 // Runs of tokens: a CTA reads one tile of positions for kTileHeads heads, all of them at once in 16-byte
 // words to shared memory.  One thread: 16 channels of one token's key or value.  The prompts above (84 MB in,
-// 268 MB out): 66.5 us = 5300 GB/s, 81% of the measured copy rate; one tile at a time took 79 us.
+// 268 MB out): 64.5 us = 5450 GB/s, 83% of the measured copy rate; one tile at a time took 79 us.
 template <int D, typename T>
 __global__ void __launch_bounds__(256) cache_read_tiles_kernel(const ReadParams p) {
     using At = TileAt<D>;

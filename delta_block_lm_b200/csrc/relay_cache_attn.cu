@@ -38,18 +38,22 @@
 // tokens, and the units of all items, one after another, are dealt to the CTAs that the GPU holds in
 // equal runs, whatever the lengths are: a CTA finds its run in the lengths, so the host does not need
 // them.  A CTA's four warps take turns at steps of 32 tokens, each with a ring of its own that bulk
-// copies fill (tcgen05 would need 64 or 128 query rows to a tile, and a kernel with it holds an SM
-// alone).  An item that one CTA holds whole is finished there; the others' sums go to the workspace,
-// and the CTA that arrives last at an item joins them.  The prefix's launch comes before the
-// sequences', which starts beside it and joins its sums to every item's.
+// copies fill (tcgen05 needs 64 or 128 query rows to a tile, which only the rows of all sequences at a
+// shared prefix make).  An item that one CTA holds whole is finished there; the others' sums go to the
+// workspace, and the CTA that arrives last at an item joins them.  The prefix's launch comes before the
+// sequences', which joins its sums to every item's and may start before it has ended: its CTAs come up
+// as the prefix's leave (those of 16 rows hold an SM's registers two by two, so the two launches take
+// 30 and 55 us alone and 85 together; what is saved is the gap between them).
 //
 // Bound: the codes' way from memory to operand.  131072 tokens of one sequence, 16 heads of 128 (336
-// MB): 79 us = 4240 GB/s, 65% of the measured copy rate; 358 instructions a warp and tile of 16 tokens,
-// issue slots 61% and ALU 54% busy (LOP3, shifts and byte permutes; a tile needs 64 + 32 + 8 of them).
-// The slope is 83% of the copy rate (131072 to 262144 tokens); the rest is some 20 us of starts, joins
-// and an uneven end.  Tried and slower: 3 and 5 CTAs an SM, steps of 16 and 64 tokens, rings of 1, 3
-// and 4 stages, CTAs of 2 and 8 warps, the next item's copies before this one's sums are joined
-// (registers), shifts as high products.
+// MB): 80.8 us = 4150 GB/s, 63% of the measured copy rate; 356 instructions a warp and tile of 16 tokens,
+// issue slots 60% and ALU 54% busy (LOP3, shifts and byte permutes; a tile needs 64 + 32 + 8 of them).
+// The slope is 79% of the copy rate (131072 to 262144 tokens); the rest is some 16 us of starts, joins
+// and an uneven end.  CTAs of 2 and 8 warps instead of 4: 131072 tokens 91 and 79 us for 82, 64 sequences after
+// a prefix 83.6 and 92 for 85.7, 48 ragged 47 and 48.6 for 43.2, six drafts 37.7 and 38.3 for 35; a rule by
+// shape is not taken.  Tried in an earlier build and slower: 3 and 5 CTAs an SM, steps of 16 and 64 tokens,
+// rings of 1, 3 and 4 stages, the next item's copies before this one's sums are joined (registers), shifts as
+// high products.
 #include <float.h>
 
 #include "relay_cache.cuh"
@@ -345,7 +349,7 @@ struct AttnLayout {
 // NR groups of 8 columns; E = 2: a row in every column, E = 1 (up to 4 rows): in the even columns only,
 // which saves the arithmetic of the others (a lane holds two neighbouring columns of every product).
 // CTAs that an SM holds, by the registers that a tile's sums and operands take.  f32 rows, up to 4 of them, at 3 and 4
-// CTAs: one sequence of 100000 tokens, 16 heads of 128, 83.9 and 99.5 us, 16 of 500 to 4000 tokens 49 and 57 us.
+// CTAs: one sequence of 100000 tokens, 16 heads of 128, 83.6 and 97 us, 16 of 500 to 4000 tokens 49 and 55 us.
 constexpr int held_at(int nr, int e, bool bf16) { return nr == 2 ? 2 : e == 2 || !bf16 ? 3 : 4; }
 template <int NR, int E>
 constexpr int rows_of_tile() { return NR * 4 * E; }
@@ -1044,7 +1048,8 @@ struct Segment {  // the prefix, or the sequences' own tokens
 Segment segment_of(int64_t rows, int64_t items, int64_t tokens, int start, bool bf16) {
     Segment s{};
     s.e = rows <= 4 ? 1 : 2;
-    // two groups of columns share the codes' operands: 16 rows of 48 sequences 64 us, in two tiles of 8 70 us (f32 rows
+    // two groups of columns share the codes' operands: 16 rows of 48 sequences 67 us, in two tiles of 8 73 us; 12 rows (six
+    // drafts of two heads) 35 us both ways; the prefix of 64 sequences 85.7 and 83.9 us with what follows it (f32 rows
     // take the registers twice)
     s.nr = bf16 && rows > 8 ? 2 : 1;
     s.rows = 4 * s.e * s.nr;
@@ -1066,10 +1071,10 @@ Plan plan_of(const dbl_relay_cache_attention_args* a) {
     const int64_t TG = a->queries * (a->heads / a->cache.kv_heads), H = a->cache.kv_heads, N = a->n_seq;
     const bool bf16 = a->dtype == DBL_BF16;
     const size_t row = (size_t)(a->cache.head_dim + kPartPad) * 4;
-    // A prefix has a launch of its own (about 12 us) where reading it with every sequence's own tokens costs more.
-    // Measured at 16 heads of 128, 1024 own tokens, apart and with them: 64 sequences, prefix 512: 67 and 66 us, 1024:
-    // 68 and 80, 4096: 82 and 172; 16 sequences, 512: 30 and 26, 1024: 31 and 30, 4096: 34 and 52; 4 sequences, 4096:
-    // 23 and 22.
+    // A prefix has a launch of its own where reading it with every sequence's own tokens costs more.  Measured at 16
+    // heads of 128, 1024 own tokens, apart and with them: 64 sequences, prefix 512: 70 and 69 us, 1024: 71 and 85, 4096:
+    // 85 and 183; 16 sequences, 512: 30 and 27, 1024: 31 and 31.6, 4096: 35 and 55; 4 sequences, 1024: 18 and 17, 4096:
+    // 23.6 and 22.6.
     const bool apart = N >= 4 && N * H * a->prefix_len >= kApart;
     L.lead = a->prefix_len > 0 && !apart ? (int)(ceil_div(a->prefix_len, kCacheTile) * kCacheTile) : 0;
     L.own = segment_of(TG, N * H, L.lead + a->table_width * a->cache.page_size, kStart, bf16);

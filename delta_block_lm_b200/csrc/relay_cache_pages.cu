@@ -19,9 +19,8 @@ namespace {
 
 constexpr int CT = 1024;             // threads of a CTA
 constexpr int MOST_WARPS = 8 * CT / 32;
-// Table entries and pages that one CTA deals with.  Measured, release + fork + reserve: 8 sequences (100
-// entries and pages) 15 us by one CTA, 23 us by eight; 32 sequences (2 K) 21 and 26 us; 256 sequences (14 K)
-// 73 and 36 us.
+// Table entries and pages that one CTA deals with.  Measured, release + fork + reserve, by one CTA and by eight: 8
+// sequences (74 entries and pages) and 32 (308) 18 and 25 us, 256 (14 K) 71 and 35 us.
 constexpr int64_t kSmallState = 4096;
 
 struct PageParams {

@@ -9,7 +9,7 @@ The state is four tensors that the caller owns:
 
     pool        uint8 [pages, kv_heads, page_size / 16, 20 head_dim] (``relay_cache_pool``)
     page_table  int32 [sequences, width]: each sequence's pages in order, -1 where it has none
-    lengths     int32 [sequences]: tokens held
+    lengths     int32 [sequences]: tokens held; lowering one drops a sequence's last tokens
     refs        int32 [pages]: how many entries of the page table hold a page (0: free)
 
 The pool is written in place; calls that change the page table, lengths or refs return new tensors
