@@ -19,7 +19,9 @@
 //     lowest four bits it would be 14 to 18: an error of 1e-6 in the sums of small calls); for f32 rows the
 //     codes go to the top of the mantissa (code * 2^-18, 20 to 24 bits).  The values' codes become normal
 //     numbers around zero (code - 8), so that long sums neither drop bits nor cancel:
-//     o = sum r (code - 8) + sum p (min + 8 scale), r the rounded p scale.
+//     o = sum r (code - 8) + sum p (min + 8 scale), r the rounded p scale.  For f32 rows it is code - 7.5, the
+//     codes' mean, for two shifts more: the sums truncate, and half a scale a token that grows in one of them
+//     and is taken off in the other left an error of 2e-5 after 90000 tokens (now 1e-6).
 //   * q is held in f16 relative to a power of two of its own row (bf16 q: exact; f32 q: two f16
 //     parts, 22 bits), p scale in f16 relative to a power of two near the largest of its row and group of
 //     channels (f32: again two parts), so that a group of small values is as exact as one of large ones.
@@ -206,7 +208,7 @@ __device__ __forceinline__ float pow2(int e) {  // 0 below 2^-126; e < 128
 
 // The operand registers of the 8 codes of w, codes (0, 4), (1, 5), (2, 6), (3, 7), and what they are
 // multiplied by to be the codes (code_unit).
-enum class Codes { kMid, kHigh, kCentred };
+enum class Codes { kMid, kHigh, kCentred, kHalf };
 // (x & mask) | bits in one instruction, which takes one constant: the other one stays in a register.
 __device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {
     uint32_t r;
@@ -221,6 +223,11 @@ __device__ __forceinline__ void code_operands(uint32_t w, uint32_t (&r)[4]) {
     } else if constexpr (C == Codes::kMid) {
         r[0] = (w << 4) & 0x00F000F0u, r[1] = w & 0x00F000F0u;
         r[2] = (w >> 4) & 0x00F000F0u, r[3] = (w >> 8) & 0x00F000F0u;
+    } else if constexpr (C == Codes::kHalf) {  // 1144 = 1024 + 16 * 7.5
+        r[0] = and_or(w << 4, 0x00F000F0u, 0x64006400u), r[1] = and_or(w, 0x00F000F0u, 0x64006400u);
+        r[2] = and_or(w >> 4, 0x00F000F0u, 0x64006400u), r[3] = and_or(w >> 8, 0x00F000F0u, 0x64006400u);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) asm("add.rn.f16x2 %0, %0, %1;" : "+r"(r[i]) : "r"(0xE478E478u));
     } else {  // 1024 + x is the f16 with mantissa x; 1032 = 1024 + 8, 1152 = 1024 + 16 * 8
         const uint32_t v = w >> 8;
         r[0] = and_or(w, 0x000F000Fu, 0x64006400u), r[1] = and_or(w, 0x00F000F0u, 0x64006400u);
@@ -232,7 +239,7 @@ __device__ __forceinline__ void code_operands(uint32_t w, uint32_t (&r)[4]) {
 }
 template <Codes C>
 constexpr float code_unit(int i) {
-    return C == Codes::kHigh ? 262144.f : C == Codes::kMid ? 1048576.f : i & 1 ? 0.0625f : 1.f;
+    return C == Codes::kHigh ? 262144.f : C == Codes::kMid ? 1048576.f : C == Codes::kHalf || i & 1 ? 0.0625f : 1.f;
 }
 
 // The operand whose rows are the 2 G scales and minima of a tile's tokens (scale 0, minimum 0, scale 1,
@@ -349,7 +356,7 @@ struct AttnLayout {
 // NR groups of 8 columns; E = 2: a row in every column, E = 1 (up to 4 rows): in the even columns only,
 // which saves the arithmetic of the others (a lane holds two neighbouring columns of every product).
 // CTAs that an SM holds, by the registers that a tile's sums and operands take.  f32 rows, up to 4 of them, at 3 and 4
-// CTAs: one sequence of 100000 tokens, 16 heads of 128, 83.6 and 97 us, 16 of 500 to 4000 tokens 49 and 55 us.
+// CTAs: one sequence of 100000 tokens, 16 heads of 128, 84.5 and 99 us, 16 of 500 to 4000 tokens 49.5 and 56 us.
 constexpr int held_at(int nr, int e, bool bf16) { return nr == 2 ? 2 : e == 2 || !bf16 ? 3 : 4; }
 template <int NR, int E>
 constexpr int rows_of_tile() { return NR * 4 * E; }
@@ -364,7 +371,7 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E, sizeof(T) == 2)) cache_
     constexpr bool SPLIT = sizeof(T) == 4;
     constexpr int NP = SPLIT ? 2 : 1;  // f16 parts of q and of p
     constexpr int PER = 16 / sizeof(T);
-    constexpr Codes KX = SPLIT ? Codes::kHigh : Codes::kMid, VX = Codes::kCentred;
+    constexpr Codes KX = SPLIT ? Codes::kHigh : Codes::kMid, VX = SPLIT ? Codes::kHalf : Codes::kCentred;
     extern __shared__ __align__(128) uint8_t smem[];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     uint64_t* bar = reinterpret_cast<uint64_t*>(smem + L::OFF_BAR) + warp * NS;
@@ -618,7 +625,7 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E, sizeof(T) == 2)) cache_
     const int clear = lift ? -1 : min(limit_of(0), c1);  // steps that end here need no mask; -1: scores times 2^kLift
 
     float acc[NR][G][2][4];  // [group][channels 4 g + 0, 1 | 2, 3]: (ch 0, row 2t), (0, 2t+1), (1, 2t), (1, 2t+1)
-    float omin[NR][E][G];    // f32: sum p (min + 8 scale) of this lane's tokens
+    float omin[NR][E][G];    // f32: sum p (min + 7.5 scale) of this lane's tokens
     float pacc[NR][4];       // bf16: sum p scale, sum p min: lanes g = 2 j, 2 j + 1 hold group j
     float l[NR][E], top[NR][E];      // sums; largest inner score of the lane
     // p = 2^(f (inner - ref) - kSlack) <= 1; the inner score at which ref is raised.  The difference comes first: it is
@@ -886,7 +893,7 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E, sizeof(T) == 2)) cache_
                 for (int nr = 0; nr < NR; ++nr) {
                     if constexpr (SPLIT) {
                         const float sa = group_scale(va.w[j]), sb = group_scale(vb.w[j]);
-                        const float ma = fmaf(8.f, sa, group_min(va.w[j])), mb = fmaf(8.f, sb, group_min(vb.w[j]));
+                        const float ma = fmaf(7.5f, sa, group_min(va.w[j])), mb = fmaf(7.5f, sb, group_min(vb.w[j]));
 #pragma unroll
                         for (int e = 0; e < E; ++e)
                             omin[nr][e][j] = fmaf(s[i][nr][e], ma, fmaf(s[i][nr][E + e], mb, omin[nr][e][j]));

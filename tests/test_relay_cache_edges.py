@@ -421,6 +421,24 @@ def test_attention_queries_of_all_sizes(cuda, native_lib, dtype, exponents, k_ex
     _ok()
 
 
+@gpu
+@pytest.mark.parametrize("d,g", [(64, 7), (128, 1)])
+def test_attention_long_sums_of_f32_rows(cuda, native_lib, d, g):
+    """95000 tokens whose values average out, ten sequences on the same pages, so that one warp sums 34 steps: the result
+    is small beside its terms, and no term of one sign may grow in a sum that drops bits.  A warp adds 136 times
+    (34 steps of 2 tiles and 2 parts), each time dropping at most 2^-23 of a sum, half of it on average."""
+    rng = np.random.default_rng(d)
+    n, hkv, t = 10, 2, 95000
+    k, v = (torch.as_tensor(rng.standard_normal((t, hkv, d))).to(cuda, BF16) for _ in "kv")
+    pool, tab, held, kk, vv = _cache(cuda, [k], [v], 64)
+    q = torch.as_tensor(rng.standard_normal((n, 1, hkv * g, d)) * 0.05).to(cuda, F32)
+    got = dbl.relay_cache_attention(q, pool, tab.expand(n, -1).contiguous(), held.expand(n).contiguous())
+    want = _attend(q.double().cpu().numpy(), kk * n, vv * n, [t] * n)
+    err = got[0].double().cpu().numpy() - want[0]
+    assert np.linalg.norm(err) <= 136 * 2.0 ** -24 * np.linalg.norm(want[0])
+    _ok()
+
+
 # ------------------------------------------------------------------------------------------ threads, streams, graphs
 def test_threads_do_not_share_a_workspace(monkeypatch):
     """A call can be two launches that hand results over in its workspace, and the interpreter lock is let go in between:
