@@ -58,6 +58,8 @@
 // high products.
 #include <float.h>
 
+#include <algorithm>
+
 #include "relay_cache.cuh"
 #include "tc_ptx.cuh"
 
@@ -73,6 +75,9 @@ constexpr int UNIT = W * STEP;    // tokens of a unit
 constexpr int64_t kApart = 1 << 19;  // sequences x kv heads x tokens of a prefix with a launch of its own
 constexpr int kStart = 3;         // units that the start and end of an item cost (about 6 us, a unit 2 us)
 constexpr int kCounterBytes = DBL_RELAY_CACHE_COUNTER_BYTES;
+// Units of a run.  16 f32 sequences of 131072 tokens whose values average out, 16 heads of 128, are off by 2.5e-5 of the
+// result in runs of 443 units and by 7e-6 in runs of 148; 1048576 tokens, 16 heads, 700 us by one round and 708 by three.
+constexpr int kRun = 128;
 constexpr int WIN = 32 / TS;      // steps whose page numbers the lanes of a warp hold
 constexpr int kCacheWaitFull = 40;  // wait-site code (dbl_device_error)
 constexpr int kNoPage = -1, kPast = -2;
@@ -120,6 +125,11 @@ __device__ __forceinline__ void mma_f16_zero(float (&c)[4], uint32_t a0, uint32_
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
         : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+__device__ __forceinline__ void mma_bf16_zero(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};\n"
+        : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
@@ -626,7 +636,9 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E, sizeof(T) == 2)) cache_
 
     float acc[NR][G][2][4];  // [group][channels 4 g + 0, 1 | 2, 3]: (ch 0, row 2t), (0, 2t+1), (1, 2t), (1, 2t+1)
     float omin[NR][E][G];    // f32: sum p (min + 7.5 scale) of this lane's tokens
-    float pacc[NR][4];       // bf16: sum p scale, sum p min: lanes g = 2 j, 2 j + 1 hold group j
+    // bf16: sum p scale, sum p min: lanes g = 2 j, 2 j + 1 hold group j.  They grow with every token and are taken from
+    // each other, so they are added up in f32 (a step's in the tensor cores, whose sums truncate).
+    float pacc[NR][E];
     float l[NR][E], top[NR][E];      // sums; largest inner score of the lane
     // p = 2^(f (inner - ref) - kSlack) <= 1; the inner score at which ref is raised.  The difference comes first: it is
     // exact near ref, while f ref has a rounding of its own, of any size where the scores are large.
@@ -639,10 +651,8 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E, sizeof(T) == 2)) cache_
 #pragma unroll
             for (int i = 0; i < 8; ++i) acc[nr][j][i / 4][i % 4] = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) pacc[nr][i] = 0.f;
-#pragma unroll
         for (int e = 0; e < E; ++e) {
-            l[nr][e] = ref[nr][e] = 0.f;
+            l[nr][e] = ref[nr][e] = pacc[nr][e] = 0.f;
             top[nr][e] = bar_[nr][e] = -INFINITY;
 #pragma unroll
             for (int j = 0; j < G; ++j) omin[nr][e][j] = 0.f, mult[nr][e][j] = kMostMult;
@@ -852,6 +862,7 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E, sizeof(T) == 2)) cache_
                         for (int x = e; x < 8; x += 2) acc[nr][j][x / 4][x % 4] *= c;
                     }
         };
+        float pstep[NR][4];  // the step's part of pacc
 #pragma unroll
         for (int i = 0; i < TS; ++i) {
             const uint8_t* tile = st + i * L::TB;
@@ -862,10 +873,14 @@ __global__ void __launch_bounds__(W * 32, held_at(NR, E, sizeof(T) == 2)) cache_
                 for (int nr = 0; nr < NR; ++nr) {
                     float a0 = s[i][nr][0], a1 = E == 2 ? s[i][nr][E - 1] : 0.f, b0 = s[i][nr][E], b1 = E == 2 ? s[i][nr][2 * E - 1] : 0.f;
                     const uint32_t ha = pack_bf16x2(a0, a1), hb = pack_bf16x2(b0, b1);
-                    mma_bf16(pacc[nr], w, transpose8x8(ha), transpose8x8(hb));
+                    if (i == 0) mma_bf16_zero(pstep[nr], w, transpose8x8(ha), transpose8x8(hb));
+                    else mma_bf16(pstep[nr], w, transpose8x8(ha), transpose8x8(hb));
                     a0 -= bf16_lo(ha), b0 -= bf16_lo(hb);
                     if constexpr (E == 2) a1 -= bf16_hi(ha), b1 -= bf16_hi(hb);
-                    mma_bf16(pacc[nr], w, transpose8x8(pack_bf16x2(a0, a1)), transpose8x8(pack_bf16x2(b0, b1)));
+                    mma_bf16(pstep[nr], w, transpose8x8(pack_bf16x2(a0, a1)), transpose8x8(pack_bf16x2(b0, b1)));
+                    if (i == TS - 1)
+#pragma unroll
+                        for (int e = 0; e < E; ++e) pacc[nr][e] += pstep[nr][e];
                 }
             }
             if (__any_sync(0xffffffffu, weigh(i) > kMostF16)) {
@@ -1062,8 +1077,11 @@ Segment segment_of(int64_t rows, int64_t items, int64_t tokens, int start, bool 
     s.rows = 4 * s.e * s.nr;
     s.tiles = (int)ceil_div(rows, s.rows);
     s.units = items * s.tiles * (start + (tokens > UNIT ? ceil_div(tokens, UNIT) : 1));
+    // As many CTAs as the GPU holds, in more rounds of them where a run would be longer than kRun units, as far as the
+    // counters go: the tensor cores' sums truncate, and each is a run's.
     const int64_t held = 148 * held_at(s.nr, s.e, bf16), runs = ceil_div(s.units, start + 1);
-    s.grid = runs < held ? runs : held;
+    const int64_t rounds = std::min(ceil_div(s.units, held * kRun), (int64_t)kCounterBytes / 4 / held);
+    s.grid = std::min(runs, held * rounds);
     return s;
 }
 

@@ -439,6 +439,27 @@ def test_attention_long_sums_of_f32_rows(cuda, native_lib, d, g):
     _ok()
 
 
+@gpu
+def test_attention_long_sums_of_bf16_rows(cuda, native_lib):
+    """16 sequences on the same 131072 tokens, whose values average out: beside the rounding of the output to bf16 there is
+    the rounding of p scale to f16 (a tenth of it) and no more, however many steps a warp sums (443 in one run)."""
+    torch.manual_seed(1)
+    n, t, h, d, page = 16, 131072, 16, 64, 64
+    pool = dbl.relay_cache_pool(t // page, h, d, page, device=cuda)
+    tab, held = torch.randperm(t // page, device=cuda).to(torch.int32)[None], _i32([0], cuda)
+    for _ in range(8):
+        k, v = (torch.randn(1, t // 8, h, d, device=cuda) for _ in "kv")
+        held = dbl.relay_cache_append(pool, tab, held, k, v)
+    q = (torch.randn(n, h, d, device=cuda) * 0.05).bfloat16()
+    o, _, _ = dbl.relay_cache_attention(q, pool, tab.expand(n, -1).contiguous(), held.expand(n).contiguous())
+    k, v = dbl.relay_cache_read(pool, tab, held, tokens=t, dtype=F32)
+    for a in (0, 7, 15):
+        p = torch.softmax(q[:, a].double() @ k[0, :, a].double().T * d ** -0.5, -1)
+        want = p @ v[0, :, a].double()
+        assert (o[:, a].double() - want).norm() <= 1.1 * (want.bfloat16().double() - want).norm()
+    _ok()
+
+
 # ------------------------------------------------------------------------------------------ threads, streams, graphs
 def test_threads_do_not_share_a_workspace(monkeypatch):
     """A call can be two launches that hand results over in its workspace, and the interpreter lock is let go in between:
