@@ -22,8 +22,8 @@
 //     o = sum r (code - 8) + sum p (min + 8 scale), r the rounded p scale.  For f32 rows it is code - 7.5, the
 //     codes' mean, for two shifts more: the sums truncate, and half a scale a token that grows in one of them
 //     and is taken off in the other left an error of 2e-5 after 90000 tokens (now 1e-6).
-//   * q is held in f16 relative to a power of two of its own row (bf16 q: exact; f32 q: two f16
-//     parts, 22 bits), p scale in f16 relative to a power of two near the largest of its row and group of
+//   * q is held in f16 relative to a power of two of its own row (bf16 q: exact down to 2^-31 of the row's
+//     largest; f32 q: two f16 parts, 22 bits down to 2^-17 of it, then fewer), p scale in f16 relative to a power of two near the largest of its row and group of
 //     channels (f32: again two parts), so that a group of small values is as exact as one of large ones.
 //   * the minima are operands as they lie in memory: a token's (scale, minimum) words are the bf16
 //     pairs of a row, met by zeros in the scales' places (keys), or read by a transposing ldmatrix
@@ -45,12 +45,12 @@
 // workspace, and the CTA that arrives last at an item joins them.  The prefix's launch comes before the
 // sequences', which joins its sums to every item's and may start before it has ended: its CTAs come up
 // as the prefix's leave (those of 16 rows hold an SM's registers two by two, so the two launches take
-// 30 and 55 us alone and 85 together; what is saved is the gap between them).
+// 30 and 54 us alone and 85 together; what is saved is the gap between them).
 //
 // Bound: the codes' way from memory to operand.  131072 tokens of one sequence, 16 heads of 128 (336
-// MB): 80.8 us = 4150 GB/s, 63% of the measured copy rate; 356 instructions a warp and tile of 16 tokens,
+// MB): 81.8 us = 4100 GB/s, 63% of the measured copy rate; 363 instructions a warp and tile of 16 tokens,
 // issue slots 60% and ALU 54% busy (LOP3, shifts and byte permutes; a tile needs 64 + 32 + 8 of them).
-// The slope is 79% of the copy rate (131072 to 262144 tokens); the rest is some 16 us of starts, joins
+// The slope is 78% of the copy rate (131072 to 262144 tokens); the rest is some 16 us of starts, joins
 // and an uneven end.  CTAs of 2 and 8 warps instead of 4: 131072 tokens 91 and 79 us for 82, 64 sequences after
 // a prefix 83.6 and 92 for 85.7, 48 ragged 47 and 48.6 for 43.2, six drafts 37.7 and 38.3 for 35; a rule by
 // shape is not taken.  Tried in an earlier build and slower: 3 and 5 CTAs an SM, steps of 16 and 64 tokens,
